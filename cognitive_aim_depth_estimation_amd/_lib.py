@@ -61,6 +61,18 @@ SIGNATURES = {
     "cogaim_heatmap_postprocess": [P, P, I, I, I, P],
     "cogaim_curiosity_sample": [P, P, P, P, P, LL, P, P, I, I, I, P],
     "cogaim_curiosity_finish": [P, P, LL, P, P, P, P, P, P, P, P, P, I, I, I, P],
+    "cogaim_layernorm_train_fwd": [P, I, LL, P, P, P, I, LL, P, P, P, P, I, I, F, P],
+    "cogaim_layernorm_bwd_workspace_bytes": [I, I],
+    "cogaim_layernorm_bwd": [P, I, LL, P, I, LL, P, P, P, P, P, P, I, LL, P, I, LL, P, P, I, I, P, LL, P],
+    "cogaim_pack8": [P, I, LL, P, P, I, I, P],
+    "cogaim_unpack8": [P, P, P, I, LL, I, I, I, P],
+    "cogaim_activation_bwd": [P, I, LL, P, P, P, I, LL, I, I, I, P],
+    "cogaim_linear_fwd_workspace_bytes": [P],
+    "cogaim_linear_fwd": [P, P, LL, P],
+    "cogaim_linear_bwd_input_workspace_bytes": [P],
+    "cogaim_linear_bwd_input": [P, P, LL, P],
+    "cogaim_linear_bwd_weight_workspace_bytes": [P],
+    "cogaim_linear_bwd_weight": [P, P, LL, P],
 }
 
 
@@ -76,6 +88,27 @@ class MlpChainDesc(C.Structure):
                 ("in0", P), ("in0_ld", LL), ("in0_part_stride", LL),
                 ("in1", P), ("in1_ld", LL), ("in1_len", I), ("in1_off", I),
                 ("scale", P), ("out", P), ("out_ld", LL), ("out_len", I), ("out_off", I)]
+
+
+class LinearFwdDesc(C.Structure):
+    """cogaim_linear_fwd_desc of include/cogaim.h."""
+    _fields_ = ([(n, P) for n in ("x", "w", "bias", "scale", "residual", "y", "codes", "exponents")]
+                + [(n, LL) for n in ("ldx", "ldw", "ldr", "ldy")]
+                + [(n, I) for n in ("M", "N", "K", "dtype", "residual_dtype", "y_dtype", "activation", "reserved")])
+
+
+class LinearBwdInputDesc(C.Structure):
+    """cogaim_linear_bwd_input_desc of include/cogaim.h."""
+    _fields_ = ([(n, P) for n in ("dy", "w", "scale", "codes", "exponents", "dx", "a")]
+                + [(n, LL) for n in ("lddy", "ldw", "lddx", "lda")]
+                + [(n, I) for n in ("M", "N", "K", "dtype", "dx_dtype", "activation")])
+
+
+class LinearBwdWeightDesc(C.Structure):
+    """cogaim_linear_bwd_weight_desc of include/cogaim.h."""
+    _fields_ = ([(n, P) for n in ("dy", "x", "codes", "exponents", "x_scale", "x_shift", "w", "bias", "scale", "dw", "db", "ds")]
+                + [(n, LL) for n in ("lddy", "ldx", "ldw", "lddw")]
+                + [(n, I) for n in ("M", "N", "K", "dtype", "dw_dtype", "reserved")])
 
 
 def mlp_chain(layers, in0, in0_ld, in0_len, out, out_ld, out_len, out_off, B, in0_off=0, in0_parts=1, in0_part_stride=0,
@@ -96,6 +129,10 @@ OPTIONAL = {"cogaim_set_gemm_algo": [I]}
 
 _NO_STATUS = {"cogaim_version", "cogaim_host_pointer_ok", "cogaim_gemm_workspace_bytes", "cogaim_focal_colsum_rows", "cogaim_weighted_tokens_rows",
               "cogaim_focal_rowstats_parts", "cogaim_focal_scores_colsum_blocks"}
+# results in bytes (or -22): 64 bits wide
+_BYTES = {"cogaim_gemm_workspace_bytes", "cogaim_layernorm_bwd_workspace_bytes", "cogaim_linear_fwd_workspace_bytes",
+          "cogaim_linear_bwd_input_workspace_bytes", "cogaim_linear_bwd_weight_workspace_bytes"}
+_NO_STATUS |= _BYTES
 _lib = None
 
 
@@ -118,7 +155,7 @@ def lib() -> C.PyDLL:
         for name, args in SIGNATURES.items():
             fn = getattr(handle, name)
             fn.argtypes = args
-            fn.restype = LL if name == "cogaim_gemm_workspace_bytes" else I
+            fn.restype = LL if name in _BYTES else I
         for name, args in OPTIONAL.items():
             if hasattr(handle, name):
                 fn = getattr(handle, name)

@@ -8,9 +8,12 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcogaim.so")
-SOURCES = ["gemm.hip", "gemm_rowln.hip", "attention.hip", "rowwise.hip", "focal.hip", "small.hip", "preprocess.hip"]
+SOURCES = ["gemm.hip", "gemm_rowln.hip", "attention.hip", "rowwise.hip", "focal.hip", "small.hip", "preprocess.hip",
+           "train_rows.hip", "train_linear.hip"]
 # attention.hip: without NaN-honouring, fmaxf on MFMA results needs no canonicalising v_max (x3 fewer max ops)
-EXTRA_FLAGS = {"attention.hip": ["-fno-honor-nans"]}
+EXTRA_FLAGS = {"attention.hip": ["-fno-honor-nans"],
+               "train_rows.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],     # no packed fp32 arithmetic
+               "train_linear.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
 
 
 def _hipcc() -> str:
@@ -24,7 +27,7 @@ def needs_build() -> bool:
     if not os.path.exists(LIB):
         return True
     t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "cogaim.h")]
     return any(os.path.getmtime(d) > t for d in deps)
 
 

@@ -1,0 +1,284 @@
+// MFMA main loop of the linear layers' training products (included by train_linear.hip):
+//   C[m][n] = sum_k A(m, k) B(n, k),  16-bit operands, fp32 accumulation,
+// for every combination of operand layouts that a linear layer's three products need:
+//   forward          y = x W^T       A = x  [m][k],  B = W  [n][k]     both contiguous along k
+//   input gradient   dx = dy W       A = dy [m][k],  B = W  [k][n]     B contiguous along n
+//   weight gradient  dW = dy^T x     A = dy [k][m],  B = x  [k][n]     both contiguous across k
+// An operand contiguous along k is staged [row][64 k] and read with ds_read_b128; one contiguous across k is staged as
+// it lies, [64 k][columns], and read with the transposing ds_read_b64_tr_b16, which hands a lane four consecutive k of
+// its column: no operand is ever transposed in memory.  Staging is 16-byte LDS-DMA (buffer_load ... lds) into a ring
+// of STAGES K-tiles of 64; the XOR swizzles below are applied to the DMA's source address (its destination is
+// lane-linear) and again to the fragment reads, and spread the rows a read touches over all LDS banks.  Rows past the
+// matrix read as zero through the buffer resource's size; a last K-tile that is not whole is masked by moving lanes
+// past its end out of the resource.
+//
+// Accumulators hold C^T fragments (B is the MFMA's row operand), so a lane owns one row m and, with the column order
+// below, runs of eight consecutive n: fragment j of a wave's strip covers columns 32 (j / 2) + 8 q + 4 (j % 2) + e for
+// accumulator element e of the lanes with lane / 16 = q.  16-bit results leave as 16-byte stores and the 32 columns of
+// an 8-bit group lie in four lanes.
+#pragma once
+#include "train_common.h"
+
+namespace {
+using namespace train;
+
+constexpr int TK = 64;                     // k per tile
+
+struct Operands {
+  const void* A; const void* B; long long lda, ldb;
+  int rows_a, rows_b;                      // rows of A and B as stored along m and n: the matrix, with a copied operand's padding
+  int KA, KB;                              // k of A and B as stored: KA may hold zero columns past KB
+  int M, N;                                // the result
+  int tiles_m, tiles_n, splits, kt_per_split;
+  float* col_sum;                          // weight gradient: [splits][M] sums of A over k (the bias' gradient), or null
+};
+
+__device__ __forceinline__ int swz_k_plain(int r) { return (r >> 1) & 7; }                               // rows r, r + 1, ...
+__device__ __forceinline__ int swz_k_wide(int r) { return ((r >> 1) & 1) | (((r >> 3) & 3) << 1); }      // rows of the column order
+template <int R> __device__ __forceinline__ int swz_x_plain(int k) {                                    // in 32-byte units
+  return R >= 128 ? (k & 3) | (((k >> 3) & 1) << 2) : ((k >> 1) & 1) | (((k >> 3) & 1) << 1);
+}
+template <int R> __device__ __forceinline__ int swz_x_wide(int k) { return R >= 128 ? k & 3 : (k >> 1) & 1; }   // in 64-byte units
+
+// 64 lanes bring 1 KiB into LDS.  Written as asm because the compiler answers the builtin with a wait for all DMA in
+// flight before every transposing read (it cannot tell the ring's stages apart); the kernel counts its own waits.  No
+// register is written.
+__device__ __forceinline__ void dma16(unsigned lane_offset, u32x4v rsrc, unsigned lds_offset) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :: "v"(lane_offset), "s"(rsrc), "s"(lds_offset) : "m0");
+}
+
+// One operand's side of the DMA: R rows (or columns), NW waves; KC: contiguous along k; WIDE: column order of B.
+template <int R, int NW, bool KC, bool WIDE> struct Stager {
+  static constexpr int PIECES = R / 8 / NW;
+  unsigned off[PIECES], chunk[KC ? PIECES : 1];
+  unsigned long long base; long long left, step;      // next K-tile's first byte, bytes of the operand from there
+  int k_left;                                         // k from there to the operand's end
+  unsigned lds0;
+  __device__ __forceinline__ void init(const void* p, long long ld, int first, int count, int K, int k0, int wave, int lane, unsigned lds) {
+    lds0 = lds + wave * PIECES * 1024;
+    k_left = K - k0;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int piece = wave * PIECES + i;
+      if constexpr (KC) {
+        const int r = piece * 8 + (lane >> 3);
+        const int c = (lane & 7) ^ (WIDE ? swz_k_wide(r) : swz_k_plain(r));
+        off[i] = (unsigned)r * (unsigned)(ld * 2) + (unsigned)c * 16;
+        chunk[i] = (unsigned)c * 8;
+      } else {
+        constexpr int CR = R / 8, RP = 64 / CR;       // 16-byte chunks per k, k per piece
+        const int k = piece * RP + lane / CR;
+        const int c = (lane % CR) ^ (WIDE ? swz_x_wide<R>(k) << 2 : swz_x_plain<R>(k) << 1);
+        off[i] = (unsigned)k * (unsigned)(ld * 2) + (unsigned)c * 16;
+      }
+    }
+    if constexpr (KC) {
+      base = reinterpret_cast<unsigned long long>(p) + ((unsigned long long)first * ld + k0) * 2;
+      left = (((long long)count - first - 1) * ld + K - k0) * 2;
+      step = TK * 2;
+    } else {
+      base = reinterpret_cast<unsigned long long>(p) + ((unsigned long long)k0 * ld + first) * 2;
+      left = (((long long)K - k0 - 1) * ld + count - first) * 2;
+      step = TK * ld * 2;
+    }
+  }
+  // without `live` the loads are dropped (and still counted by the wait)
+  __device__ __forceinline__ void issue(bool live, unsigned stage_lds) {
+    const unsigned n = live && left > 0 ? (unsigned)(left < 0x7ffffff0LL ? left : 0x7ffffff0LL) : 0u;
+    u32x4v rsrc;
+    rsrc[0] = __builtin_amdgcn_readfirstlane((unsigned)base);
+    rsrc[1] = __builtin_amdgcn_readfirstlane((unsigned)(base >> 32) & 0xffffu);
+    rsrc[2] = __builtin_amdgcn_readfirstlane(n);
+    rsrc[3] = 0x00020000u;
+    if (KC && k_left < TK) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+        dma16((int)chunk[KC ? i : 0] < k_left ? off[i] : 0xffffff00u, rsrc, __builtin_amdgcn_readfirstlane(stage_lds + lds0 + i * 1024));
+    } else {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) dma16(off[i], rsrc, __builtin_amdgcn_readfirstlane(stage_lds + lds0 + i * 1024));
+    }
+    base += step; left -= step; k_left -= TK;
+  }
+};
+
+// eight 16-bit values of fragment data through two transposing reads (k 0-3 and 4-7 of the lane's eight)
+template <class T> struct TrRead;
+typedef __bf16 bf16x4t __attribute__((ext_vector_type(4)));
+typedef __fp16 f16x4t __attribute__((__vector_size__(8)));
+template <> struct TrRead<__bf16> {
+  static __device__ __forceinline__ bf16x8 read(const char* p, int second) {
+    typedef __attribute__((address_space(3))) bf16x4t* lp;
+    const bf16x4t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lp)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lp)(p + second));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+template <> struct TrRead<_Float16> {
+  static __device__ __forceinline__ f16x8 read(const char* p, int second) {
+    typedef __attribute__((address_space(3))) f16x4t* lp;
+    const f16x4t lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lp)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lp)(p + second));
+    return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+// the fragment reads of one operand: `i` a fragment of the wave's strip, `s` the k32 half
+template <class T, int R, bool KC, bool WIDE> struct Reader {
+  using v8 = typename Half<T>::v8;
+  int at, flip;
+  __device__ __forceinline__ void init(int strip, int lane) {         // strip: the wave's first row (column) in the tile
+    const int fr = lane & 15, fq = lane >> 4;
+    if constexpr (KC) {
+      const int r = strip + (WIDE ? 8 * (fr >> 2) + (fr & 3) : fr);
+      at = r * 128; flip = (fq ^ (WIDE ? swz_k_wide(r) : swz_k_plain(r))) << 4;      // fragments move r by multiples the swizzles ignore
+    } else {
+      const int k = 8 * fq + (fr >> 2);
+      if constexpr (WIDE) at = k * (R * 2) + (((strip / 32) ^ swz_x_wide<R>(k)) << 6) + (fr & 3) * 16;
+      else at = k * (R * 2) + (((strip / 16) ^ swz_x_plain<R>(k)) << 5) + (fr & 3) * 8;
+      flip = 0;
+    }
+  }
+  __device__ __forceinline__ v8 read(const char* stage, int i, int s) const {
+    if constexpr (KC) {
+      const int row = WIDE ? 4 * (i & 1) + 32 * (i >> 1) : 16 * i;
+      return *reinterpret_cast<const v8*>(stage + at + row * 128 + (flip ^ (s << 6)));
+    } else if constexpr (WIDE) {
+      return TrRead<T>::read(stage + (at ^ ((i >> 1) << 6)) + (i & 1) * 8 + s * (32 * R * 2), 4 * R * 2);
+    } else {
+      return TrRead<T>::read(stage + (at ^ (i << 5)) + s * (32 * R * 2), 4 * R * 2);
+    }
+  }
+};
+
+// bijective XCD-aware remap: blocks of one XCD (bid % 8) get a contiguous range
+__device__ __forceinline__ int xcd_range(int bid, int n) {
+  const int q = n >> 3, r = n & 7, x = bid & 7;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
+}
+
+template <int BM_, int BN_, int WM_, int WN_, int ST_> struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = ST_, NW = WM_ * WN_;
+  static constexpr int MI = BM_ / WM_ / 16, NJ = BN_ / WN_ / 16;
+  static constexpr int STAGE = (BM_ + BN_) * TK * 2;
+};
+
+template <class T, bool AKC, bool BKC, class TL, class Epi>
+__global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, Epi epi) {
+  constexpr int BM = TL::BM, BN = TL::BN, MI = TL::MI, NJ = TL::NJ, ST = TL::STAGES;
+  constexpr int PER_STAGE = (BM + BN) / 8 / TL::NW;                   // DMA instructions a wave issues per K-tile
+  __shared__ __attribute__((aligned(1024))) char smem[ST * TL::STAGE];
+  using H = Half<T>;
+  using v8 = typename H::v8;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / TL::WN, wn = wave % TL::WN;
+  const int tiles = g.tiles_m * g.tiles_n;
+  const int id = xcd_range(blockIdx.x, gridDim.x);
+  const int split = id / tiles, tile = id - split * tiles;
+  // bands of 8 tile rows: the 32 tiles an XCD works on at a time share 8 row panels and 4 column panels
+  constexpr int BAND = 8;
+  const int band = tile / (BAND * g.tiles_n), in_band = tile - band * BAND * g.tiles_n;
+  const int rows = g.tiles_m - band * BAND < BAND ? g.tiles_m - band * BAND : BAND;
+  const int tn = in_band / rows, tm = band * BAND + in_band - tn * rows;
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int nk_all = (g.KA + TK - 1) / TK;
+  const int kt0 = split * g.kt_per_split;
+  int nk = nk_all - kt0; nk = nk < g.kt_per_split ? nk : g.kt_per_split;        // K-tiles of this block (at least 1)
+
+  Stager<BM, TL::NW, AKC, false> sa;
+  Stager<BN, TL::NW, BKC, true> sb;
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+  sa.init(g.A, g.lda, m0, g.rows_a, g.KA, kt0 * TK, wave, lane, lds);
+  sb.init(g.B, g.ldb, n0, g.rows_b, g.KB, kt0 * TK, wave, lane, lds + BM * TK * 2);
+  int issued = 0;
+  auto issue = [&](int slot) {
+    sa.issue(issued < nk, slot * TL::STAGE);
+    sb.issue(issued < nk, slot * TL::STAGE);
+    ++issued;
+  };
+  Reader<T, BM, AKC, false> ra;
+  Reader<T, BN, BKC, true> rb;
+  ra.init(wm * (BM / TL::WM), lane);
+  rb.init(wn * (BN / TL::WN), lane);
+
+  f32x4 acc[MI][NJ];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // sums of A over k for the bias' gradient: products with a fragment of ones, the row fragments dealt to the WN waves
+  // that share them; only the blocks of the first tile column
+  constexpr bool SUMS = !AKC;
+  constexpr int NS = SUMS ? MI / TL::WN : 1;
+  static_assert(!SUMS || MI % TL::WN == 0, "row fragments are dealt evenly");
+  f32x4 sums[NS];
+  v8 ones;
+  const bool with_sums = SUMS && g.col_sum && tn == 0;
+  if constexpr (SUMS) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = (T)1.0f;
+  }
+
+#pragma unroll
+  for (int p = 0; p < ST - 1; ++p) issue(p);
+  int slot = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    // this K-tile has landed (the ST - 2 younger ones may still be in flight) and this wave's reads of the slot that is
+    // refilled next are done; behind the barrier that holds for every wave
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((ST - 2) * PER_STAGE) : "memory");
+    issue(slot == 0 ? ST - 1 : slot - 1);
+    const char* as = smem + slot * TL::STAGE;
+    const char* bs = as + BM * TK * 2;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      v8 bf[NJ], af[MI];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) bf[j] = rb.read(bs, j, s);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) af[i] = ra.read(as, i, s);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = H::mfma16(bf[j], af[i], acc[i][j]);
+      if constexpr (SUMS) {
+        if (with_sums) {
+#pragma unroll
+          for (int q = 0; q < NS; ++q) sums[q] = H::mfma16(ones, ra.read(as, wn * NS + q, s), sums[q]);
+        }
+      }
+    }
+    slot = slot == ST - 1 ? 0 : slot + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // the dropped loads past the end
+  const int fr = lane & 15, fq = lane >> 4;
+  const int mw = m0 + wm * (BM / TL::WM) + fr, nw = n0 + wn * (BN / TL::WN) + 8 * fq;
+  if constexpr (SUMS) {
+    if (with_sums && fq == 0) {
+#pragma unroll
+      for (int q = 0; q < NS; ++q) {
+        const int m = mw + 16 * (wn * NS + q);
+        if (m < g.M) g.col_sum[(size_t)split * g.M + m] = sums[q][0];
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < NJ / 2; ++h) {
+    const int n = nw + 32 * h;
+    typename Epi::Columns col;
+    epi.columns(n, col);
+    typename Epi::Row next;
+    epi.template fetch<true>(mw, n, next);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const typename Epi::Row now = next;
+      if (i + 1 < MI) epi.template fetch<true>(mw + 16 * (i + 1), n, next);   // the next row's reads go out ahead of this row's stores
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] = acc[i][2 * h][e]; v[4 + e] = acc[i][2 * h + 1][e]; }
+      epi.template finish<true, 16, 32>(split, mw + 16 * i, n, v, col, now);
+    }
+  }
+}
+
+}  // namespace

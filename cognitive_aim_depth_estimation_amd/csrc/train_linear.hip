@@ -1,0 +1,488 @@
+// Linear layers' training products: forward with bias, activation, LayerScale, residual and an 8-bit copy of the
+// pre-activation in the epilogue; gradient of the input with the derivative of the activation below in the epilogue;
+// gradients of weight, bias and LayerScale.  Main loop in train_gemm.h.
+//
+// Every product is one launch of the main loop when its tiles fill the chip; with fewer tiles the sum is split over k,
+// the parts leave fp32 partial tiles in the workspace and a join kernel adds them in order and applies the epilogue
+// (no atomics: results do not depend on timing).
+#include "train_gemm.h"
+#include "../../include/cogaim.h"
+
+namespace {
+
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+constexpr long long MAX_LD = 1 << 21;      // a tile's 256 rows stay inside a buffer resource's 32-bit offsets
+
+// ---- epilogues ---------------------------------------------------------------------------------------------------
+// finish<FAST, X1, X2>: eight columns [n, n + 8) of row m; the four lanes that hold a group of 32 are X1 and X2 apart.
+// Every lane of the wave calls it (the 8-bit group maximum crosses lanes); rows and columns past the matrix are dropped
+// here.  FAST: the width is a multiple of eight and every array takes 16-byte accesses (`fast()`); the main loop carries
+// only that form, sixteen times unrolled, and leaves any other result to the join kernel.
+template <bool FAST>
+__device__ __forceinline__ void store_run8(void* p, int dt, long long ld, bool vec, int m, int n, int N, const float (&y)[8]) {
+  const size_t at = (size_t)m * ld + n;
+  if (FAST || (vec && n + 8 <= N)) store_vec8(p, dt, at, y);
+  else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n + j < N) store_one(p, dt, at + j, y[j]);
+  }
+}
+
+template <int ACT>
+struct EpiForward {                          // y = act(acc + bias) * scale + residual, codes of acc + bias
+  const float* bias; const float* scale; const void* res; void* y; signed char* codes; unsigned char* bytes;
+  long long ldr, ldy; int M, N, res_dt, y_dt; bool res_vec, y_vec, code_vec;
+  bool fast() const { return (N & 7) == 0 && y_vec && (!res || res_vec) && (!codes || code_vec); }
+  struct Columns { float b[8], s[8]; };
+  struct Row { Raw8 r; };
+  __device__ __forceinline__ void columns(int n, Columns& c) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int at = n + j < N ? n + j : N - 1;
+      c.b[j] = bias ? bias[at] : 0.f;
+      c.s[j] = ACT == ACT_NONE && scale ? scale[at] : 1.f;
+    }
+  }
+  template <bool FAST>
+  __device__ __forceinline__ void fetch(int m, int n, Row& r) const {
+    if (res && (FAST || (res_vec && n + 8 <= N)) && m < M && n < N) r.r = load_raw8(res, res_dt, (size_t)m * ldr + n);
+  }
+  template <bool FAST, int X1, int X2>
+  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns& c, const Row& r) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += c.b[j];
+    if (codes) {
+      unsigned top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = umax(top, (FAST ? n : n + j) < N ? mag_bits(v[j]) : 0u);
+      top = umax(top, (unsigned)__shfl_xor((int)top, X1, 64));
+      top = umax(top, (unsigned)__shfl_xor((int)top, X2, 64));
+      if (m < M && n < N) {
+        const unsigned byte = group_byte(top);
+        const u32x2 q = pack_codes(v, byte);
+        signed char* to = codes + (size_t)m * N + n;
+        if (FAST || (code_vec && n + 8 <= N)) *reinterpret_cast<u32x2*>(to) = q;
+        else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (n + j < N) to[j] = (signed char)(q[j >> 2] >> (8 * (j & 3)));
+        }
+        if ((n & (GROUP - 1)) == 0) bytes[(size_t)m * groups_of(N) + n / GROUP] = (unsigned char)byte;
+      }
+    }
+    if (m >= M || n >= N) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (ACT == ACT_RELU) v[j] = relu_of(v[j]);
+      else if constexpr (ACT == ACT_GELU) v[j] = gelu_of(v[j]);
+      else v[j] *= c.s[j];
+    }
+    if (res) {
+      float a[8];
+      if (FAST || (res_vec && n + 8 <= N)) cvt_raw8(r.r, res_dt, a);
+      else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = n + j < N ? load_one(res, res_dt, (size_t)m * ldr + n + j) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += a[j];
+    }
+    store_run8<FAST>(y, y_dt, ldy, y_vec, m, n, N, v);
+  }
+};
+
+template <int ACT>
+struct EpiInput {                            // dx = acc * act'(u), a = act(u), u from its 8-bit copy
+  const signed char* codes; const unsigned char* bytes; void* dx; void* a; long long lddx, lda;
+  int M, N, dx_dt, a_dt; bool dx_vec, a_vec, code_vec;
+  bool fast() const { return (N & 7) == 0 && dx_vec && (!a || a_vec) && (!codes || code_vec); }
+  struct Columns {};
+  struct Row { u32x2 q; unsigned byte; };
+  __device__ __forceinline__ void columns(int, Columns&) const {}
+  template <bool FAST>
+  __device__ __forceinline__ void fetch(int m, int n, Row& r) const {
+    if constexpr (ACT != ACT_NONE) {
+      if (m < M && n < N) {
+        const signed char* p = codes + (size_t)m * N + n;
+        if (FAST || (code_vec && n + 8 <= N)) r.q = *reinterpret_cast<const u32x2*>(p);
+        else {
+          r.q = u32x2{0, 0};
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (n + j < N) r.q[j >> 2] |= (unsigned)(unsigned char)p[j] << (8 * (j & 3));
+        }
+        r.byte = bytes[(size_t)m * groups_of(N) + n / GROUP];
+      }
+    }
+  }
+  template <bool FAST, int X1, int X2>
+  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row& r) const {
+    if (m >= M || n >= N) return;
+    if constexpr (ACT != ACT_NONE) {
+      float u[8];
+      decode8(r.q, group_step(r.byte), u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float value, slope;
+        if constexpr (ACT == ACT_GELU) gelu_both(u[j], value, slope);
+        else { value = relu_of(u[j]); slope = relu_slope(u[j]); }
+        v[j] *= slope;
+        u[j] = value;
+      }
+      if (a) store_run8<FAST>(a, a_dt, lda, a_vec, m, n, N, u);
+    }
+    store_run8<FAST>(dx, dx_dt, lddx, dx_vec, m, n, N, v);
+  }
+};
+
+struct EpiPlain {                            // the product itself
+  void* out; long long ld; int M, N, dt; bool vec;
+  struct Columns {};
+  struct Row {};
+  __device__ __forceinline__ void columns(int, Columns&) const {}
+  template <bool FAST>
+  __device__ __forceinline__ void fetch(int, int, Row&) const {}
+  template <bool FAST, int X1, int X2>
+  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row&) const {
+    if (m < M && n < N) store_run8<FAST>(out, dt, ld, vec, m, n, N, v);
+  }
+};
+
+struct EpiPart {                             // fp32 partial sums [split][M][Np], Np = N rounded up to 8
+  float* part; int M, Np;
+  struct Columns {};
+  struct Row {};
+  __device__ __forceinline__ void columns(int, Columns&) const {}
+  template <bool FAST>
+  __device__ __forceinline__ void fetch(int, int, Row&) const {}
+  template <bool FAST, int X1, int X2>
+  __device__ __forceinline__ void finish(int split, int m, int n, float (&v)[8], const Columns&, const Row&) const {
+    if (m < M && n < Np) store_vec8(part, DT_FP32, ((size_t)split * M + m) * Np + n, v);
+  }
+};
+
+// adds the parts of eight columns in split order and applies the epilogue; four neighbouring threads hold a group
+template <class Epi>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int M, int N, int Np, Epi epi) {
+  const int per_row = (int)groups_of(N) * 4;
+  const long long i = blockIdx.x * 256LL + threadIdx.x;
+  const long long row = i / per_row;
+  const int n = (int)(i - row * per_row) * 8;
+  const int m = row < M ? (int)row : M;                       // past the end: dropped by the epilogue
+  typename Epi::Columns col;
+  epi.columns(n < N ? n : 0, col);
+  typename Epi::Row r;
+  epi.template fetch<false>(m, n, r);
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  if (m < M && n < N) {
+    for (int s = 0; s < splits; ++s) {
+      const float4* p = reinterpret_cast<const float4*>(part + ((size_t)s * M + m) * Np + n);
+      const float4 x = p[0], y = p[1];
+      v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    }
+  }
+  epi.template finish<false, 1, 2>(0, m, n, v, col, r);
+}
+
+// One block per row n of the weight's gradient:  G = sum of the parts, with x = xh * xs + xt put back
+// (sum_m dy (xh xs + xt) = (dy^T xh) xs + (sum_m dy) xt);  dW = s G, db = s sum dy, ds = sum_k W G + b sum dy.
+struct WeightFinish {
+  const float* part; const float* col_sum; const float* xs; const float* xt; const float* scale; const void* W; const float* bias;
+  void* dW; float* db; float* ds; long long ldw, lddw; int N, K, Kp, splits, dt, dw_dt; bool vec;
+};
+__global__ __launch_bounds__(256) void weight_finish_kernel(WeightFinish a) {
+  __shared__ float red[4];
+  const int n = blockIdx.x;
+  float total = 0.f;
+  for (int s = 0; s < a.splits; ++s) total += a.col_sum[(size_t)s * a.N + n];
+  const float sc = a.scale ? a.scale[n] : 1.f;
+  float dot = 0.f;
+  for (int k = threadIdx.x * 4; k < a.K; k += 1024) {
+    float g[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+      const float4 p = *reinterpret_cast<const float4*>(a.part + ((size_t)s * a.N + n) * a.Kp + k);
+      g[0] += p.x; g[1] += p.y; g[2] += p.z; g[3] += p.w;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (k + j >= a.K) continue;
+      if (a.xs) g[j] *= a.xs[k + j];
+      if (a.xt) g[j] = __builtin_fmaf(total, a.xt[k + j], g[j]);
+      if (a.ds) dot = __builtin_fmaf(load_one(a.W, a.dt, (size_t)n * a.ldw + k + j), g[j], dot);
+      g[j] *= sc;
+    }
+    const size_t at = (size_t)n * a.lddw + k;
+    if (a.vec && k + 4 <= a.K && a.dw_dt == DT_FP32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.dW) + at) = make_float4(g[0], g[1], g[2], g[3]);
+    else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k + j < a.K) store_one(a.dW, a.dw_dt, at + j, g[j]);
+    }
+  }
+  if (a.ds) {
+    dot = block_sum_256(dot, red);
+    if (threadIdx.x == 0) a.ds[n] = dot + (a.bias ? a.bias[n] * total : 0.f);
+  }
+  if (a.db && threadIdx.x == 0) a.db[n] = sc * total;
+}
+
+// Copy of an operand whose rows 16-byte loads cannot address (odd widths, strides or bases), padded with zeros to a
+// multiple of eight columns; with `scale`, row r times scale[r] (rounded once to 16 bits: the matrix cores take it so).
+__global__ __launch_bounds__(256) void copy_rows_kernel(const unsigned short* __restrict__ src, long long ld, int R, int C, int C8,
+                                                        const float* __restrict__ scale, int dt, unsigned short* __restrict__ dst) {
+  const unsigned runs = (unsigned)C8 / 8;
+  const unsigned long long total = (unsigned long long)R * runs;
+  for (unsigned long long i = blockIdx.x * 256ULL + threadIdx.x; i < total; i += 256ULL * gridDim.x) {
+    const unsigned long long r = i / runs;
+    const int c = (int)(i - r * runs) * 8;
+    u32x4v w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      unsigned two = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int k = c + 2 * j + e;
+        unsigned h = k < C ? src[r * ld + k] : 0u;
+        if (scale && k < C) h = bits16((dt == DT_BF16 ? __uint_as_float(h << 16) : half_bits((unsigned short)h)) * scale[r], dt);
+        two |= h << (16 * e);
+      }
+      w[j] = two;
+    }
+    *reinterpret_cast<u32x4v*>(dst + r * C8 + c) = w;
+  }
+}
+
+// ---- plans -------------------------------------------------------------------------------------------------------
+using T256 = Tile<256, 256, 2, 4, 2>;
+using T128 = Tile<128, 128, 2, 2, 2>;
+using T64 = Tile<64, 64, 2, 2, 4>;
+
+struct Shape { int tile, tiles_m, tiles_n, splits, kt_per_split; };      // tile: 256, 128 or 64
+
+Shape shape_of(int M, int N, int K) {
+  const int nk = (K + TK - 1) / TK;
+  auto tiles = [&](int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); };
+  Shape s;
+  if (tiles(256) >= 160 || (tiles(256) >= 32 && nk >= 64)) s.tile = 256;
+  else if (tiles(128) >= 64) s.tile = 128;
+  else s.tile = 64;
+  s.tiles_m = (M + s.tile - 1) / s.tile; s.tiles_n = (N + s.tile - 1) / s.tile;
+  const long long t = (long long)s.tiles_m * s.tiles_n;
+  const long long room = s.tile == 256 ? 256 : 512;                      // blocks that run at a time
+  long long want = t >= room ? 1 : room / t;
+  const int least = s.tile == 256 ? 8 : 4;                               // K-tiles a part needs to be worth its partial sums
+  if (want > nk / least) want = nk / least;
+  if (want < 1) want = 1;
+  s.kt_per_split = (int)((nk + want - 1) / want);
+  s.splits = (nk + s.kt_per_split - 1) / s.kt_per_split;                 // no part is empty
+  return s;
+}
+
+long long round256(long long v) { return (v + 255) / 256 * 256; }
+int round8(int v) { return (v + 7) & ~7; }
+
+// an operand as the main loop takes it: `copy` when 16-byte loads cannot address it
+struct Side { const void* p; long long ld; int rows, cols; bool copy; const float* scale; };
+Side side(const void* p, long long ld, int rows, int cols, const float* scale = nullptr) {
+  Side s{p, ld, rows, cols, scale || (cols & 7) || (ld & 7) || !aligned(p, 16), scale};
+  return s;
+}
+long long copy_bytes(const Side& s) { return s.copy ? round256((long long)s.rows * round8(s.cols) * 2) : 0; }
+
+int run_copy(Side& s, int dt, char*& ws, hipStream_t st) {
+  if (!s.copy) return COGAIM_OK;
+  const int c8 = round8(s.cols);
+  const unsigned long long runs = (unsigned long long)s.rows * (c8 / 8);
+  unsigned long long blocks = (runs + 255) / 256;
+  if (blocks > 256 * 32) blocks = 256 * 32;
+  hipLaunchKernelGGL(copy_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, st, (const unsigned short*)s.p, s.ld, s.rows, s.cols, c8,
+                     s.scale, dt, (unsigned short*)ws);
+  s.p = ws; s.ld = c8; s.cols = c8;
+  ws += round256((long long)s.rows * c8 * 2);
+  return COGAIM_LAUNCH_CHECK();
+}
+
+template <class T, bool AKC, bool BKC, class Epi>
+int launch_gemm(const Operands& g, int tile, const Epi& e, hipStream_t st) {
+  const long long blocks = (long long)g.tiles_m * g.tiles_n * g.splits;
+  if (blocks <= 0 || blocks >= (1LL << 31)) return COGAIM_EINVAL;
+  if (tile == 256) hipLaunchKernelGGL((train_gemm_kernel<T, AKC, BKC, T256, Epi>), dim3((unsigned)blocks), dim3(512), 0, st, g, e);
+  else if (tile == 128) hipLaunchKernelGGL((train_gemm_kernel<T, AKC, BKC, T128, Epi>), dim3((unsigned)blocks), dim3(256), 0, st, g, e);
+  else hipLaunchKernelGGL((train_gemm_kernel<T, AKC, BKC, T64, Epi>), dim3((unsigned)blocks), dim3(256), 0, st, g, e);
+  return COGAIM_LAUNCH_CHECK();
+}
+
+// the epilogue runs in a kernel of its own: parts to add, or a result that 16-byte stores cannot reach
+template <class Epi> bool joins(const Shape& s, const Epi& e) { return s.splits > 1 || !e.fast(); }
+
+template <class T, bool AKC, bool BKC, class Epi>
+int product(const Operands& g, const Shape& s, const Epi& e, float* part, hipStream_t st) {
+  if (!joins(s, e)) return launch_gemm<T, AKC, BKC>(g, s.tile, e, st);
+  const int Np = round8(g.N);
+  const int rc = launch_gemm<T, AKC, BKC>(g, s.tile, EpiPart{part, g.M, Np}, st);
+  if (rc) return rc;
+  const long long threads = (long long)g.M * groups_of(g.N) * 4;
+  if ((threads + 255) / 256 >= (1LL << 31)) return COGAIM_EINVAL;
+  hipLaunchKernelGGL((join_kernel<Epi>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, part, s.splits, g.M, g.N, Np, e);
+  return COGAIM_LAUNCH_CHECK();
+}
+
+Operands operands(const Side& a, const Side& b, bool akc, bool bkc, int M, int N, const Shape& s) {
+  Operands g{};
+  g.A = a.p; g.B = b.p; g.lda = a.ld; g.ldb = b.ld;
+  g.rows_a = akc ? a.rows : a.cols; g.KA = akc ? a.cols : a.rows;
+  g.rows_b = bkc ? b.rows : b.cols; g.KB = bkc ? b.cols : b.rows;
+  g.M = M; g.N = N; g.tiles_m = s.tiles_m; g.tiles_n = s.tiles_n; g.splits = s.splits; g.kt_per_split = s.kt_per_split;
+  g.col_sum = nullptr;
+  return g;
+}
+bool half_dt(int dt) { return dt == DT_BF16 || dt == DT_FP16; }
+bool any_dt(int dt) { return dt >= 0 && dt <= 2; }
+bool vec_ok(const void* p, long long ld) { return aligned(p, 16) && (ld & 7) == 0; }
+bool matrix_ok(const void* p, long long ld, int cols, int elem) { return p && ld >= cols && ld <= MAX_LD && aligned(p, elem); }
+
+bool forward_ok(const cogaim_linear_fwd_desc* d) {
+  if (!d || d->M <= 0 || d->N <= 0 || d->K <= 0 || !half_dt(d->dtype) || !any_dt(d->y_dtype)) return false;
+  if (!matrix_ok(d->x, d->ldx, d->K, 2) || !matrix_ok(d->w, d->ldw, d->K, 2) || !matrix_ok(d->y, d->ldy, d->N, dt_size(d->y_dtype))) return false;
+  if (d->residual && (!any_dt(d->residual_dtype) || !matrix_ok(d->residual, d->ldr, d->N, dt_size(d->residual_dtype)))) return false;
+  if (d->activation < ACT_NONE || d->activation > ACT_GELU || (d->scale && d->activation != ACT_NONE)) return false;
+  return !d->codes == !d->exponents;
+}
+bool input_ok(const cogaim_linear_bwd_input_desc* d) {
+  if (!d || d->M <= 0 || d->N <= 0 || d->K <= 0 || !half_dt(d->dtype) || !any_dt(d->dx_dtype)) return false;
+  if (!matrix_ok(d->dy, d->lddy, d->N, 2) || !matrix_ok(d->w, d->ldw, d->K, 2) || !matrix_ok(d->dx, d->lddx, d->K, dt_size(d->dx_dtype))) return false;
+  if (d->activation < ACT_NONE || d->activation > ACT_GELU) return false;
+  if ((d->activation == ACT_NONE) != !d->codes || !d->codes != !d->exponents) return false;
+  return !d->a || (d->activation != ACT_NONE && matrix_ok(d->a, d->lda, d->K, 2));
+}
+bool weight_ok(const cogaim_linear_bwd_weight_desc* d) {
+  if (!d || d->M <= 0 || d->N <= 0 || d->K <= 0 || !half_dt(d->dtype) || !any_dt(d->dw_dtype)) return false;
+  if (!matrix_ok(d->dy, d->lddy, d->N, 2) || !matrix_ok(d->dw, d->lddw, d->K, dt_size(d->dw_dtype)) || !d->db) return false;
+  if (!d->codes != !d->exponents || !d->x == !d->codes) return false;
+  if (d->x && !matrix_ok(d->x, d->ldx, d->K, 2)) return false;
+  if ((d->x_scale || d->x_shift) && !d->codes) return false;
+  if (!d->ds != !d->scale) return false;
+  return !d->ds || matrix_ok(d->w, d->ldw, d->K, 2);
+}
+}  // namespace
+
+// the epilogues of a descriptor
+template <int ACT> EpiForward<ACT> forward_epi(const cogaim_linear_fwd_desc* d) {
+  return EpiForward<ACT>{d->bias, d->scale, d->residual, d->y, (signed char*)d->codes, (unsigned char*)d->exponents, d->ldr,
+                         d->ldy, d->M, d->N, d->residual_dtype, d->y_dtype, d->residual && vec_ok(d->residual, d->ldr),
+                         vec_ok(d->y, d->ldy), (d->N & 7) == 0 && aligned(d->codes, 8)};
+}
+template <int ACT> EpiInput<ACT> input_epi(const cogaim_linear_bwd_input_desc* d) {
+  return EpiInput<ACT>{(const signed char*)d->codes, (const unsigned char*)d->exponents, d->dx, d->a, d->lddx, d->lda, d->M,
+                       d->K, d->dx_dtype, d->dtype, vec_ok(d->dx, d->lddx), d->a && vec_ok(d->a, d->lda),
+                       (d->K & 7) == 0 && aligned(d->codes, 8)};
+}
+
+extern "C" {
+
+long long cogaim_linear_fwd_workspace_bytes(const cogaim_linear_fwd_desc* d) {
+  if (!forward_ok(d)) return COGAIM_EINVAL;
+  const Shape s = shape_of(d->M, d->N, d->K);
+  return copy_bytes(side(d->x, d->ldx, d->M, d->K)) + copy_bytes(side(d->w, d->ldw, d->N, d->K)) +
+         (joins(s, forward_epi<ACT_NONE>(d)) ? (long long)s.splits * d->M * round8(d->N) * 4 : 0);
+}
+
+int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long long workspace_bytes, void* stream) {
+  const long long need = cogaim_linear_fwd_workspace_bytes(d);
+  if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
+  hipStream_t st = (hipStream_t)stream;
+  const Shape s = shape_of(d->M, d->N, d->K);
+  Side a = side(d->x, d->ldx, d->M, d->K), b = side(d->w, d->ldw, d->N, d->K);
+  char* ws = (char*)workspace;
+  int rc = run_copy(a, d->dtype, ws, st);
+  if (!rc) rc = run_copy(b, d->dtype, ws, st);
+  if (rc) return rc;
+  const Operands g = operands(a, b, true, true, d->M, d->N, s);
+#define FWD_RUN(T_)                                                                                                    \
+  (d->activation == ACT_RELU ? product<T_, true, true>(g, s, forward_epi<ACT_RELU>(d), (float*)ws, st)                         \
+   : d->activation == ACT_GELU ? product<T_, true, true>(g, s, forward_epi<ACT_GELU>(d), (float*)ws, st)                       \
+                               : product<T_, true, true>(g, s, forward_epi<ACT_NONE>(d), (float*)ws, st))
+  return d->dtype == DT_BF16 ? FWD_RUN(__bf16) : FWD_RUN(_Float16);
+}
+
+long long cogaim_linear_bwd_input_workspace_bytes(const cogaim_linear_bwd_input_desc* d) {
+  if (!input_ok(d)) return COGAIM_EINVAL;
+  const Shape s = shape_of(d->M, d->K, d->N);
+  return copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + copy_bytes(side(d->w, d->ldw, d->N, d->K, d->scale)) +
+         (joins(s, input_epi<ACT_NONE>(d)) ? (long long)s.splits * d->M * round8(d->K) * 4 : 0);
+}
+
+int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspace, long long workspace_bytes, void* stream) {
+  const long long need = cogaim_linear_bwd_input_workspace_bytes(d);
+  if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
+  hipStream_t st = (hipStream_t)stream;
+  const Shape s = shape_of(d->M, d->K, d->N);
+  Side a = side(d->dy, d->lddy, d->M, d->N), b = side(d->w, d->ldw, d->N, d->K, d->scale);
+  char* ws = (char*)workspace;
+  int rc = run_copy(a, d->dtype, ws, st);
+  if (!rc) rc = run_copy(b, d->dtype, ws, st);
+  if (rc) return rc;
+  const Operands g = operands(a, b, true, false, d->M, d->K, s);
+#define IN_RUN(T_)                                                                                                     \
+  (d->activation == ACT_RELU ? product<T_, true, false>(g, s, input_epi<ACT_RELU>(d), (float*)ws, st)                         \
+   : d->activation == ACT_GELU ? product<T_, true, false>(g, s, input_epi<ACT_GELU>(d), (float*)ws, st)                       \
+                               : product<T_, true, false>(g, s, input_epi<ACT_NONE>(d), (float*)ws, st))
+  return d->dtype == DT_BF16 ? IN_RUN(__bf16) : IN_RUN(_Float16);
+}
+
+// whether the row-wise second kernel runs (parts to add, or something to put on the finished sums)
+static bool weight_needs_finish(const cogaim_linear_bwd_weight_desc* d, const Shape& s) {
+  return s.splits > 1 || d->x_scale || d->x_shift || d->scale || (d->K & 7) || !vec_ok(d->dw, d->lddw);
+}
+
+long long cogaim_linear_bwd_weight_workspace_bytes(const cogaim_linear_bwd_weight_desc* d) {
+  if (!weight_ok(d)) return COGAIM_EINVAL;
+  const Shape s = shape_of(d->N, d->K, d->M);
+  const long long x = d->codes ? round256((long long)d->M * round8(d->K) * 2) : copy_bytes(side(d->x, d->ldx, d->M, d->K));
+  const long long part = weight_needs_finish(d, s) ? round256((long long)s.splits * d->N * round8(d->K) * 4) + (long long)s.splits * d->N * 4 : 0;
+  return copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + x + part;
+}
+
+int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* workspace, long long workspace_bytes, void* stream) {
+  const long long need = cogaim_linear_bwd_weight_workspace_bytes(d);
+  if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
+  hipStream_t st = (hipStream_t)stream;
+  const Shape s = shape_of(d->N, d->K, d->M);
+  char* ws = (char*)workspace;
+  Side a = side(d->dy, d->lddy, d->M, d->N), b{};
+  int rc = run_copy(a, d->dtype, ws, st);
+  if (rc) return rc;
+  if (d->codes) {
+    // the 8-bit rows as 16-bit values in front of the product (a power-of-two step makes them exact in bf16)
+    const int k8 = round8(d->K);
+    rc = cogaim_unpack8(d->codes, d->exponents, ws, d->dtype, k8, d->M, d->K, k8, stream);
+    b = Side{ws, k8, d->M, k8, false, nullptr};
+    ws += round256((long long)d->M * k8 * 2);
+  } else {
+    b = side(d->x, d->ldx, d->M, d->K);
+    rc = run_copy(b, d->dtype, ws, st);
+  }
+  if (rc) return rc;
+  Operands g = operands(a, b, false, false, d->N, d->K, s);
+  if (!weight_needs_finish(d, s)) {
+    g.col_sum = d->db;
+    const EpiPlain e{d->dw, d->lddw, d->N, d->K, d->dw_dtype, true};
+    return d->dtype == DT_BF16 ? launch_gemm<__bf16, false, false>(g, s.tile, e, st) : launch_gemm<_Float16, false, false>(g, s.tile, e, st);
+  }
+  const int kp = round8(d->K);
+  float* part = (float*)ws;
+  float* sums = (float*)(ws + round256((long long)s.splits * d->N * kp * 4));
+  g.col_sum = sums;
+  const EpiPart e{part, d->N, kp};
+  rc = d->dtype == DT_BF16 ? launch_gemm<__bf16, false, false>(g, s.tile, e, st) : launch_gemm<_Float16, false, false>(g, s.tile, e, st);
+  if (rc) return rc;
+  const WeightFinish f{part, sums, d->x_scale, d->x_shift, d->scale, d->w, d->bias, d->dw, d->db, d->ds, d->ldw, d->lddw,
+                       d->N, d->K, kp, s.splits, d->dtype, d->dw_dtype, vec_ok(d->dw, d->lddw)};
+  hipLaunchKernelGGL(weight_finish_kernel, dim3(d->N), dim3(256), 0, st, f);
+  return COGAIM_LAUNCH_CHECK();
+}
+
+}  // extern "C"

@@ -302,6 +302,83 @@ int cogaim_curiosity_finish(const float* rec, const float* cls, long long ld_cls
  * attn fp32 [B,N], out fp32 [B,G*G]; N <= 6144. */
 int cogaim_heatmap_postprocess(const float* attn, float* out, int B, int N, int G, void* stream);
 
+/* ---- training -----------------------------------------------------------
+ * The training form of the encoder's row-wise and matrix parts.  No counterpart in the reference's own code: its
+ * train.py:145-160 leaves the backward pass of these modules (hf:348-378) to torch's autograd.
+ *
+ *  - element types at run time: 0 bf16, 1 fp16, 2 fp32; matrices are [rows, columns] with a leading dimension in
+ *    elements (any that is at least the row length: rows that 16-byte accesses cannot address take a slower path);
+ *    base pointers are aligned to their element;
+ *  - `workspace`: device memory of at least the stated number of bytes, 16-byte aligned, free for other use once the
+ *    call's work on `stream` is done;
+ *  - sums run in a fixed order: the same inputs give the same bits;
+ *  - 8-bit activations ("codes" int8 [rows, D] contiguous, "exponents" uint8 [rows, ceil(D / 32)] contiguous): groups of
+ *    32 columns of a row share the step 2^(exponent - 127), the smallest from 2^-126 up for which the group's largest
+ *    magnitude rounds to at most 127 steps; a code is x / step rounded to nearest, ties to even.  Exponent 255 marks a
+ *    group that held an infinity or a NaN: all of it stands for NaN.  Steps are powers of two, so a value is exact in
+ *    bf16; in fp16 it is rounded once.  Where a code's rounding would pass the largest finite value (63.5 steps of 2^122;
+ *    65504 in fp16) it is held below it.
+ */
+
+/* hf:348,353,441 nn.LayerNorm with what its backward pass needs: y = (x - mean) rstd * gamma + beta, mean and
+ * rstd = (variance + eps)^-1/2 per row (fp32 [M]), and, unless codes is NULL, the rows (x - mean) rstd in 8 bits.  D <= 16384. */
+int cogaim_layernorm_train_fwd(const void* x, int x_dtype, long long ldx, const float* gamma, const float* beta, void* y,
+                               int y_dtype, long long ldy, float* mean, float* rstd, void* codes, void* exponents, int M,
+                               int D, float eps, void* stream);
+
+/* Its backward pass, from either x and mean or the 8-bit rows (the other NULL): with h the normalised rows and g = dy * gamma,
+ *   dx = rstd (g - mean(g) - h mean(g h)) + add (add NULL: nothing; may be dx itself),  dgamma = sum over rows of dy h,
+ *   dbeta = sum over rows of dy. */
+long long cogaim_layernorm_bwd_workspace_bytes(int M, int D);
+int cogaim_layernorm_bwd(const void* dy, int dy_dtype, long long lddy, const void* x, int x_dtype, long long ldx,
+                         const void* codes, const void* exponents, const float* mean, const float* rstd,
+                         const float* gamma, const void* add, int add_dtype, long long ldadd, void* dx, int dx_dtype,
+                         long long lddx, float* dgamma, float* dbeta, int M, int D, void* workspace,
+                         long long workspace_bytes, void* stream);
+
+/* x [M, D] to 8 bits, and back into out [M, width >= D] (columns past D are written as zero). */
+int cogaim_pack8(const void* x, int x_dtype, long long ldx, void* codes, void* exponents, int M, int D, void* stream);
+int cogaim_unpack8(const void* codes, const void* exponents, void* out, int out_dtype, long long ldo, int M, int D, int width,
+                   void* stream);
+
+/* du = dy * act'(u), u from its 8-bit copy; activation 1 ReLU, 2 erf GELU. */
+int cogaim_activation_bwd(const void* dy, int dy_dtype, long long lddy, const void* codes, const void* exponents, void* du,
+                          int du_dtype, long long lddu, int activation, int M, int D, void* stream);
+
+/* nn.Linear with all that may follow it (hf:199-213, 246-252, 277-278, 286-297, 370-378):
+ *   u = x W^T + bias,  y = act(u) + residual  or  y = u * scale + residual,  and u in 8 bits unless codes is NULL.
+ * x [M,K], w [N,K] of `dtype` (0 or 1), bias, scale fp32 [N] (NULL: none), residual and y [M,N] of their own types (y may
+ * be the residual).  activation 0 none, 1 ReLU, 2 erf GELU; scale (LayerScale) only without one. */
+typedef struct {
+  const void* x; const void* w; const float* bias; const float* scale; const void* residual; void* y; void* codes; void* exponents;
+  long long ldx, ldw, ldr, ldy; int M, N, K, dtype, residual_dtype, y_dtype, activation, reserved;
+} cogaim_linear_fwd_desc;
+long long cogaim_linear_fwd_workspace_bytes(const cogaim_linear_fwd_desc* desc);
+int cogaim_linear_fwd(const cogaim_linear_fwd_desc* desc, void* workspace, long long workspace_bytes, void* stream);
+
+/* Gradient of a linear layer's input, and of the activation that produced that input:
+ *   dx = ((dy * scale) W) * act'(u),  u [M,K] the pre-activation of the layer below in 8 bits;  a = act(u) unless NULL
+ * (the layer's own input again, for its weight's gradient).  activation 0: no u.  With scale, W * scale is rounded to
+ * `dtype` for the matrix cores. */
+typedef struct {
+  const void* dy; const void* w; const float* scale; const void* codes; const void* exponents; void* dx; void* a;
+  long long lddy, ldw, lddx, lda; int M, N, K, dtype, dx_dtype, activation;
+} cogaim_linear_bwd_input_desc;
+long long cogaim_linear_bwd_input_workspace_bytes(const cogaim_linear_bwd_input_desc* desc);
+int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* desc, void* workspace, long long workspace_bytes, void* stream);
+
+/* Gradients of a linear layer's parameters.  x [M,K] is given in 16 bits, or in 8 bits with x = xh * x_scale + x_shift
+ * (fp32 [K], NULL: 1 and 0; a LayerNorm's weight and bias over its kept rows).  dW [N,K] = scale * dy^T x, db [N] =
+ * scale * sum over rows of dy, and, with scale (fp32 [N]), ds [N] = sum over rows of dy (x W^T + bias), for which w and
+ * bias (NULL: none) are read; without scale ds is NULL. */
+typedef struct {
+  const void* dy; const void* x; const void* codes; const void* exponents; const float* x_scale; const float* x_shift;
+  const void* w; const float* bias; const float* scale; void* dw; float* db; float* ds;
+  long long lddy, ldx, ldw, lddw; int M, N, K, dtype, dw_dtype, reserved;
+} cogaim_linear_bwd_weight_desc;
+long long cogaim_linear_bwd_weight_workspace_bytes(const cogaim_linear_bwd_weight_desc* desc);
+int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* desc, void* workspace, long long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
