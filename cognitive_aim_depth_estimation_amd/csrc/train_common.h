@@ -50,19 +50,16 @@ __device__ __forceinline__ unsigned bits16(float y, int dt) {
   if (dt == DT_BF16) return __builtin_bit_cast(unsigned short, (__bf16)y);
   return __builtin_bit_cast(unsigned short, (_Float16)y);
 }
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ void store_vec8(void* p, int dt, size_t off, const float (&y)[8]) {   // 16-byte aligned
   if (dt == DT_FP32) {
     float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + off);
     q[0] = make_float4(y[0], y[1], y[2], y[3]); q[1] = make_float4(y[4], y[5], y[6], y[7]);
   } else {
+    const f32x8 v = {y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
     u32x4v w;
-    if (dt == DT_BF16) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = bits16(y[2 * i], DT_BF16) | (bits16(y[2 * i + 1], DT_BF16) << 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = bits16(y[2 * i], DT_FP16) | (bits16(y[2 * i + 1], DT_FP16) << 16);
-    }
+    if (dt == DT_BF16) w = __builtin_bit_cast(u32x4v, __builtin_convertvector(v, bf16x8));
+    else w = __builtin_bit_cast(u32x4v, __builtin_convertvector(v, f16x8));
     *reinterpret_cast<u32x4v*>(reinterpret_cast<unsigned short*>(p) + off) = w;
   }
 }
@@ -94,20 +91,45 @@ __device__ __forceinline__ float group_inverse(unsigned byte) {          // 1 / 
 __device__ __forceinline__ float group_step(unsigned byte) {
   return byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
 }
-__device__ __forceinline__ int code_of(float x, float inverse, float most) {
-  const float q = __builtin_rintf(x * inverse);
-  return (int)(inverse == 0.f ? 0.f : __builtin_amdgcn_fmed3f(q, -most, most));
-}
-__device__ __forceinline__ float most_code(unsigned byte) { return byte == 249u ? 63.f : 127.f; }
 __device__ __forceinline__ unsigned mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 __device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
+// Largest magnitude of eight values as bits, NaN above all: `maximum` passes a NaN on (v_maximum3_f32, two values an
+// instruction).
+__device__ __forceinline__ unsigned top_bits8(const float (&v)[8]) {
+  float m = fabsf(v[0]);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) m = __builtin_elementwise_maximum(m, fabsf(v[j]));
+  return mag_bits(m);
+}
+// x / step to the nearest integer in the low bits of a float: adding 1.5 * 2^23 leaves no fraction bits, and rounds ties
+// to even as any fp32 addition
+__device__ __forceinline__ unsigned code_bits(float x, float inverse) {
+  return __float_as_uint(__builtin_fmaf(x, inverse, 12582912.f));
+}
+// the two kinds of group that code_bits does not serve: no step (all codes 0), and the largest step (codes end at 63)
+__device__ __forceinline__ bool group_is_rare(unsigned byte) { return byte >= 249u; }
+__device__ __forceinline__ int code_of_rare(float x, unsigned byte) {
+  if (byte == 255u) return 0;
+  return (int)__builtin_amdgcn_fmed3f(__builtin_rintf(x * group_inverse(byte)), -63.f, 63.f);
+}
+__device__ __forceinline__ int code_of(float x, unsigned byte) {
+  return group_is_rare(byte) ? code_of_rare(x, byte) : (int)(signed char)code_bits(x, group_inverse(byte));
+}
 __device__ __forceinline__ u32x2 pack_codes(const float (&v)[8], unsigned byte) {
-  const float inverse = group_inverse(byte), most = most_code(byte);
+  const float inverse = group_inverse(byte);
   u32x2 r;
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    r[h] = (code_of(v[4 * h], inverse, most) & 255) | ((code_of(v[4 * h + 1], inverse, most) & 255) << 8) |
-           ((code_of(v[4 * h + 2], inverse, most) & 255) << 16) | ((unsigned)code_of(v[4 * h + 3], inverse, most) << 24);
+  for (int h = 0; h < 2; ++h) {
+    const unsigned lo = __builtin_amdgcn_perm(code_bits(v[4 * h + 1], inverse), code_bits(v[4 * h], inverse), 0x0c0c0400u);
+    const unsigned hi = __builtin_amdgcn_perm(code_bits(v[4 * h + 3], inverse), code_bits(v[4 * h + 2], inverse), 0x04000c0cu);
+    r[h] = lo | hi;
+  }
+  if (group_is_rare(byte)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      r[h] = (code_of_rare(v[4 * h], byte) & 255) | ((code_of_rare(v[4 * h + 1], byte) & 255) << 8) |
+             ((code_of_rare(v[4 * h + 2], byte) & 255) << 16) | ((unsigned)code_of_rare(v[4 * h + 3], byte) << 24);
+  }
   return r;
 }
 __device__ __forceinline__ void decode8(u32x2 c, float step, float (&v)[8]) {
@@ -120,34 +142,32 @@ __device__ __forceinline__ float hold_fp16(float y) { return y > 65504.f ? 65504
 
 // ---- activations -----------------------------------------------------------------------------------------------------
 // Phi(-a), the normal distribution's lower tail, for a in [0, 5.5]: log2 Phi(-a) is close to a parabola, and a
-// degree-8 polynomial (weighted minimax fit in Chebyshev form, weight Phi(-a) max(1, a)) followed by one exp2 is within
-// 6e-8 of Phi and of a Phi in fp32.  Past 5.5 both are under 1.1e-7 and the value at 5.5 is kept.
+// degree-6 polynomial (weighted minimax fit in Chebyshev form, weight Phi(-a) max(1, a)) followed by one exp2 is within
+// 2.1e-7 of Phi and 1.9e-7 of a Phi in fp32.  Past 5.5 both are under 1.1e-7 and the value at 5.5 is kept.  Every
+// instruction here is issued once for each element of a product's result, beside which the matrix pipe stands still:
+// degree 8 (6e-8) would be two more of about thirteen.
 __device__ __forceinline__ float phi_tail(float a) {
-  float p = -2.275866336e-06f;
-  p = __builtin_fmaf(p, a, 3.296794603e-05f);
-  p = __builtin_fmaf(p, a, -1.572784386e-04f);
-  p = __builtin_fmaf(p, a, -2.024798159e-04f);
-  p = __builtin_fmaf(p, a, 7.142783143e-03f);
-  p = __builtin_fmaf(p, a, -5.254643783e-02f);
-  p = __builtin_fmaf(p, a, -4.591930509e-01f);
-  p = __builtin_fmaf(p, a, -1.151106954e+00f);
-  p = __builtin_fmaf(p, a, -9.999999404e-01f);
+  float p = 2.503479118e-05f;
+  p = __builtin_fmaf(p, a, -6.991717964e-04f);
+  p = __builtin_fmaf(p, a, 7.853832096e-03f);
+  p = __builtin_fmaf(p, a, -5.307037011e-02f);
+  p = __builtin_fmaf(p, a, -4.590140283e-01f);
+  p = __builtin_fmaf(p, a, -1.151128888e+00f);
+  p = __builtin_fmaf(p, a, -9.999995232e-01f);
   return __builtin_amdgcn_exp2f(p);
 }
-__device__ __forceinline__ float relu_of(float x) { return x < 0.f ? 0.f : x; }      // a NaN stays one
+__device__ __forceinline__ float relu_of(float x) { return __builtin_elementwise_maximum(x, 0.f); }      // a NaN stays one
 // x Phi(x) = max(x, 0) - |x| Phi(-|x|)
 __device__ __forceinline__ float gelu_of(float x) {
   const float a = fminf(fabsf(x), 5.5f);
-  return relu_of(x) - a * phi_tail(a);
+  return __builtin_fmaf(-a, phi_tail(a), relu_of(x));
 }
-// value and derivative: Phi(x) + x phi(x), phi(x) = exp(-x^2 / 2) / sqrt(2 pi)
+// value and derivative for a decoded x (finite or NaN): Phi(x) + x phi(x), phi(x) = exp(-x^2 / 2) / sqrt(2 pi)
 __device__ __forceinline__ void gelu_both(float x, float& value, float& slope) {
-  const float ax = fabsf(x), a = fminf(ax, 5.5f), q = phi_tail(a);
-  value = relu_of(x) - a * q;
-  const float b = fminf(ax, 16.f);                         // phi(16) is 0 in fp32; keeps inf * 0 out
-  const float bell = 0.3989422804f * __builtin_amdgcn_exp2f(-0.7213475204f * b * b);
-  const float d = (x < 0.f ? q : 1.f - q) + __builtin_copysignf(b, x) * bell;
-  slope = x != x ? x : d;
+  const float a = fminf(fabsf(x), 5.5f), q = phi_tail(a);
+  value = __builtin_fmaf(-a, q, relu_of(x));
+  const float bell = __builtin_amdgcn_exp2f(x * x * -0.7213475204f);       // 0 for large x, NaN for NaN
+  slope = __builtin_fmaf(x * 0.3989422804f, bell, 0.5f + __builtin_copysignf(0.5f - q, x));
 }
 __device__ __forceinline__ float relu_slope(float x) { return x > 0.f ? 1.f : x != x ? x : 0.f; }
 

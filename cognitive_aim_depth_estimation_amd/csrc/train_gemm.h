@@ -18,6 +18,7 @@
 // an 8-bit group lie in four lanes.
 #pragma once
 #include "train_common.h"
+#include <type_traits>
 
 namespace {
 using namespace train;
@@ -48,19 +49,34 @@ __device__ __forceinline__ void dma16(unsigned lane_offset, u32x4v rsrc, unsigne
                :: "v"(lane_offset), "s"(rsrc), "s"(lds_offset) : "m0");
 }
 
-// One operand's side of the DMA: R rows (or columns), NW waves; KC: contiguous along k; WIDE: column order of B.
-template <int R, int NW, bool KC, bool WIDE> struct Stager {
+// One operand's side of the DMA: R rows (or columns), NW waves; KC: contiguous along k; WIDE: column order of B.  A wave
+// brings PIECES KiB of every K-tile, the first half of them into the part of the stage that the eight-step loop below
+// releases first: contiguous along k, the later-read rows of every wave's strip (SPLIT / 2 .. SPLIT - 1 of each SPLIT of
+// A, the others of B); contiguous across k, the first 32 k.
+template <int R, int NW, bool KC, bool WIDE, int SPLIT> struct Stager {
   static constexpr int PIECES = R / 8 / NW;
   unsigned off[PIECES], chunk[KC ? PIECES : 1];
+  unsigned dst[PIECES];
   unsigned long long base; long long left, step;      // next K-tile's first byte, bytes of the operand from there
   int k_left;                                         // k from there to the operand's end
-  unsigned lds0;
+  u32x4v rsrc;
+  __device__ __forceinline__ static int piece_of(int wave, int i) {
+    constexpr int H = PIECES / 2 < 1 ? 1 : PIECES / 2;
+    const int second = i / H, e = wave * H + i % H;   // place among the pieces of its half
+    if constexpr (KC) {
+      constexpr int P = SPLIT / 16;                   // pieces (8 rows) in half a strip
+      const int in_strip = e / P * (2 * P) + e % P;   // the first half of the strips
+      return in_strip + ((second ^ (WIDE ? 0 : 1)) ? P : 0);
+    } else {
+      return e + second * (R / 16);
+    }
+  }
   __device__ __forceinline__ void init(const void* p, long long ld, int first, int count, int K, int k0, int wave, int lane, unsigned lds) {
-    lds0 = lds + wave * PIECES * 1024;
     k_left = K - k0;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int piece = wave * PIECES + i;
+      const int piece = piece_of(wave, i);
+      dst[i] = __builtin_amdgcn_readfirstlane(lds + piece * 1024);
       if constexpr (KC) {
         const int r = piece * 8 + (lane >> 3);
         const int c = (lane & 7) ^ (WIDE ? swz_k_wide(r) : swz_k_plain(r));
@@ -83,24 +99,20 @@ template <int R, int NW, bool KC, bool WIDE> struct Stager {
       step = TK * ld * 2;
     }
   }
-  // without `live` the loads are dropped (and still counted by the wait)
-  __device__ __forceinline__ void issue(bool live, unsigned stage_lds) {
+  // the resource of the next K-tile; without `live` its loads are dropped (and still counted by the waits)
+  __device__ __forceinline__ void aim(bool live) {
     const unsigned n = live && left > 0 ? (unsigned)(left < 0x7ffffff0LL ? left : 0x7ffffff0LL) : 0u;
-    u32x4v rsrc;
     rsrc[0] = __builtin_amdgcn_readfirstlane((unsigned)base);
     rsrc[1] = __builtin_amdgcn_readfirstlane((unsigned)(base >> 32) & 0xffffu);
     rsrc[2] = __builtin_amdgcn_readfirstlane(n);
     rsrc[3] = 0x00020000u;
-    if (KC && k_left < TK) {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i)
-        dma16((int)chunk[KC ? i : 0] < k_left ? off[i] : 0xffffff00u, rsrc, __builtin_amdgcn_readfirstlane(stage_lds + lds0 + i * 1024));
-    } else {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) dma16(off[i], rsrc, __builtin_amdgcn_readfirstlane(stage_lds + lds0 + i * 1024));
-    }
-    base += step; left -= step; k_left -= TK;
   }
+  __device__ __forceinline__ void piece(int i, unsigned stage) {
+    unsigned o = off[i];
+    if (KC && k_left < TK) o = (int)chunk[KC ? i : 0] < k_left ? o : 0xffffff00u;
+    dma16(o, rsrc, __builtin_amdgcn_readfirstlane(dst[i] + stage));
+  }
+  __device__ __forceinline__ void advance() { base += step; left -= step; k_left -= TK; }
 };
 
 // eight 16-bit values of fragment data through two transposing reads (k 0-3 and 4-7 of the lane's eight)
@@ -156,7 +168,8 @@ __device__ __forceinline__ int xcd_range(int bid, int n) {
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
 }
 
-template <int BM_, int BN_, int WM_, int WN_, int ST_> struct Tile {
+template <int BM_, int BN_, int WM_, int WN_, int ST_, bool STEPS_> struct Tile {
+  static constexpr bool STEPS = STEPS_;                     // the eight-step loop
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = ST_, NW = WM_ * WN_;
   static constexpr int MI = BM_ / WM_ / 16, NJ = BN_ / WN_ / 16;
   static constexpr int STAGE = (BM_ + BN_) * TK * 2;
@@ -184,16 +197,17 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
   const int kt0 = split * g.kt_per_split;
   int nk = nk_all - kt0; nk = nk < g.kt_per_split ? nk : g.kt_per_split;        // K-tiles of this block (at least 1)
 
-  Stager<BM, TL::NW, AKC, false> sa;
-  Stager<BN, TL::NW, BKC, true> sb;
   const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+  Stager<BM, TL::NW, AKC, false, BM / TL::WM> sa;
+  Stager<BN, TL::NW, BKC, true, BN / TL::WN> sb;
   sa.init(g.A, g.lda, m0, g.rows_a, g.KA, kt0 * TK, wave, lane, lds);
   sb.init(g.B, g.ldb, n0, g.rows_b, g.KB, kt0 * TK, wave, lane, lds + BM * TK * 2);
   int issued = 0;
-  auto issue = [&](int slot) {
-    sa.issue(issued < nk, slot * TL::STAGE);
-    sb.issue(issued < nk, slot * TL::STAGE);
+  sa.aim(true); sb.aim(true);
+  auto advance = [&]() {
     ++issued;
+    sa.advance(); sb.advance();
+    sa.aim(issued < nk); sb.aim(issued < nk);
   };
   Reader<T, BM, AKC, false> ra;
   Reader<T, BN, BKC, true> rb;
@@ -211,44 +225,119 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
   constexpr int NS = SUMS ? MI / TL::WN : 1;
   static_assert(!SUMS || MI % TL::WN == 0, "row fragments are dealt evenly");
   f32x4 sums[NS];
-  v8 ones;
   const bool with_sums = SUMS && g.col_sum && tn == 0;
   if constexpr (SUMS) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ones[e] = (T)1.0f;
   }
-
+  auto add_sums = [&](const char* stage, int s) __attribute__((always_inline)) {
+    if constexpr (SUMS) {
+      if (with_sums) {
+        v8 ones;
 #pragma unroll
-  for (int p = 0; p < ST - 1; ++p) issue(p);
-  int slot = 0;
-  for (int kt = 0; kt < nk; ++kt) {
-    // this K-tile has landed (the ST - 2 younger ones may still be in flight) and this wave's reads of the slot that is
-    // refilled next are done; behind the barrier that holds for every wave
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((ST - 2) * PER_STAGE) : "memory");
-    issue(slot == 0 ? ST - 1 : slot - 1);
-    const char* as = smem + slot * TL::STAGE;
-    const char* bs = as + BM * TK * 2;
+        for (int e = 0; e < 8; ++e) ones[e] = (T)1.0f;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      v8 bf[NJ], af[MI];
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) bf[j] = rb.read(bs, j, s);
-#pragma unroll
-      for (int i = 0; i < MI; ++i) af[i] = ra.read(as, i, s);
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = H::mfma16(bf[j], af[i], acc[i][j]);
-      if constexpr (SUMS) {
-        if (with_sums) {
-#pragma unroll
-          for (int q = 0; q < NS; ++q) sums[q] = H::mfma16(ones, ra.read(as, wn * NS + q, s), sums[q]);
-        }
+        for (int q = 0; q < NS; ++q) sums[q] = H::mfma16(ones, ra.read(stage, wn * NS + q, s), sums[q]);
       }
     }
-    slot = slot == ST - 1 ? 0 : slot + 1;
+  };
+
+  if constexpr (TL::STEPS) {
+    // Two stages.  A K-tile is eight steps of 8 MFMAs, a quarter of the wave's tile at one k32 half each, ordered so that
+    // a step changes one operand; the fragments of a step are read between the MFMAs of the one before it, and the
+    // eight DMA pieces that a wave owes the K-tile after the next go out one per step, in the order in which the stage's
+    // halves fall free: the first half behind the barrier in mid-tile, the second behind the one at its end.
+    static_assert(MI == 8 && NJ == 4 && ST == 2 && decltype(sa)::PIECES == 4 && decltype(sb)::PIECES == 4, "written for 128 x 64 a wave");
+    v8 ax[4], ay[4], wa[2], wb[2];
+    unsigned fill = 0;                                       // stage the DMA fills
+    auto piece = [&](int q) __attribute__((always_inline)) {
+      if (q == 0) sa.piece(0, fill);
+      if (q == 1) sa.piece(1, fill);
+      if (q == 2) sb.piece(0, fill);
+      if (q == 3) sb.piece(1, fill);
+      if (q == 4) sa.piece(2, fill);
+      if (q == 5) sa.piece(3, fill);
+      if (q == 6) sb.piece(2, fill);
+      if (q == 7) { sb.piece(3, fill); advance(); fill ^= TL::STAGE; }
+    };
+#pragma unroll
+    for (int q = 0; q < 8; ++q) piece(q);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) piece(q);
+    asm volatile("s_waitcnt vmcnt(4)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ax[i] = ra.read(smem, i, 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) wa[j] = rb.read(smem + BM * TK * 2, j, 0);
+// one step: MFMAs of rows 4 mh_.., columns 2 nh_..; reads `load_(k)` behind the first nl_ of them, piece q_ behind the sixth
+#define TRAIN_STEP(af_, wf_, mh_, nh_, nl_, load_, q_)                                                                  \
+  _Pragma("unroll") for (int k_ = 0; k_ < 8; ++k_) {                                                                    \
+    acc[(mh_) * 4 + (k_ >> 1)][(nh_) * 2 + (k_ & 1)] =                                                                  \
+        H::mfma16(wf_[k_ & 1], af_[k_ >> 1], acc[(mh_) * 4 + (k_ >> 1)][(nh_) * 2 + (k_ & 1)]);                         \
+    if (k_ < (nl_)) { load_; }                                                                                          \
+    if (k_ == 6) piece(q_);                                                                                             \
+    __builtin_amdgcn_sched_barrier(0);                                                                                  \
+  }
+    auto ktile = [&](auto stage_c) __attribute__((always_inline)) {
+      constexpr int S0 = decltype(stage_c)::value * TL::STAGE, S1 = TL::STAGE - S0;
+      const char* const as = smem + S0;
+      const char* const bs = as + BM * TK * 2;
+      const char* const an = smem + S1;
+      const char* const bn = an + BM * TK * 2;
+      __builtin_amdgcn_sched_barrier(0);
+      TRAIN_STEP(ax, wa, 0, 0, 2, wb[k_] = rb.read(bs, 2 + k_, 0), 4)
+      add_sums(as, 0);
+      TRAIN_STEP(ax, wb, 0, 1, 4, ay[k_] = ra.read(as, 4 + k_, 0), 5)
+      TRAIN_STEP(ay, wb, 1, 1, 4, ax[k_] = ra.read(as, 4 + k_, 1), 6)
+      TRAIN_STEP(ay, wa, 1, 0, 2, wb[k_] = rb.read(bs, k_, 1), 7)
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      TRAIN_STEP(ax, wb, 1, 0, 2, wa[k_] = rb.read(bs, 2 + k_, 1), 0)
+      add_sums(as, 1);
+      TRAIN_STEP(ax, wa, 1, 1, 4, ay[k_] = ra.read(as, k_, 1), 1)
+      TRAIN_STEP(ay, wa, 0, 1, 0, , 2)
+      asm volatile("s_waitcnt vmcnt(3) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      TRAIN_STEP(ay, wb, 0, 0, 6, if (k_ < 4) ax[k_ & 3] = ra.read(an, k_, 0); else wa[k_ & 1] = rb.read(bn, k_ & 1, 0), 3)
+    };
+    for (int kt = 0; kt < nk; kt += 2) {
+      ktile(std::integral_constant<int, 0>{});
+      if (kt + 1 < nk) ktile(std::integral_constant<int, 1>{});
+    }
+#undef TRAIN_STEP
+  } else {
+    auto stage_all = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < decltype(sa)::PIECES; ++i) sa.piece(i, slot * TL::STAGE);
+#pragma unroll
+      for (int i = 0; i < decltype(sb)::PIECES; ++i) sb.piece(i, slot * TL::STAGE);
+      advance();
+    };
+#pragma unroll
+    for (int p = 0; p < ST - 1; ++p) stage_all(p);
+    int slot = 0;
+    for (int kt = 0; kt < nk; ++kt) {
+      // this K-tile has landed (the ST - 2 younger ones may still be in flight) and this wave's reads of the slot that is
+      // refilled next are done; behind the barrier that holds for every wave
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((ST - 2) * PER_STAGE) : "memory");
+      stage_all(slot == 0 ? ST - 1 : slot - 1);
+      const char* as = smem + slot * TL::STAGE;
+      const char* bs = as + BM * TK * 2;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        v8 bf[NJ], af[MI];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) bf[j] = rb.read(bs, j, s);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) af[i] = ra.read(as, i, s);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j] = H::mfma16(bf[j], af[i], acc[i][j]);
+        add_sums(as, s);
+      }
+      slot = slot == ST - 1 ? 0 : slot + 1;
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // the dropped loads past the end
   const int fr = lane & 15, fq = lane >> 4;
@@ -267,16 +356,15 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
     const int n = nw + 32 * h;
     typename Epi::Columns col;
     epi.columns(n, col);
-    typename Epi::Row next;
-    epi.template fetch<true>(mw, n, next);
+    typename Epi::Row row[MI];                               // all reads of the strip ahead of its first store
+#pragma unroll
+    for (int i = 0; i < MI; ++i) epi.template fetch<true>(mw + 16 * i, n, row[i]);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const typename Epi::Row now = next;
-      if (i + 1 < MI) epi.template fetch<true>(mw + 16 * (i + 1), n, next);   // the next row's reads go out ahead of this row's stores
       float v[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) { v[e] = acc[i][2 * h][e]; v[4 + e] = acc[i][2 * h + 1][e]; }
-      epi.template finish<true, 16, 32>(split, mw + 16 * i, n, v, col, now);
+      epi.template finish<true, 16, 32>(split, mw + 16 * i, n, v, col, row[i]);
     }
   }
 }

@@ -53,9 +53,11 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += c.b[j];
     if (codes) {
-      unsigned top = 0;
+      if constexpr (!FAST) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = umax(top, (FAST ? n : n + j) < N ? mag_bits(v[j]) : 0u);
+        for (int j = 0; j < 8; ++j) v[j] = n + j < N ? v[j] : 0.f;
+      }
+      unsigned top = n < N ? top_bits8(v) : 0u;
       top = umax(top, (unsigned)__shfl_xor((int)top, X1, 64));
       top = umax(top, (unsigned)__shfl_xor((int)top, X2, 64));
       if (m < M && n < N) {
@@ -256,9 +258,9 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(const unsigned short* __
 }
 
 // ---- plans -------------------------------------------------------------------------------------------------------
-using T256 = Tile<256, 256, 2, 4, 2>;
-using T128 = Tile<128, 128, 2, 2, 2>;
-using T64 = Tile<64, 64, 2, 2, 4>;
+using T256 = Tile<256, 256, 2, 4, 2, true>;
+using T128 = Tile<128, 128, 2, 2, 2, false>;
+using T64 = Tile<64, 64, 2, 2, 4, false>;
 
 struct Shape { int tile, tiles_m, tiles_n, splits, kt_per_split; };      // tile: 256, 128 or 64
 

@@ -63,14 +63,14 @@ template <int V> __device__ __forceinline__ unsigned group_max(unsigned m) {
 // codes and exponent byte of a thread's run (every thread of the wave calls this; `in` = the run lies in the row)
 template <int V> __device__ __forceinline__ void save_run(const float (&v)[V], bool in, signed char* codes, unsigned char* bytes,
                                                           long long row, int D, int col) {
-  unsigned m = 0;
-#pragma unroll
-  for (int j = 0; j < V; ++j) m = umax(m, mag_bits(v[j]));
+  unsigned m;
+  if constexpr (V == 8) m = top_bits8(v);
+  else m = mag_bits(v[0]);
   m = group_max<V>(in ? m : 0u);
   if (!in) return;
   const unsigned byte = group_byte(m);
   if constexpr (V == 8) *reinterpret_cast<u32x2*>(codes + row * D + col) = pack_codes(v, byte);
-  else codes[row * D + col] = (signed char)code_of(v[0], group_inverse(byte), most_code(byte));
+  else codes[row * D + col] = (signed char)code_of(v[0], byte);
   if ((col & (GROUP - 1)) == 0) bytes[row * groups_of(D) + col / GROUP] = (unsigned char)byte;
 }
 
