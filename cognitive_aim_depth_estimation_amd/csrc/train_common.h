@@ -51,6 +51,11 @@ __device__ __forceinline__ unsigned bits16(float y, int dt) {
   return __builtin_bit_cast(unsigned short, (_Float16)y);
 }
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ void pack_half8(const float (&y)[8], int dt, void* to) {       // eight 16-bit values in registers
+  const f32x8 v = {y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
+  if (dt == DT_BF16) { const bf16x8 h = __builtin_convertvector(v, bf16x8); __builtin_memcpy(to, &h, 16); }
+  else { const f16x8 h = __builtin_convertvector(v, f16x8); __builtin_memcpy(to, &h, 16); }
+}
 __device__ __forceinline__ void store_vec8(void* p, int dt, size_t off, const float (&y)[8]) {   // 16-byte aligned
   if (dt == DT_FP32) {
     float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + off);
@@ -71,6 +76,23 @@ __device__ __forceinline__ float load_one(const void* p, int dt, size_t off) {
 __device__ __forceinline__ void store_one(void* p, int dt, size_t off, float y) {
   if (dt == DT_FP32) reinterpret_cast<float*>(p)[off] = y;
   else reinterpret_cast<unsigned short*>(p)[off] = (unsigned short)bits16(y, dt);
+}
+
+// Sum over the 64 lanes, result in every lane, without the LDS permute path: rotations inside rows of 16 lanes (DPP), then
+// the two row-swap instructions of gfx950.
+__device__ __forceinline__ float wave_sum_dpp(float v) {
+#define TRAIN_ROR(ctrl_) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl_, 0xf, 0xf, false))
+  v += TRAIN_ROR(0x128);   // row_ror:8
+  v += TRAIN_ROR(0x124);   // row_ror:4
+  v += TRAIN_ROR(0x122);   // row_ror:2
+  v += TRAIN_ROR(0x121);   // row_ror:1
+#undef TRAIN_ROR
+  unsigned u = __float_as_uint(v);
+  auto s16 = __builtin_amdgcn_permlane16_swap(u, u, false, false);      // rows (0,1) and (2,3) meet
+  v = __uint_as_float(s16[0]) + __uint_as_float(s16[1]);
+  u = __float_as_uint(v);
+  auto s32 = __builtin_amdgcn_permlane32_swap(u, u, false, false);      // the two halves meet
+  return __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
 }
 
 // ---- 8-bit activations -----------------------------------------------------------------------------------------------

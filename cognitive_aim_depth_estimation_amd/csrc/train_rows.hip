@@ -7,11 +7,11 @@
 namespace {
 using namespace train;
 
-// A row lives in the registers of TPR threads.  V = 8: a thread owns runs of eight consecutive columns (16-byte
-// accesses; four neighbouring threads hold a group of 32); V = 1: single columns, neighbouring threads neighbouring
-// columns, for widths or strides that 16-byte accesses cannot serve.  NCH = runs per thread.
+// A row lives in the registers of TPR threads, NCH runs of eight consecutive columns each (runs t, t + TPR, ...; four
+// neighbouring threads hold a group of 32).  Rows may begin at any element: runs are moved with 16-byte accesses of
+// whatever alignment the row has (gfx950 takes them), and the one run that crosses a row's end element by element.
 template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
-  v = wave_sum(v);
+  v = wave_sum_dpp(v);
   if constexpr (TPR > 64) {
     __syncthreads();                                        // the previous sum's readers are done
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -23,7 +23,7 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red)
   return v;
 }
 template <int TPR> __device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
-  a = wave_sum(a); b = wave_sum(b);
+  a = wave_sum_dpp(a); b = wave_sum_dpp(b);
   if constexpr (TPR > 64) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = a; red[16 + (threadIdx.x >> 6)] = b; }
@@ -34,96 +34,147 @@ template <int TPR> __device__ __forceinline__ void row_sum2(float& a, float& b, 
   }
 }
 
-template <int V> struct Raw { Raw8 r; };
-template <> struct Raw<1> { unsigned r; };
-template <int V> __device__ __forceinline__ Raw<V> load_run(const void* p, int dt, size_t off) {
-  Raw<V> o;
-  if constexpr (V == 8) o.r = load_raw8(p, dt, off);
-  else o.r = dt == DT_FP32 ? reinterpret_cast<const unsigned*>(p)[off] : reinterpret_cast<const unsigned short*>(p)[off];
-  return o;
-}
-template <int V> __device__ __forceinline__ void cvt_run(const Raw<V>& o, int dt, float (&v)[V]) {
-  if constexpr (V == 8) cvt_raw8(o.r, dt, v);
-  else v[0] = dt == DT_FP16 ? half_bits((unsigned short)o.r) : __uint_as_float(dt == DT_FP32 ? o.r : o.r << 16);
-}
-template <int V> __device__ __forceinline__ void store_run(void* p, int dt, size_t off, const float (&y)[V]) {
-  if constexpr (V == 8) store_vec8(p, dt, off, y);
-  else store_one(p, dt, off, y[0]);
-}
-template <int V> __device__ __forceinline__ void load_f32(const float* p, int off, float (&v)[V]) {
+// Run `c .. c + 7` of a row of D elements that begins at element `row`, zeros past its end.
+template <int DT> struct Run { u32x4v w; };
+template <> struct Run<DT_FP32> { u32x4v w, v; };
+template <int DT> __device__ __forceinline__ Run<DT> load_run(const void* p, long long row, int c, int D) {
+  Run<DT> r;
+  if constexpr (DT == DT_FP32) {
+    const unsigned* q = reinterpret_cast<const unsigned*>(p) + row + c;
+    if (c + 8 <= D) { __builtin_memcpy(&r.w, q, 16); __builtin_memcpy(&r.v, q + 4, 16); }
+    else {
 #pragma unroll
-  for (int j = 0; j < V; ++j) v[j] = p[off + j];
-}
-// largest magnitude over a group of 32 columns: 32 / V neighbouring threads
-template <int V> __device__ __forceinline__ unsigned group_max(unsigned m) {
+      for (int j = 0; j < 4; ++j) { r.w[j] = c + j < D ? q[j] : 0u; r.v[j] = c + 4 + j < D ? q[4 + j] : 0u; }
+    }
+  } else {
+    const unsigned short* q = reinterpret_cast<const unsigned short*>(p) + row + c;
+    if (c + 8 <= D) __builtin_memcpy(&r.w, q, 16);
+    else {
 #pragma unroll
-  for (int o = 1; o < 32 / V; o <<= 1) m = umax(m, (unsigned)__shfl_xor((int)m, o, 64));
-  return m;
+      for (int j = 0; j < 4; ++j) r.w[j] = (c + 2 * j < D ? (unsigned)q[2 * j] : 0u) | (c + 2 * j + 1 < D ? (unsigned)q[2 * j + 1] << 16 : 0u);
+    }
+  }
+  return r;
 }
-// codes and exponent byte of a thread's run (every thread of the wave calls this; `in` = the run lies in the row)
-template <int V> __device__ __forceinline__ void save_run(const float (&v)[V], bool in, signed char* codes, unsigned char* bytes,
-                                                          long long row, int D, int col) {
-  unsigned m;
-  if constexpr (V == 8) m = top_bits8(v);
-  else m = mag_bits(v[0]);
-  m = group_max<V>(in ? m : 0u);
-  if (!in) return;
+template <int DT> __device__ __forceinline__ void cvt_run(const Run<DT>& r, float (&v)[8]) {
+  if constexpr (DT == DT_FP32) cvt_raw8(Raw8{r.w, r.v}, DT, v);
+  else cvt_raw8(Raw8{r.w, r.w}, DT, v);
+}
+// the same of a type known at run time (uniform over the launch)
+typedef Raw8 AnyRun;
+__device__ __forceinline__ AnyRun load_any(const void* p, int dt, long long row, int c, int D) {
+  if (dt == DT_FP32) {
+    const Run<DT_FP32> r = load_run<DT_FP32>(p, row, c, D);
+    return AnyRun{r.w, r.v};
+  }
+  const Run<DT_BF16> r = load_run<DT_BF16>(p, row, c, D);
+  return AnyRun{r.w, r.w};
+}
+__device__ __forceinline__ void cvt_any(const AnyRun& o, int dt, float (&v)[8]) { cvt_raw8(o, dt, v); }
+__device__ __forceinline__ void store_any(void* p, int dt, long long row, int c, int D, const float (&y)[8]) {
+  if (dt == DT_FP32) {
+    float* q = reinterpret_cast<float*>(p) + row + c;
+    if (c + 8 <= D) __builtin_memcpy(q, y, 32);
+    else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) if (c + j < D) q[j] = y[j];
+    }
+  } else {
+    unsigned short* q = reinterpret_cast<unsigned short*>(p) + row + c;
+    unsigned short h[8];
+    pack_half8(y, dt, h);
+    if (c + 8 <= D) __builtin_memcpy(q, h, 16);
+    else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) if (c + j < D) q[j] = h[j];
+    }
+  }
+}
+__device__ __forceinline__ u32x2 load_codes(const signed char* row, int c, int D) {
+  u32x2 q = {0, 0};
+  if (c + 8 <= D) __builtin_memcpy(&q, row + c, 8);
+  else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (c + j < D) q[j >> 2] |= (unsigned)(unsigned char)row[c + j] << (8 * (j & 3));
+  }
+  return q;
+}
+__device__ __forceinline__ void load_f32(const float* p, int c, int D, float (&v)[8]) {
+  cvt_run<DT_FP32>(load_run<DT_FP32>(p, 0, c, D), v);
+}
+// codes and exponent byte of a thread's run; all four threads of a group call this together, with zeros past the row's end
+__device__ __forceinline__ void save_run(const float (&v)[8], signed char* codes, unsigned char* bytes, long long row, int D, int c) {
+  unsigned m = top_bits8(v);
+  m = umax(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0xB1 /* quad_perm [1,0,3,2] */, 0xf, 0xf, true));
+  m = umax(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x4E /* quad_perm [2,3,0,1] */, 0xf, 0xf, true));
+  if (c >= D) return;
   const unsigned byte = group_byte(m);
-  if constexpr (V == 8) *reinterpret_cast<u32x2*>(codes + row * D + col) = pack_codes(v, byte);
-  else codes[row * D + col] = (signed char)code_of(v[0], byte);
-  if ((col & (GROUP - 1)) == 0) bytes[row * groups_of(D) + col / GROUP] = (unsigned char)byte;
+  const u32x2 q = pack_codes(v, byte);
+  signed char* to = codes + row * D + c;
+  if (c + 8 <= D) __builtin_memcpy(to, &q, 8);
+  else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (c + j < D) to[j] = (signed char)(q[j >> 2] >> (8 * (j & 3)));
+  }
+  if ((c & (GROUP - 1)) == 0) bytes[row * groups_of(D) + c / GROUP] = (unsigned char)byte;
 }
 
 struct LnFwd {
   const void* x; const float* gamma; const float* beta; void* y; float* mean; float* rstd;
-  signed char* codes; unsigned char* bytes; long long ldx, ldy; int M, D, x_dt, y_dt; float eps;
+  signed char* codes; unsigned char* bytes; long long ldx, ldy; int M, D, y_dt; float eps;
 };
 
-template <int V, int TPR, int NCH>
+template <int XDT, int TPR, int NCH>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_fwd_kernel(LnFwd a) {
   __shared__ float red[32];
   const int t = threadIdx.x & (TPR - 1);
   constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
   const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
   if (RPB > 1 && row >= a.M) return;                        // whole waves: a row per wave
-  Raw<V> raw[NCH];
+  Run<XDT> raw[NCH];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int c = (t + TPR * i) * V;
-    if (c < a.D) raw[i] = load_run<V>(a.x, a.x_dt, row * a.ldx + c);
+    const int c = (t + TPR * i) * 8;
+    if (c < a.D) raw[i] = load_run<XDT>(a.x, row * a.ldx, c, a.D);
   }
-  float v[NCH][V];
+  float v[NCH][8];
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const bool in = (t + TPR * i) * V < a.D;
-    if (in) cvt_run<V>(raw[i], a.x_dt, v[i]);
+    const int c = (t + TPR * i) * 8;
+    if (c < a.D) cvt_run<XDT>(raw[i], v[i]);
+    else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) { v[i][j] = in ? v[i][j] : 0.f; sum += v[i][j]; }
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += v[i][j];
   }
   const float mean = row_sum<TPR>(sum, red) / (float)a.D;
   float sq = 0.f;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const bool in = (t + TPR * i) * V < a.D;
+    const int c = (t + TPR * i) * 8;
 #pragma unroll
-    for (int j = 0; j < V; ++j) { v[i][j] = in ? v[i][j] - mean : 0.f; sq += v[i][j] * v[i][j]; }
+    for (int j = 0; j < 8; ++j) {
+      v[i][j] = c + j < a.D ? v[i][j] - mean : 0.f;
+      sq = __builtin_fmaf(v[i][j], v[i][j], sq);
+    }
   }
   const float rstd = 1.f / sqrtf(row_sum<TPR>(sq, red) / (float)a.D + a.eps);
   if (t == 0) { a.mean[row] = mean; a.rstd[row] = rstd; }
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int c = (t + TPR * i) * V;
-    const bool in = c < a.D;
+    const int c = (t + TPR * i) * 8;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[i][j] *= rstd;
-    if (a.codes) save_run<V>(v[i], in, a.codes, a.bytes, row, a.D, c);
-    if (in) {
-      float g[V], b[V], y[V];
-      load_f32<V>(a.gamma, c, g); load_f32<V>(a.beta, c, b);
+    for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
+    if (a.codes) save_run(v[i], a.codes, a.bytes, row, a.D, c);
+    if (c < a.D) {
+      float g[8], b[8], y[8];
+      load_f32(a.gamma, c, a.D, g); load_f32(a.beta, c, a.D, b);
 #pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = __builtin_fmaf(v[i][j], g[j], b[j]);
-      store_run<V>(a.y, a.y_dt, row * a.ldy + c, y);
+      for (int j = 0; j < 8; ++j) y[j] = __builtin_fmaf(v[i][j], g[j], b[j]);
+      store_any(a.y, a.y_dt, row * a.ldy, c, a.D, y);
     }
   }
 }
@@ -135,59 +186,59 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_fwd_kernel(LnF
 struct LnBwd {
   const void* dy; const void* x; const signed char* codes; const unsigned char* bytes; const float* mean; const float* rstd;
   const float* gamma; const void* add; void* dx; float* part;
-  long long lddy, ldx, ldadd, lddx; int M, D, dy_dt, x_dt, add_dt, dx_dt;
+  long long lddy, ldx, ldadd, lddx; int M, D, add_dt, dx_dt;
 };
 
-template <int V, int TPR, int NCH>
+constexpr int SRC_CODES = 3;               // the rows come from their 8-bit copy
+template <int DYT, int SRC, int TPR, int NCH>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnBwd a) {
   constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
+  constexpr int XDT = SRC == SRC_CODES ? DT_BF16 : SRC;
   __shared__ float red[32];
-  __shared__ float acc[RPB > 1 ? RPB * TPR * NCH * V : 1];
+  __shared__ float acc[RPB > 1 ? RPB * TPR * NCH * 8 : 1];
   const int t = threadIdx.x & (TPR - 1), sub = threadIdx.x / TPR;
-  float dg[NCH][V], db[NCH][V];
+  float dg[NCH][8], db[NCH][8];
 #pragma unroll
   for (int i = 0; i < NCH; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) { dg[i][j] = 0.f; db[i][j] = 0.f; }
+    for (int j = 0; j < 8; ++j) { dg[i][j] = 0.f; db[i][j] = 0.f; }
   const long long groups = groups_of(a.D);
   for (long long row = (long long)blockIdx.x * RPB + sub; row < a.M; row += (long long)gridDim.x * RPB) {
-    Raw<V> rdy[NCH], rx[NCH];
+    Run<DYT> rdy[NCH];
+    Run<XDT> rx[NCH];
     u32x2 rc[NCH];
     unsigned rb[NCH];
+    AnyRun radd[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (t + TPR * i) * V;
+      const int c = (t + TPR * i) * 8;
       if (c < a.D) {
-        rdy[i] = load_run<V>(a.dy, a.dy_dt, row * a.lddy + c);
-        if (a.codes) {
-          if constexpr (V == 8) rc[i] = *reinterpret_cast<const u32x2*>(a.codes + row * a.D + c);
-          else rc[i][0] = (unsigned char)a.codes[row * a.D + c];
+        rdy[i] = load_run<DYT>(a.dy, row * a.lddy, c, a.D);
+        if constexpr (SRC == SRC_CODES) {
+          rc[i] = load_codes(a.codes + row * a.D, c, a.D);
           rb[i] = a.bytes[row * groups + c / GROUP];
-        } else rx[i] = load_run<V>(a.x, a.x_dt, row * a.ldx + c);
+        } else rx[i] = load_run<XDT>(a.x, row * a.ldx, c, a.D);
+        if (a.add) radd[i] = load_any(a.add, a.add_dt, row * a.ldadd, c, a.D);
       }
     }
-    const float rstd = a.rstd[row], mean = a.codes ? 0.f : a.mean[row];
-    float g[NCH][V], h[NCH][V];
+    const float rstd = a.rstd[row], mean = SRC == SRC_CODES ? 0.f : a.mean[row];
+    float g[NCH][8], h[NCH][8];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (t + TPR * i) * V;
-      const bool in = c < a.D;
-      if (in) {
-        float dy[V], gm[V];
-        cvt_run<V>(rdy[i], a.dy_dt, dy);
-        if (a.codes) {
-          const float step = group_step(rb[i]);
-          if constexpr (V == 8) decode8(rc[i], step, h[i]);
-          else h[i][0] = (float)(signed char)rc[i][0] * step;
-        } else {
-          cvt_run<V>(rx[i], a.x_dt, h[i]);
+      const int c = (t + TPR * i) * 8;
+      if (c < a.D) {
+        float dy[8], gm[8];
+        cvt_run<DYT>(rdy[i], dy);
+        if constexpr (SRC == SRC_CODES) decode8(rc[i], group_step(rb[i]), h[i]);
+        else {
+          cvt_run<XDT>(rx[i], h[i]);
 #pragma unroll
-          for (int j = 0; j < V; ++j) h[i][j] = (h[i][j] - mean) * rstd;
+          for (int j = 0; j < 8; ++j) h[i][j] = (h[i][j] - mean) * rstd;
         }
-        load_f32<V>(a.gamma, c, gm);
+        load_f32(a.gamma, c, a.D, gm);                      // zeros past the row's end: g is zero there, as dy is
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
+        for (int j = 0; j < 8; ++j) {
           dg[i][j] = __builtin_fmaf(dy[j], h[i][j], dg[i][j]);
           db[i][j] += dy[j];
           g[i][j] = dy[j] * gm[j];
@@ -200,19 +251,18 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnB
     s1 /= (float)a.D; s2 /= (float)a.D;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (t + TPR * i) * V;
+      const int c = (t + TPR * i) * 8;
       if (c < a.D) {
-        float o[V];
+        float o[8];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = rstd * (g[i][j] - s1 - h[i][j] * s2);
+        for (int j = 0; j < 8; ++j) o[j] = rstd * (g[i][j] - s1 - h[i][j] * s2);
         if (a.add) {
-          const Raw<V> ra = load_run<V>(a.add, a.add_dt, row * a.ldadd + c);
-          float ad[V];
-          cvt_run<V>(ra, a.add_dt, ad);
+          float ad[8];
+          cvt_any(radd[i], a.add_dt, ad);
 #pragma unroll
-          for (int j = 0; j < V; ++j) o[j] += ad[j];
+          for (int j = 0; j < 8; ++j) o[j] += ad[j];
         }
-        store_run<V>(a.dx, a.dx_dt, row * a.lddx + c, o);
+        store_any(a.dx, a.dx_dt, row * a.lddx, c, a.D, o);
       }
     }
   }
@@ -225,28 +275,23 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnB
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) acc[((sub * NCH + i) * V + j) * TPR + t] = which ? db[i][j] : dg[i][j];
+        for (int j = 0; j < 8; ++j) acc[((sub * NCH + i) * 8 + j) * TPR + t] = which ? db[i][j] : dg[i][j];
       __syncthreads();
+      // columns dealt to all threads; value (run, j) of thread run % TPR lies at run / TPR
+      for (int c = threadIdx.x; c < a.D; c += RPB * TPR) {
+        const int run = c >> 3, at = ((run / TPR) * 8 + (c & 7)) * TPR + (run & (TPR - 1));
+        float s = acc[at];
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        const int c = (t + TPR * i) * V;
-        if (c < a.D && sub == (i & (RPB - 1))) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            float s = acc[(i * V + j) * TPR + t];
-#pragma unroll
-            for (int w = 1; w < RPB; ++w) s += acc[((w * NCH + i) * V + j) * TPR + t];
-            out[which * a.D + c + j] = s;
-          }
-        }
+        for (int w = 1; w < RPB; ++w) s += acc[w * NCH * 8 * TPR + at];
+        out[which * a.D + c] = s;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const int c = (t + TPR * i) * V;
-        if (c < a.D)
+        const int c = (t + TPR * i) * 8;
 #pragma unroll
-          for (int j = 0; j < V; ++j) out[which * a.D + c + j] = which ? db[i][j] : dg[i][j];
+        for (int j = 0; j < 8; ++j)
+          if (c + j < a.D) out[which * a.D + c + j] = which ? db[i][j] : dg[i][j];
       }
     }
   }
@@ -290,118 +335,119 @@ struct Walk {
   }
 };
 
-// x [M, D] -> codes [M, D], bytes [M, groups].  32 / V neighbouring threads per group.
-template <int V>
-__global__ __launch_bounds__(256) void pack8_kernel(const void* __restrict__ x, int dt, long long ldx,
-                                                    signed char* __restrict__ codes, unsigned char* __restrict__ bytes,
-                                                    int M, int D) {
-  const unsigned per_row = (unsigned)groups_of(D) * (GROUP / V);
-  const unsigned long long total = (unsigned long long)M * per_row;
-  // rounded up to whole waves: every lane of a wave takes part in its group's maximum
-  const unsigned long long rounded = (total + 63) / 64 * 64;
-  for (Walk w(per_row); w.i < rounded; w.step()) {
-    const unsigned long long row = w.row;
-    const int c = (int)w.run * V;
-    const bool in = w.i < total && c < D;
-    float v[V];
-    if (in) {
-      const Raw<V> r = load_run<V>(x, dt, row * ldx + c);
-      cvt_run<V>(r, dt, v);
-    } else {
+// x [M, D] -> codes [M, D], bytes [M, groups].  Four neighbouring threads per group, a row's last group whole.
+template <int DT>
+__global__ __launch_bounds__(256) void pack8_kernel(const void* __restrict__ x, long long ldx, signed char* __restrict__ codes,
+                                                    unsigned char* __restrict__ bytes, int M, int D) {
+  for (Walk w((unsigned)groups_of(D) * 4); w.row < (unsigned long long)M; w.step()) {     // a group's threads leave together
+    const int c = (int)w.run * 8;
+    float v[8];
+    if (c < D) cvt_run<DT>(load_run<DT>(x, (long long)w.row * ldx, c, D), v);
+    else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = 0.f;
+      for (int j = 0; j < 8; ++j) v[j] = 0.f;
     }
-    save_run<V>(v, in, codes, bytes, (long long)row, D, c);
+    save_run(v, codes, bytes, (long long)w.row, D, c);
   }
 }
 
 // codes [M, D] -> out [M, width >= D] (columns past D are written as zero)
-template <int V>
+template <int DT>
 __global__ __launch_bounds__(256) void unpack8_kernel(const signed char* __restrict__ codes,
                                                       const unsigned char* __restrict__ bytes, void* __restrict__ out,
-                                                      int dt, long long ldo, int M, int D, int width) {
-  const unsigned per_row = (unsigned)(width + V - 1) / V;
-  const unsigned long long total = (unsigned long long)M * per_row;
+                                                      long long ldo, int M, int D, int width) {
   const long long groups = groups_of(D);
-  for (Walk w(per_row); w.i < total; w.step()) {
-    const unsigned long long row = w.row;
-    const int c = (int)w.run * V;
-    float v[V];
+  for (Walk w((unsigned)(width + 7) / 8); w.row < (unsigned long long)M; w.step()) {
+    const long long row = (long long)w.row;
+    const int c = (int)w.run * 8;
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = 0.f;
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
     if (c < D) {
-      const float step = group_step(bytes[row * groups + c / GROUP]);
-      if constexpr (V == 8) decode8(*reinterpret_cast<const u32x2*>(codes + row * D + c), step, v);
-      else v[0] = (float)codes[row * D + c] * step;
-      if (dt == DT_FP16) {
+      const u32x2 q = load_codes(codes + row * D, c, D);
+      float u[8];
+      decode8(q, group_step(bytes[row * groups + c / GROUP]), u);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = hold_fp16(v[j]);
+      for (int j = 0; j < 8; ++j) {
+        if (DT == DT_FP16) u[j] = hold_fp16(u[j]);
+        v[j] = c + j < D ? u[j] : 0.f;
       }
     }
-    store_run<V>(out, dt, row * ldo + c, v);
+    store_any(out, DT, row * ldo, c, width, v);
   }
 }
 
 // du = dy * act'(u), u from its 8-bit copy
-template <int V>
-__global__ __launch_bounds__(256) void act_bwd_kernel(const void* __restrict__ dy, int dy_dt, long long lddy,
+template <int DT>
+__global__ __launch_bounds__(256) void act_bwd_kernel(const void* __restrict__ dy, long long lddy,
                                                       const signed char* __restrict__ codes,
                                                       const unsigned char* __restrict__ bytes, void* __restrict__ du,
                                                       int du_dt, long long lddu, int act, int M, int D) {
-  const unsigned per_row = (unsigned)(D + V - 1) / V;
-  const unsigned long long total = (unsigned long long)M * per_row;
   const long long groups = groups_of(D);
-  for (Walk w(per_row); w.i < total; w.step()) {
-    const unsigned long long row = w.row;
-    const int c = (int)w.run * V;
-    const Raw<V> r = load_run<V>(dy, dy_dt, row * lddy + c);
-    const float step = group_step(bytes[row * groups + c / GROUP]);
-    float u[V], g[V];
-    if constexpr (V == 8) decode8(*reinterpret_cast<const u32x2*>(codes + row * D + c), step, u);
-    else u[0] = (float)codes[row * D + c] * step;
-    cvt_run<V>(r, dy_dt, g);
+  for (Walk w((unsigned)(D + 7) / 8); w.row < (unsigned long long)M; w.step()) {
+    const long long row = (long long)w.row;
+    const int c = (int)w.run * 8;
+    const Run<DT> r = load_run<DT>(dy, row * lddy, c, D);
+    const u32x2 q = load_codes(codes + row * D, c, D);
+    float u[8], g[8];
+    decode8(q, group_step(bytes[row * groups + c / GROUP]), u);
+    cvt_run<DT>(r, g);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
+    for (int j = 0; j < 8; ++j) {
       float value, slope;
       if (act == ACT_GELU) gelu_both(u[j], value, slope);
       else slope = relu_slope(u[j]);
       g[j] *= slope;
     }
-    store_run<V>(du, du_dt, row * lddu + c, g);
+    store_any(du, du_dt, row * lddu, c, D, g);
   }
 }
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 bool dt_ok(int dt) { return dt >= 0 && dt <= 2; }
-// may eight elements at a time be moved with 16-byte accesses?
-bool vec_rows(const void* p, long long ld) { return aligned(p, 16) && (ld & 7) == 0; }
 unsigned blocks_for(unsigned long long threads) {
   const unsigned long long b = (threads + 255) / 256;
   return (unsigned)(b > 256 * 32 ? 256 * 32 : b);
 }
 constexpr int LN_MAX_D = 16384;
 // blocks of the backward kernel: 16 waves a CU keep enough rows in flight; each leaves a partial row of 2 D floats
-int ln_bwd_blocks(int M, int D, bool vec) {
-  const int rpb = (vec ? D <= 2048 : D <= 1024) ? 4 : 1;
+int ln_bwd_blocks(int M, int D) {
+  const int rpb = D <= 1024 ? 4 : 1, most = D <= 8192 ? 1024 : 512;
   const long long want = ((long long)M + rpb - 1) / rpb;
-  return (int)(want < 1024 ? want : 1024);
+  return (int)(want < most ? want : most);
+}
+template <int XDT> void run_ln_fwd(const LnFwd& a, hipStream_t st) {
+#define LN_LAUNCH(TPR_, NCH_, RPB_, TH_) hipLaunchKernelGGL((ln_train_fwd_kernel<XDT, TPR_, NCH_>), dim3((unsigned)(((long long)a.M + RPB_ - 1) / RPB_)), dim3(TH_), 0, st, a)
+#define LN_BY_WIDTH(D_)                              \
+  if (D_ <= 512) LN_LAUNCH(64, 1, 4, 256);           \
+  else if (D_ <= 1024) LN_LAUNCH(64, 2, 4, 256);     \
+  else if (D_ <= 2048) LN_LAUNCH(256, 1, 1, 256);    \
+  else if (D_ <= 4096) LN_LAUNCH(256, 2, 1, 256);    \
+  else if (D_ <= 8192) LN_LAUNCH(1024, 1, 1, 1024);  \
+  else LN_LAUNCH(1024, 2, 1, 1024);
+  LN_BY_WIDTH(a.D)
+#undef LN_LAUNCH
+}
+template <int DYT, int SRC> void run_ln_bwd(const LnBwd& a, int blocks, hipStream_t st) {
+#define LN_LAUNCH(TPR_, NCH_, RPB_, TH_) hipLaunchKernelGGL((ln_train_bwd_kernel<DYT, SRC, TPR_, NCH_>), dim3(blocks), dim3(TH_), 0, st, a)
+  LN_BY_WIDTH(a.D)
+#undef LN_LAUNCH
+}
+template <int DYT> void run_ln_bwd_from(const LnBwd& a, int x_dt, int blocks, hipStream_t st) {
+  if (a.codes) run_ln_bwd<DYT, SRC_CODES>(a, blocks, st);
+  else if (x_dt == DT_BF16) run_ln_bwd<DYT, DT_BF16>(a, blocks, st);
+  else if (x_dt == DT_FP16) run_ln_bwd<DYT, DT_FP16>(a, blocks, st);
+  else run_ln_bwd<DYT, DT_FP32>(a, blocks, st);
 }
 }  // namespace
 
-#define LN_BY_WIDTH(KERNEL, LAUNCH)                                                                     \
-  if (vec) {                                                                                            \
-    if (D <= 512) LAUNCH((KERNEL<8, 64, 1>), 4, 256)                                                    \
-    else if (D <= 1024) LAUNCH((KERNEL<8, 64, 2>), 4, 256)                                              \
-    else if (D <= 2048) LAUNCH((KERNEL<8, 64, 4>), 4, 256)                                              \
-    else if (D <= 4096) LAUNCH((KERNEL<8, 256, 2>), 1, 256)                                             \
-    else if (D <= 8192) LAUNCH((KERNEL<8, 256, 4>), 1, 256)                                             \
-    else LAUNCH((KERNEL<8, 1024, 2>), 1, 1024)                                                          \
-  } else {                                                                                              \
-    if (D <= 256) LAUNCH((KERNEL<1, 64, 4>), 4, 256)                                                    \
-    else if (D <= 1024) LAUNCH((KERNEL<1, 64, 16>), 4, 256)                                             \
-    else if (D <= 4096) LAUNCH((KERNEL<1, 256, 16>), 1, 256)                                            \
-    else LAUNCH((KERNEL<1, 1024, 16>), 1, 1024)                                                         \
-  }
+// KERNEL<type> launched for a run-time type
+#define BY_TYPE(DT_, KERNEL_, ...)                                                     \
+  do {                                                                                 \
+    if ((DT_) == DT_BF16) hipLaunchKernelGGL(KERNEL_<DT_BF16>, __VA_ARGS__);           \
+    else if ((DT_) == DT_FP16) hipLaunchKernelGGL(KERNEL_<DT_FP16>, __VA_ARGS__);      \
+    else hipLaunchKernelGGL(KERNEL_<DT_FP32>, __VA_ARGS__);                            \
+  } while (0)
 
 extern "C" {
 
@@ -412,11 +458,10 @@ int cogaim_layernorm_train_fwd(const void* x, int x_dtype, long long ldx, const 
       !beta || !y || !mean || !rstd || !codes != !exponents || !(eps >= 0.f) || !aligned(x, dt_size(x_dtype)) ||
       !aligned(y, dt_size(y_dtype)))
     return COGAIM_EINVAL;
-  const bool vec = (D & 7) == 0 && vec_rows(x, ldx) && vec_rows(y, ldy) && aligned(codes, 8);
-  const LnFwd a{x, gamma, beta, y, mean, rstd, (signed char*)codes, (unsigned char*)exponents, ldx, ldy, M, D, x_dtype, y_dtype, eps};
-#define LN_LAUNCH(K_, RPB_, TH_) hipLaunchKernelGGL(K_, dim3((unsigned)(((long long)M + RPB_ - 1) / RPB_)), dim3(TH_), 0, (hipStream_t)stream, a);
-  LN_BY_WIDTH(ln_train_fwd_kernel, LN_LAUNCH)
-#undef LN_LAUNCH
+  const LnFwd a{x, gamma, beta, y, mean, rstd, (signed char*)codes, (unsigned char*)exponents, ldx, ldy, M, D, y_dtype, eps};
+  if (x_dtype == DT_BF16) run_ln_fwd<DT_BF16>(a, (hipStream_t)stream);
+  else if (x_dtype == DT_FP16) run_ln_fwd<DT_FP16>(a, (hipStream_t)stream);
+  else run_ln_fwd<DT_FP32>(a, (hipStream_t)stream);
   return COGAIM_LAUNCH_CHECK();
 }
 
@@ -438,14 +483,12 @@ int cogaim_layernorm_bwd(const void* dy, int dy_dtype, long long lddy, const voi
   if (!aligned(dy, dt_size(dy_dtype)) || !aligned(dx, dt_size(dx_dtype)) || !aligned(workspace, 4) ||
       workspace_bytes < cogaim_layernorm_bwd_workspace_bytes(M, D))
     return COGAIM_EINVAL;
-  const bool vec = (D & 7) == 0 && vec_rows(dy, lddy) && vec_rows(dx, lddx) && (x ? vec_rows(x, ldx) : aligned(codes, 8)) &&
-                   (!add || vec_rows(add, ldadd));
   const LnBwd a{dy, x, (const signed char*)codes, (const unsigned char*)exponents, mean, rstd, gamma, add, dx,
-                (float*)workspace, lddy, ldx, ldadd, lddx, M, D, dy_dtype, x_dtype, add_dtype, dx_dtype};
-  const int nblk = ln_bwd_blocks(M, D, vec);
-#define LN_LAUNCH(K_, RPB_, TH_) hipLaunchKernelGGL(K_, dim3(nblk), dim3(TH_), 0, (hipStream_t)stream, a);
-  LN_BY_WIDTH(ln_train_bwd_kernel, LN_LAUNCH)
-#undef LN_LAUNCH
+                (float*)workspace, lddy, ldx, ldadd, lddx, M, D, add_dtype, dx_dtype};
+  const int nblk = ln_bwd_blocks(M, D);
+  if (dy_dtype == DT_BF16) run_ln_bwd_from<DT_BF16>(a, x_dtype, nblk, (hipStream_t)stream);
+  else if (dy_dtype == DT_FP16) run_ln_bwd_from<DT_FP16>(a, x_dtype, nblk, (hipStream_t)stream);
+  else run_ln_bwd_from<DT_FP32>(a, x_dtype, nblk, (hipStream_t)stream);
   hipLaunchKernelGGL(ln_train_reduce_kernel, dim3((2 * D + 31) / 32), dim3(1024), 0, (hipStream_t)stream,
                      (const float*)workspace, dgamma, dbeta, nblk, D);
   return COGAIM_LAUNCH_CHECK();
@@ -454,10 +497,8 @@ int cogaim_layernorm_bwd(const void* dy, int dy_dtype, long long lddy, const voi
 int cogaim_pack8(const void* x, int x_dtype, long long ldx, void* codes, void* exponents, int M, int D, void* stream) {
   if (M <= 0 || D <= 0 || !dt_ok(x_dtype) || ldx < D || !x || !codes || !exponents || !aligned(x, dt_size(x_dtype)))
     return COGAIM_EINVAL;
-  const bool vec = (D & 7) == 0 && vec_rows(x, ldx) && aligned(codes, 8);
-  const unsigned long long threads = (unsigned long long)M * groups_of(D) * (vec ? 4 : 32);
-  if (vec) hipLaunchKernelGGL(pack8_kernel<8>, dim3(blocks_for(threads)), dim3(256), 0, (hipStream_t)stream, x, x_dtype, ldx, (signed char*)codes, (unsigned char*)exponents, M, D);
-  else hipLaunchKernelGGL(pack8_kernel<1>, dim3(blocks_for(threads)), dim3(256), 0, (hipStream_t)stream, x, x_dtype, ldx, (signed char*)codes, (unsigned char*)exponents, M, D);
+  BY_TYPE(x_dtype, pack8_kernel, dim3(blocks_for((unsigned long long)M * groups_of(D) * 4)), dim3(256), 0, (hipStream_t)stream, x, ldx,
+          (signed char*)codes, (unsigned char*)exponents, M, D);
   return COGAIM_LAUNCH_CHECK();
 }
 
@@ -466,10 +507,8 @@ int cogaim_unpack8(const void* codes, const void* exponents, void* out, int out_
   if (M <= 0 || D <= 0 || width < D || !dt_ok(out_dtype) || ldo < width || !codes || !exponents || !out ||
       !aligned(out, dt_size(out_dtype)))
     return COGAIM_EINVAL;
-  const bool vec = (D & 7) == 0 && (width & 7) == 0 && vec_rows(out, ldo) && aligned(codes, 8);
-  const unsigned long long threads = (unsigned long long)M * (vec ? width / 8 : width);
-  if (vec) hipLaunchKernelGGL(unpack8_kernel<8>, dim3(blocks_for(threads)), dim3(256), 0, (hipStream_t)stream, (const signed char*)codes, (const unsigned char*)exponents, out, out_dtype, ldo, M, D, width);
-  else hipLaunchKernelGGL(unpack8_kernel<1>, dim3(blocks_for(threads)), dim3(256), 0, (hipStream_t)stream, (const signed char*)codes, (const unsigned char*)exponents, out, out_dtype, ldo, M, D, width);
+  BY_TYPE(out_dtype, unpack8_kernel, dim3(blocks_for((unsigned long long)M * ((width + 7LL) / 8))), dim3(256), 0, (hipStream_t)stream,
+          (const signed char*)codes, (const unsigned char*)exponents, out, ldo, M, D, width);
   return COGAIM_LAUNCH_CHECK();
 }
 
@@ -479,10 +518,8 @@ int cogaim_activation_bwd(const void* dy, int dy_dtype, long long lddy, const vo
       !du || (activation != ACT_RELU && activation != ACT_GELU) || !aligned(dy, dt_size(dy_dtype)) ||
       !aligned(du, dt_size(du_dtype)))
     return COGAIM_EINVAL;
-  const bool vec = (D & 7) == 0 && vec_rows(dy, lddy) && vec_rows(du, lddu) && aligned(codes, 8);
-  const unsigned long long threads = (unsigned long long)M * (vec ? D / 8 : D);
-  if (vec) hipLaunchKernelGGL(act_bwd_kernel<8>, dim3(blocks_for(threads)), dim3(256), 0, (hipStream_t)stream, dy, dy_dtype, lddy, (const signed char*)codes, (const unsigned char*)exponents, du, du_dtype, lddu, activation, M, D);
-  else hipLaunchKernelGGL(act_bwd_kernel<1>, dim3(blocks_for(threads)), dim3(256), 0, (hipStream_t)stream, dy, dy_dtype, lddy, (const signed char*)codes, (const unsigned char*)exponents, du, du_dtype, lddu, activation, M, D);
+  BY_TYPE(dy_dtype, act_bwd_kernel, dim3(blocks_for((unsigned long long)M * ((D + 7LL) / 8))), dim3(256), 0, (hipStream_t)stream, dy, lddy,
+          (const signed char*)codes, (const unsigned char*)exponents, du, du_dtype, lddu, activation, M, D);
   return COGAIM_LAUNCH_CHECK();
 }
 
