@@ -51,10 +51,15 @@ __device__ __forceinline__ unsigned bits16(float y, int dt) {
   return __builtin_bit_cast(unsigned short, (_Float16)y);
 }
 typedef float f32x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ void pack_half8(const float (&y)[8], int dt, void* to) {       // eight 16-bit values in registers
-  const f32x8 v = {y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
-  if (dt == DT_BF16) { const bf16x8 h = __builtin_convertvector(v, bf16x8); __builtin_memcpy(to, &h, 16); }
-  else { const f16x8 h = __builtin_convertvector(v, f16x8); __builtin_memcpy(to, &h, 16); }
+template <int V> __device__ __forceinline__ void pack_half(const float (&y)[V], int dt, void* to) {       // V 16-bit values in registers
+  typedef float fv __attribute__((ext_vector_type(V)));
+  typedef __bf16 bv __attribute__((ext_vector_type(V)));
+  typedef _Float16 hv __attribute__((ext_vector_type(V)));
+  fv v;
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = y[i];
+  if (dt == DT_BF16) { const bv h = __builtin_convertvector(v, bv); __builtin_memcpy(to, &h, 2 * V); }
+  else { const hv h = __builtin_convertvector(v, hv); __builtin_memcpy(to, &h, 2 * V); }
 }
 __device__ __forceinline__ void store_vec8(void* p, int dt, size_t off, const float (&y)[8]) {   // 16-byte aligned
   if (dt == DT_FP32) {
@@ -115,12 +120,12 @@ __device__ __forceinline__ float group_step(unsigned byte) {
 }
 __device__ __forceinline__ unsigned mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 __device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
-// Largest magnitude of eight values as bits, NaN above all: `maximum` passes a NaN on (v_maximum3_f32, two values an
+// Largest magnitude of V values as bits, NaN above all: `maximum` passes a NaN on (v_maximum3_f32, two values an
 // instruction).
-__device__ __forceinline__ unsigned top_bits8(const float (&v)[8]) {
+template <int V> __device__ __forceinline__ unsigned top_bits(const float (&v)[V]) {
   float m = fabsf(v[0]);
 #pragma unroll
-  for (int j = 1; j < 8; ++j) m = __builtin_elementwise_maximum(m, fabsf(v[j]));
+  for (int j = 1; j < V; ++j) m = __builtin_elementwise_maximum(m, fabsf(v[j]));
   return mag_bits(m);
 }
 // x / step to the nearest integer in the low bits of a float: adding 1.5 * 2^23 leaves no fraction bits, and rounds ties
@@ -134,30 +139,21 @@ __device__ __forceinline__ int code_of_rare(float x, unsigned byte) {
   if (byte == 255u) return 0;
   return (int)__builtin_amdgcn_fmed3f(__builtin_rintf(x * group_inverse(byte)), -63.f, 63.f);
 }
-__device__ __forceinline__ int code_of(float x, unsigned byte) {
-  return group_is_rare(byte) ? code_of_rare(x, byte) : (int)(signed char)code_bits(x, group_inverse(byte));
-}
-__device__ __forceinline__ u32x2 pack_codes(const float (&v)[8], unsigned byte) {
+__device__ __forceinline__ unsigned pack4(const float* v, unsigned byte) {
+  if (group_is_rare(byte))
+    return (code_of_rare(v[0], byte) & 255) | ((code_of_rare(v[1], byte) & 255) << 8) | ((code_of_rare(v[2], byte) & 255) << 16) |
+           ((unsigned)code_of_rare(v[3], byte) << 24);
   const float inverse = group_inverse(byte);
-  u32x2 r;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const unsigned lo = __builtin_amdgcn_perm(code_bits(v[4 * h + 1], inverse), code_bits(v[4 * h], inverse), 0x0c0c0400u);
-    const unsigned hi = __builtin_amdgcn_perm(code_bits(v[4 * h + 3], inverse), code_bits(v[4 * h + 2], inverse), 0x04000c0cu);
-    r[h] = lo | hi;
-  }
-  if (group_is_rare(byte)) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      r[h] = (code_of_rare(v[4 * h], byte) & 255) | ((code_of_rare(v[4 * h + 1], byte) & 255) << 8) |
-             ((code_of_rare(v[4 * h + 2], byte) & 255) << 16) | ((unsigned)code_of_rare(v[4 * h + 3], byte) << 24);
-  }
-  return r;
+  const unsigned lo = __builtin_amdgcn_perm(code_bits(v[1], inverse), code_bits(v[0], inverse), 0x0c0c0400u);
+  const unsigned hi = __builtin_amdgcn_perm(code_bits(v[3], inverse), code_bits(v[2], inverse), 0x04000c0cu);
+  return lo | hi;
 }
-__device__ __forceinline__ void decode8(u32x2 c, float step, float (&v)[8]) {
+__device__ __forceinline__ u32x2 pack_codes(const float (&v)[8], unsigned byte) { return u32x2{pack4(v, byte), pack4(v + 4, byte)}; }
+__device__ __forceinline__ void decode4(unsigned c, float step, float* v) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)(signed char)(c[i >> 2] >> (8 * (i & 3))) * step;
+  for (int i = 0; i < 4; ++i) v[i] = (float)(signed char)(c >> (8 * i)) * step;
 }
+__device__ __forceinline__ void decode8(u32x2 c, float step, float (&v)[8]) { decode4(c[0], step, v); decode4(c[1], step, v + 4); }
 // 127 steps of a group whose magnitudes reach the top of fp16 can exceed its largest finite value by less than one
 // step: such a value is held at the largest finite one (the group's own values were finite)
 __device__ __forceinline__ float hold_fp16(float y) { return y > 65504.f ? 65504.f : y < -65504.f ? -65504.f : y; }

@@ -57,7 +57,7 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = n + j < N ? v[j] : 0.f;
       }
-      unsigned top = n < N ? top_bits8(v) : 0u;
+      unsigned top = n < N ? top_bits<8>(v) : 0u;
       top = umax(top, (unsigned)__shfl_xor((int)top, X1, 64));
       top = umax(top, (unsigned)__shfl_xor((int)top, X2, 64));
       if (m < M && n < N) {

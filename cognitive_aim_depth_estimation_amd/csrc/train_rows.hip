@@ -7,9 +7,12 @@
 namespace {
 using namespace train;
 
-// A row lives in the registers of TPR threads, NCH runs of eight consecutive columns each (runs t, t + TPR, ...; four
-// neighbouring threads hold a group of 32).  Rows may begin at any element: runs are moved with 16-byte accesses of
-// whatever alignment the row has (gfx950 takes them), and the one run that crosses a row's end element by element.
+// A row lives in the registers of TPR threads, NCH runs of four consecutive columns each (runs t, t + TPR, ...; eight
+// neighbouring threads hold a group of 32): a wave's 16-byte loads of fp32 rows, and 8-byte ones of 16-bit rows, then
+// cover whole lines.  (With runs of eight, every fp32 load instruction took half of each line it touched: 4.7 TB/s.)
+// Rows may begin at any element: runs are moved with accesses of whatever alignment the row has (gfx950 takes them).
+// EVEN: the width is a multiple of the run, and no run crosses a row's end; otherwise that one is moved element by
+// element, which costs a branch around every access (and the batching of loads across it: 33 -> 24 us at 21920 x 1024).
 template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
   v = wave_sum_dpp(v);
   if constexpr (TPR > 64) {
@@ -34,87 +37,105 @@ template <int TPR> __device__ __forceinline__ void row_sum2(float& a, float& b, 
   }
 }
 
-// Run `c .. c + 7` of a row of D elements that begins at element `row`, zeros past its end.
-template <int DT> struct Run { u32x4v w; };
-template <> struct Run<DT_FP32> { u32x4v w, v; };
-template <int DT> __device__ __forceinline__ Run<DT> load_run(const void* p, long long row, int c, int D) {
-  Run<DT> r;
+// Run `c .. c + V - 1` of a row of D elements that begins at element `row`, zeros past its end.  W words hold its bits.
+template <int DT, int V> struct Run { static constexpr int W = DT == DT_FP32 ? V : V / 2; unsigned w[W]; };
+template <int DT, int V, bool EVEN> __device__ __forceinline__ Run<DT, V> load_run(const void* p, long long row, int c, int D) {
+  Run<DT, V> r;
   if constexpr (DT == DT_FP32) {
     const unsigned* q = reinterpret_cast<const unsigned*>(p) + row + c;
-    if (c + 8 <= D) { __builtin_memcpy(&r.w, q, 16); __builtin_memcpy(&r.v, q + 4, 16); }
+    if (EVEN || c + V <= D) __builtin_memcpy(r.w, q, sizeof(r.w));
     else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { r.w[j] = c + j < D ? q[j] : 0u; r.v[j] = c + 4 + j < D ? q[4 + j] : 0u; }
+      for (int j = 0; j < V; ++j) r.w[j] = c + j < D ? q[j] : 0u;
     }
   } else {
     const unsigned short* q = reinterpret_cast<const unsigned short*>(p) + row + c;
-    if (c + 8 <= D) __builtin_memcpy(&r.w, q, 16);
+    if (EVEN || c + V <= D) __builtin_memcpy(r.w, q, sizeof(r.w));
     else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r.w[j] = (c + 2 * j < D ? (unsigned)q[2 * j] : 0u) | (c + 2 * j + 1 < D ? (unsigned)q[2 * j + 1] << 16 : 0u);
+      for (int j = 0; j < V / 2; ++j) r.w[j] = (c + 2 * j < D ? (unsigned)q[2 * j] : 0u) | (c + 2 * j + 1 < D ? (unsigned)q[2 * j + 1] << 16 : 0u);
     }
   }
   return r;
 }
-template <int DT> __device__ __forceinline__ void cvt_run(const Run<DT>& r, float (&v)[8]) {
-  if constexpr (DT == DT_FP32) cvt_raw8(Raw8{r.w, r.v}, DT, v);
-  else cvt_raw8(Raw8{r.w, r.w}, DT, v);
-}
-// the same of a type known at run time (uniform over the launch)
-typedef Raw8 AnyRun;
-__device__ __forceinline__ AnyRun load_any(const void* p, int dt, long long row, int c, int D) {
+template <int V> __device__ __forceinline__ void cvt_words(const unsigned* w, int dt, float (&v)[V]) {
   if (dt == DT_FP32) {
-    const Run<DT_FP32> r = load_run<DT_FP32>(p, row, c, D);
-    return AnyRun{r.w, r.v};
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = __uint_as_float(w[j]);
+  } else if (dt == DT_BF16) {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) { v[2 * j] = bf16_lo(w[j]); v[2 * j + 1] = bf16_hi(w[j]); }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) { v[2 * j] = half_bits((unsigned short)w[j]); v[2 * j + 1] = half_bits((unsigned short)(w[j] >> 16)); }
   }
-  const Run<DT_BF16> r = load_run<DT_BF16>(p, row, c, D);
-  return AnyRun{r.w, r.w};
 }
-__device__ __forceinline__ void cvt_any(const AnyRun& o, int dt, float (&v)[8]) { cvt_raw8(o, dt, v); }
-__device__ __forceinline__ void store_any(void* p, int dt, long long row, int c, int D, const float (&y)[8]) {
+template <int DT, int V> __device__ __forceinline__ void cvt_run(const Run<DT, V>& r, float (&v)[V]) { cvt_words<V>(r.w, DT, v); }
+// the same of a type known at run time (uniform over the launch)
+template <int V, bool EVEN> __device__ __forceinline__ Run<DT_FP32, V> load_any(const void* p, int dt, long long row, int c, int D) {
+  if (dt == DT_FP32) return load_run<DT_FP32, V, EVEN>(p, row, c, D);
+  const Run<DT_BF16, V> r = load_run<DT_BF16, V, EVEN>(p, row, c, D);
+  Run<DT_FP32, V> o;
+#pragma unroll
+  for (int j = 0; j < V; ++j) o.w[j] = j < V / 2 ? r.w[j] : 0u;
+  return o;
+}
+template <int V, bool EVEN> __device__ __forceinline__ void store_any(void* p, int dt, long long row, int c, int D, const float (&y)[V]) {
   if (dt == DT_FP32) {
     float* q = reinterpret_cast<float*>(p) + row + c;
-    if (c + 8 <= D) __builtin_memcpy(q, y, 32);
+    if (EVEN || c + V <= D) __builtin_memcpy(q, y, 4 * V);
     else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) if (c + j < D) q[j] = y[j];
+      for (int j = 0; j < V; ++j) if (c + j < D) q[j] = y[j];
     }
   } else {
     unsigned short* q = reinterpret_cast<unsigned short*>(p) + row + c;
-    unsigned short h[8];
-    pack_half8(y, dt, h);
-    if (c + 8 <= D) __builtin_memcpy(q, h, 16);
+    unsigned short h[V];
+    pack_half<V>(y, dt, h);
+    if (EVEN || c + V <= D) __builtin_memcpy(q, h, 2 * V);
     else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) if (c + j < D) q[j] = h[j];
+      for (int j = 0; j < V; ++j) if (c + j < D) q[j] = h[j];
     }
   }
 }
-__device__ __forceinline__ u32x2 load_codes(const signed char* row, int c, int D) {
-  u32x2 q = {0, 0};
-  if (c + 8 <= D) __builtin_memcpy(&q, row + c, 8);
+template <int V> struct Codes { unsigned w[V / 4]; };
+template <int V, bool EVEN> __device__ __forceinline__ Codes<V> load_codes(const signed char* row, int c, int D) {
+  Codes<V> q;
+  if (EVEN || c + V <= D) __builtin_memcpy(q.w, row + c, V);
   else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) if (c + j < D) q[j >> 2] |= (unsigned)(unsigned char)row[c + j] << (8 * (j & 3));
+    for (int h = 0; h < V / 4; ++h) {
+      q.w[h] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) if (c + 4 * h + j < D) q.w[h] |= (unsigned)(unsigned char)row[c + 4 * h + j] << (8 * j);
+    }
   }
   return q;
 }
-__device__ __forceinline__ void load_f32(const float* p, int c, int D, float (&v)[8]) {
-  cvt_run<DT_FP32>(load_run<DT_FP32>(p, 0, c, D), v);
+template <int V> __device__ __forceinline__ void decode_run(const Codes<V>& q, float step, float (&v)[V]) {
+#pragma unroll
+  for (int h = 0; h < V / 4; ++h) decode4(q.w[h], step, v + 4 * h);
 }
-// codes and exponent byte of a thread's run; all four threads of a group call this together, with zeros past the row's end
-__device__ __forceinline__ void save_run(const float (&v)[8], signed char* codes, unsigned char* bytes, long long row, int D, int c) {
-  unsigned m = top_bits8(v);
+template <int V, bool EVEN> __device__ __forceinline__ void load_f32(const float* p, int c, int D, float (&v)[V]) {
+  cvt_run<DT_FP32, V>(load_run<DT_FP32, V, EVEN>(p, 0, c, D), v);
+}
+// codes and exponent byte of a thread's run; all threads of a group call this together, with zeros past the row's end
+template <int V, bool EVEN> __device__ __forceinline__ void save_run(const float (&v)[V], signed char* codes, unsigned char* bytes, long long row, int D, int c) {
+  unsigned m = top_bits<V>(v);
   m = umax(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0xB1 /* quad_perm [1,0,3,2] */, 0xf, 0xf, true));
   m = umax(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x4E /* quad_perm [2,3,0,1] */, 0xf, 0xf, true));
+  if constexpr (V == 4) m = umax(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x141 /* row_half_mirror */, 0xf, 0xf, true));
   if (c >= D) return;
   const unsigned byte = group_byte(m);
-  const u32x2 q = pack_codes(v, byte);
+  Codes<V> q;
+#pragma unroll
+  for (int h = 0; h < V / 4; ++h) q.w[h] = pack4(v + 4 * h, byte);
   signed char* to = codes + row * D + c;
-  if (c + 8 <= D) __builtin_memcpy(to, &q, 8);
+  if (EVEN || c + V <= D) __builtin_memcpy(to, q.w, V);
   else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) if (c + j < D) to[j] = (signed char)(q[j >> 2] >> (8 * (j & 3)));
+    for (int j = 0; j < V; ++j) if (c + j < D) to[j] = (signed char)(q.w[j >> 2] >> (8 * (j & 3)));
   }
   if ((c & (GROUP - 1)) == 0) bytes[row * groups_of(D) + c / GROUP] = (unsigned char)byte;
 }
@@ -124,40 +145,44 @@ struct LnFwd {
   signed char* codes; unsigned char* bytes; long long ldx, ldy; int M, D, y_dt; float eps;
 };
 
-template <int XDT, int TPR, int NCH>
+template <int XDT, int V, int TPR, int NCH, bool EVEN>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_fwd_kernel(LnFwd a) {
   __shared__ float red[32];
   const int t = threadIdx.x & (TPR - 1);
   constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
   const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
   if (RPB > 1 && row >= a.M) return;                        // whole waves: a row per wave
-  Run<XDT> raw[NCH];
+  // runs past the row's end are read from its beginning and zeroed: no branch, so all loads are in flight together
+  Run<XDT, V> raw[NCH];
+  Run<DT_FP32, V> g[NCH], b[NCH];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int c = (t + TPR * i) * 8;
-    if (c < a.D) raw[i] = load_run<XDT>(a.x, row * a.ldx, c, a.D);
+    const int c = (t + TPR * i) * V;
+    raw[i] = load_run<XDT, V, EVEN>(a.x, row * a.ldx, c < a.D ? c : 0, a.D);
   }
-  float v[NCH][8];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = (t + TPR * i) * V;
+    g[i] = load_run<DT_FP32, V, EVEN>(a.gamma, 0, c < a.D ? c : 0, a.D);
+    b[i] = load_run<DT_FP32, V, EVEN>(a.beta, 0, c < a.D ? c : 0, a.D);
+  }
+  float v[NCH][V];
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int c = (t + TPR * i) * 8;
-    if (c < a.D) cvt_run<XDT>(raw[i], v[i]);
-    else {
+    cvt_run<XDT, V>(raw[i], v[i]);
+    const bool in = (t + TPR * i) * V < a.D;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum += v[i][j];
+    for (int j = 0; j < V; ++j) { v[i][j] = in ? v[i][j] : 0.f; sum += v[i][j]; }
   }
   const float mean = row_sum<TPR>(sum, red) / (float)a.D;
   float sq = 0.f;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int c = (t + TPR * i) * 8;
+    const int c = (t + TPR * i) * V;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[i][j] = c + j < a.D ? v[i][j] - mean : 0.f;
+    for (int j = 0; j < V; ++j) {
+      v[i][j] = (EVEN ? c : c + j) < a.D ? v[i][j] - mean : 0.f;
       sq = __builtin_fmaf(v[i][j], v[i][j], sq);
     }
   }
@@ -165,16 +190,15 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_fwd_kernel(LnF
   if (t == 0) { a.mean[row] = mean; a.rstd[row] = rstd; }
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int c = (t + TPR * i) * 8;
+    const int c = (t + TPR * i) * V;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
-    if (a.codes) save_run(v[i], a.codes, a.bytes, row, a.D, c);
+    for (int j = 0; j < V; ++j) v[i][j] *= rstd;
+    if (a.codes) save_run<V, EVEN>(v[i], a.codes, a.bytes, row, a.D, c);
     if (c < a.D) {
-      float g[8], b[8], y[8];
-      load_f32(a.gamma, c, a.D, g); load_f32(a.beta, c, a.D, b);
+      float y[V];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = __builtin_fmaf(v[i][j], g[j], b[j]);
-      store_any(a.y, a.y_dt, row * a.ldy, c, a.D, y);
+      for (int j = 0; j < V; ++j) y[j] = __builtin_fmaf(v[i][j], __uint_as_float(g[i].w[j]), __uint_as_float(b[i].w[j]));
+      store_any<V, EVEN>(a.y, a.y_dt, row * a.ldy, c, a.D, y);
     }
   }
 }
@@ -190,58 +214,71 @@ struct LnBwd {
 };
 
 constexpr int SRC_CODES = 3;               // the rows come from their 8-bit copy
-template <int DYT, int SRC, int TPR, int NCH>
+template <int DYT, int SRC, int V, int TPR, int NCH, bool EVEN>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnBwd a) {
   constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
   constexpr int XDT = SRC == SRC_CODES ? DT_BF16 : SRC;
   __shared__ float red[32];
-  __shared__ float acc[RPB > 1 ? RPB * TPR * NCH * 8 : 1];
+  __shared__ float acc[RPB > 1 ? RPB * TPR * NCH * V : 1];
   const int t = threadIdx.x & (TPR - 1), sub = threadIdx.x / TPR;
-  float dg[NCH][8], db[NCH][8];
+  float dg[NCH][V], db[NCH][V];
 #pragma unroll
   for (int i = 0; i < NCH; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { dg[i][j] = 0.f; db[i][j] = 0.f; }
+    for (int j = 0; j < V; ++j) { dg[i][j] = 0.f; db[i][j] = 0.f; }
   const long long groups = groups_of(a.D);
-  for (long long row = (long long)blockIdx.x * RPB + sub; row < a.M; row += (long long)gridDim.x * RPB) {
-    Run<DYT> rdy[NCH];
-    Run<XDT> rx[NCH];
-    u32x2 rc[NCH];
-    unsigned rb[NCH];
-    AnyRun radd[NCH];
+  struct Loads { Run<DYT, V> dy[NCH]; Run<XDT, V> x[NCH]; Codes<V> codes[NCH]; unsigned byte[NCH]; Run<DT_FP32, V> add[NCH]; float rstd, mean; };
+  auto load = [&](long long row, Loads& l) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (t + TPR * i) * 8;
-      if (c < a.D) {
-        rdy[i] = load_run<DYT>(a.dy, row * a.lddy, c, a.D);
+      const int c = (t + TPR * i) * V < a.D ? (t + TPR * i) * V : 0;     // no branch around the loads
+      {
+        l.dy[i] = load_run<DYT, V, EVEN>(a.dy, row * a.lddy, c, a.D);
         if constexpr (SRC == SRC_CODES) {
-          rc[i] = load_codes(a.codes + row * a.D, c, a.D);
-          rb[i] = a.bytes[row * groups + c / GROUP];
-        } else rx[i] = load_run<XDT>(a.x, row * a.ldx, c, a.D);
-        if (a.add) radd[i] = load_any(a.add, a.add_dt, row * a.ldadd, c, a.D);
+          l.codes[i] = load_codes<V, EVEN>(a.codes + row * a.D, c, a.D);
+          l.byte[i] = a.bytes[row * groups + c / GROUP];
+        } else l.x[i] = load_run<XDT, V, EVEN>(a.x, row * a.ldx, c, a.D);
+        if (a.add) l.add[i] = load_any<V, EVEN>(a.add, a.add_dt, row * a.ldadd, c, a.D);
       }
     }
-    const float rstd = a.rstd[row], mean = SRC == SRC_CODES ? 0.f : a.mean[row];
-    float g[NCH][8], h[NCH][8];
+    l.rstd = a.rstd[row];
+    l.mean = SRC == SRC_CODES ? 0.f : a.mean[row];
+  };
+  // while a row is worked on, the next one's loads are in flight (not where 1024 threads leave a wave 128 registers)
+  constexpr bool AHEAD = TPR < 1024;
+  const long long stride = (long long)gridDim.x * RPB;
+  Loads next;
+  long long row = (long long)blockIdx.x * RPB + sub;
+  if constexpr (AHEAD) { if (row < a.M) load(row, next); }
+  float gmr[NCH][V];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) load_f32<V, EVEN>(a.gamma, (t + TPR * i) * V < a.D ? (t + TPR * i) * V : 0, a.D, gmr[i]);
+  for (; row < a.M; row += stride) {
+    Loads now;
+    if constexpr (AHEAD) {
+      now = next;
+      if (row + stride < a.M) load(row + stride, next);
+    } else load(row, now);
+    const float rstd = now.rstd, mean = now.mean;
+    float g[NCH][V], h[NCH][V];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (t + TPR * i) * 8;
+      const int c = (t + TPR * i) * V;
       if (c < a.D) {
-        float dy[8], gm[8];
-        cvt_run<DYT>(rdy[i], dy);
-        if constexpr (SRC == SRC_CODES) decode8(rc[i], group_step(rb[i]), h[i]);
+        float dy[V];
+        cvt_run<DYT, V>(now.dy[i], dy);
+        if constexpr (SRC == SRC_CODES) decode_run<V>(now.codes[i], group_step(now.byte[i]), h[i]);
         else {
-          cvt_run<XDT>(rx[i], h[i]);
+          cvt_run<XDT, V>(now.x[i], h[i]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) h[i][j] = (h[i][j] - mean) * rstd;
+          for (int j = 0; j < V; ++j) h[i][j] = (h[i][j] - mean) * rstd;
         }
-        load_f32(a.gamma, c, a.D, gm);                      // zeros past the row's end: g is zero there, as dy is
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < V; ++j) {
           dg[i][j] = __builtin_fmaf(dy[j], h[i][j], dg[i][j]);
           db[i][j] += dy[j];
-          g[i][j] = dy[j] * gm[j];
+          g[i][j] = dy[j] * gmr[i][j];
           s1 += g[i][j];
           s2 = __builtin_fmaf(g[i][j], h[i][j], s2);
         }
@@ -251,18 +288,18 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnB
     s1 /= (float)a.D; s2 /= (float)a.D;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (t + TPR * i) * 8;
+      const int c = (t + TPR * i) * V;
       if (c < a.D) {
-        float o[8];
+        float o[V];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = rstd * (g[i][j] - s1 - h[i][j] * s2);
+        for (int j = 0; j < V; ++j) o[j] = rstd * (g[i][j] - s1 - h[i][j] * s2);
         if (a.add) {
-          float ad[8];
-          cvt_any(radd[i], a.add_dt, ad);
+          float ad[V];
+          cvt_words<V>(now.add[i].w, a.add_dt, ad);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] += ad[j];
+          for (int j = 0; j < V; ++j) o[j] += ad[j];
         }
-        store_any(a.dx, a.dx_dt, row * a.lddx, c, a.D, o);
+        store_any<V, EVEN>(a.dx, a.dx_dt, row * a.lddx, c, a.D, o);
       }
     }
   }
@@ -275,22 +312,22 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnB
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[((sub * NCH + i) * 8 + j) * TPR + t] = which ? db[i][j] : dg[i][j];
+        for (int j = 0; j < V; ++j) acc[((sub * NCH + i) * V + j) * TPR + t] = which ? db[i][j] : dg[i][j];
       __syncthreads();
       // columns dealt to all threads; value (run, j) of thread run % TPR lies at run / TPR
       for (int c = threadIdx.x; c < a.D; c += RPB * TPR) {
-        const int run = c >> 3, at = ((run / TPR) * 8 + (c & 7)) * TPR + (run & (TPR - 1));
+        const int run = c / V, at = ((run / TPR) * V + c % V) * TPR + (run & (TPR - 1));
         float s = acc[at];
 #pragma unroll
-        for (int w = 1; w < RPB; ++w) s += acc[w * NCH * 8 * TPR + at];
+        for (int w = 1; w < RPB; ++w) s += acc[w * NCH * V * TPR + at];
         out[which * a.D + c] = s;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const int c = (t + TPR * i) * 8;
+        const int c = (t + TPR * i) * V;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < V; ++j)
           if (c + j < a.D) out[which * a.D + c + j] = which ? db[i][j] : dg[i][j];
       }
     }
@@ -335,71 +372,72 @@ struct Walk {
   }
 };
 
-// x [M, D] -> codes [M, D], bytes [M, groups].  Four neighbouring threads per group, a row's last group whole.
-template <int DT>
+// x [M, D] -> codes [M, D], bytes [M, groups].  32 / V neighbouring threads per group, a row's last group whole;
+// runs of four of fp32, of eight of 16-bit elements: 16 bytes a thread.
+template <int DT, int V, bool EVEN>
 __global__ __launch_bounds__(256) void pack8_kernel(const void* __restrict__ x, long long ldx, signed char* __restrict__ codes,
                                                     unsigned char* __restrict__ bytes, int M, int D) {
-  for (Walk w((unsigned)groups_of(D) * 4); w.row < (unsigned long long)M; w.step()) {     // a group's threads leave together
-    const int c = (int)w.run * 8;
-    float v[8];
-    if (c < D) cvt_run<DT>(load_run<DT>(x, (long long)w.row * ldx, c, D), v);
+  for (Walk w((unsigned)groups_of(D) * (GROUP / V)); w.row < (unsigned long long)M; w.step()) {     // a group's threads leave together
+    const int c = (int)w.run * V;
+    float v[V];
+    if (c < D) cvt_run<DT, V>(load_run<DT, V, EVEN>(x, (long long)w.row * ldx, c, D), v);
     else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      for (int j = 0; j < V; ++j) v[j] = 0.f;
     }
-    save_run(v, codes, bytes, (long long)w.row, D, c);
+    save_run<V, EVEN>(v, codes, bytes, (long long)w.row, D, c);
   }
 }
 
 // codes [M, D] -> out [M, width >= D] (columns past D are written as zero)
-template <int DT>
+template <int DT, int V, bool EVEN>
 __global__ __launch_bounds__(256) void unpack8_kernel(const signed char* __restrict__ codes,
                                                       const unsigned char* __restrict__ bytes, void* __restrict__ out,
                                                       long long ldo, int M, int D, int width) {
   const long long groups = groups_of(D);
-  for (Walk w((unsigned)(width + 7) / 8); w.row < (unsigned long long)M; w.step()) {
+  for (Walk w((unsigned)(width + V - 1) / V); w.row < (unsigned long long)M; w.step()) {
     const long long row = (long long)w.row;
-    const int c = (int)w.run * 8;
-    float v[8];
+    const int c = (int)w.run * V;
+    float v[V];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    for (int j = 0; j < V; ++j) v[j] = 0.f;
     if (c < D) {
-      const u32x2 q = load_codes(codes + row * D, c, D);
-      float u[8];
-      decode8(q, group_step(bytes[row * groups + c / GROUP]), u);
+      const Codes<V> q = load_codes<V, EVEN>(codes + row * D, c, D);
+      float u[V];
+      decode_run<V>(q, group_step(bytes[row * groups + c / GROUP]), u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < V; ++j) {
         if (DT == DT_FP16) u[j] = hold_fp16(u[j]);
         v[j] = c + j < D ? u[j] : 0.f;
       }
     }
-    store_any(out, DT, row * ldo, c, width, v);
+    store_any<V, EVEN>(out, DT, row * ldo, c, width, v);
   }
 }
 
 // du = dy * act'(u), u from its 8-bit copy
-template <int DT>
+template <int DT, int V, bool EVEN>
 __global__ __launch_bounds__(256) void act_bwd_kernel(const void* __restrict__ dy, long long lddy,
                                                       const signed char* __restrict__ codes,
                                                       const unsigned char* __restrict__ bytes, void* __restrict__ du,
                                                       int du_dt, long long lddu, int act, int M, int D) {
   const long long groups = groups_of(D);
-  for (Walk w((unsigned)(D + 7) / 8); w.row < (unsigned long long)M; w.step()) {
+  for (Walk w((unsigned)(D + V - 1) / V); w.row < (unsigned long long)M; w.step()) {
     const long long row = (long long)w.row;
-    const int c = (int)w.run * 8;
-    const Run<DT> r = load_run<DT>(dy, row * lddy, c, D);
-    const u32x2 q = load_codes(codes + row * D, c, D);
-    float u[8], g[8];
-    decode8(q, group_step(bytes[row * groups + c / GROUP]), u);
-    cvt_run<DT>(r, g);
+    const int c = (int)w.run * V;
+    const Run<DT, V> r = load_run<DT, V, EVEN>(dy, row * lddy, c, D);
+    const Codes<V> q = load_codes<V, EVEN>(codes + row * D, c, D);
+    float u[V], g[V];
+    decode_run<V>(q, group_step(bytes[row * groups + c / GROUP]), u);
+    cvt_run<DT, V>(r, g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < V; ++j) {
       float value, slope;
       if (act == ACT_GELU) gelu_both(u[j], value, slope);
       else slope = relu_slope(u[j]);
       g[j] *= slope;
     }
-    store_any(du, du_dt, row * lddu, c, D, g);
+    store_any<V, EVEN>(du, du_dt, row * lddu, c, D, g);
   }
 }
 
@@ -412,25 +450,30 @@ unsigned blocks_for(unsigned long long threads) {
 constexpr int LN_MAX_D = 16384;
 // blocks of the backward kernel: 16 waves a CU keep enough rows in flight; each leaves a partial row of 2 D floats
 int ln_bwd_blocks(int M, int D) {
-  const int rpb = D <= 1024 ? 4 : 1, most = D <= 8192 ? 1024 : 512;
+  const int rpb = D <= 1024 ? 4 : 1, most = D <= 8192 ? 768 : 512;
   const long long want = ((long long)M + rpb - 1) / rpb;
   return (int)(want < most ? want : most);
 }
 template <int XDT> void run_ln_fwd(const LnFwd& a, hipStream_t st) {
-#define LN_LAUNCH(TPR_, NCH_, RPB_, TH_) hipLaunchKernelGGL((ln_train_fwd_kernel<XDT, TPR_, NCH_>), dim3((unsigned)(((long long)a.M + RPB_ - 1) / RPB_)), dim3(TH_), 0, st, a)
-#define LN_BY_WIDTH(D_)                              \
-  if (D_ <= 512) LN_LAUNCH(64, 1, 4, 256);           \
-  else if (D_ <= 1024) LN_LAUNCH(64, 2, 4, 256);     \
-  else if (D_ <= 2048) LN_LAUNCH(256, 1, 1, 256);    \
-  else if (D_ <= 4096) LN_LAUNCH(256, 2, 1, 256);    \
-  else if (D_ <= 8192) LN_LAUNCH(1024, 1, 1, 1024);  \
-  else LN_LAUNCH(1024, 2, 1, 1024);
-  LN_BY_WIDTH(a.D)
+#define LN_LAUNCH(V_, TPR_, NCH_, RPB_, TH_) do { const dim3 grid((unsigned)(((long long)a.M + RPB_ - 1) / RPB_)); if (a.D % V_ == 0) hipLaunchKernelGGL((ln_train_fwd_kernel<XDT, V_, TPR_, NCH_, true>), grid, dim3(TH_), 0, st, a); else hipLaunchKernelGGL((ln_train_fwd_kernel<XDT, V_, TPR_, NCH_, false>), grid, dim3(TH_), 0, st, a); } while (0)
+  if (a.D <= 512) LN_LAUNCH(8, 64, 1, 4, 256);
+  else if (a.D <= 1024) LN_LAUNCH(8, 64, 2, 4, 256);
+  else if (a.D <= 2048) LN_LAUNCH(8, 256, 1, 1, 256);
+  else if (a.D <= 4096) LN_LAUNCH(8, 256, 2, 1, 256);
+  else if (a.D <= 8192) LN_LAUNCH(8, 1024, 1, 1, 1024);
+  else LN_LAUNCH(8, 1024, 2, 1, 1024);
 #undef LN_LAUNCH
 }
 template <int DYT, int SRC> void run_ln_bwd(const LnBwd& a, int blocks, hipStream_t st) {
-#define LN_LAUNCH(TPR_, NCH_, RPB_, TH_) hipLaunchKernelGGL((ln_train_bwd_kernel<DYT, SRC, TPR_, NCH_>), dim3(blocks), dim3(TH_), 0, st, a)
-  LN_BY_WIDTH(a.D)
+#define LN_LAUNCH(V_, TPR_, NCH_, RPB_, TH_) do { if (a.D % V_ == 0) hipLaunchKernelGGL((ln_train_bwd_kernel<DYT, SRC, V_, TPR_, NCH_, true>), dim3(blocks), dim3(TH_), 0, st, a); else hipLaunchKernelGGL((ln_train_bwd_kernel<DYT, SRC, V_, TPR_, NCH_, false>), dim3(blocks), dim3(TH_), 0, st, a); } while (0)
+  if (a.D <= 256) LN_LAUNCH(4, 64, 1, 4, 256);
+  else if (a.D <= 512) LN_LAUNCH(4, 64, 2, 4, 256);
+  else if (a.D <= 768) LN_LAUNCH(4, 64, 3, 4, 256);
+  else if (a.D <= 1024) LN_LAUNCH(4, 64, 4, 4, 256);
+  else if (a.D <= 2048) LN_LAUNCH(4, 256, 2, 1, 256);
+  else if (a.D <= 4096) LN_LAUNCH(4, 256, 4, 1, 256);
+  else if (a.D <= 8192) LN_LAUNCH(4, 1024, 2, 1, 1024);
+  else LN_LAUNCH(4, 1024, 4, 1, 1024);
 #undef LN_LAUNCH
 }
 template <int DYT> void run_ln_bwd_from(const LnBwd& a, int x_dt, int blocks, hipStream_t st) {
@@ -441,12 +484,17 @@ template <int DYT> void run_ln_bwd_from(const LnBwd& a, int x_dt, int blocks, hi
 }
 }  // namespace
 
-// KERNEL<type> launched for a run-time type
-#define BY_TYPE(DT_, KERNEL_, ...)                                                     \
-  do {                                                                                 \
-    if ((DT_) == DT_BF16) hipLaunchKernelGGL(KERNEL_<DT_BF16>, __VA_ARGS__);           \
-    else if ((DT_) == DT_FP16) hipLaunchKernelGGL(KERNEL_<DT_FP16>, __VA_ARGS__);      \
-    else hipLaunchKernelGGL(KERNEL_<DT_FP32>, __VA_ARGS__);                            \
+// KERNEL<type, columns a thread> launched for a run-time type
+#define BY_TYPE(DT_, D_, KERNEL_, ...)                                                                                          \
+  do {                                                                                                                          \
+    if ((DT_) == DT_FP32) BY_EVEN(DT_FP32, 4, D_, KERNEL_, __VA_ARGS__);                                                        \
+    else if ((DT_) == DT_BF16) BY_EVEN(DT_BF16, 8, D_, KERNEL_, __VA_ARGS__);                                                   \
+    else BY_EVEN(DT_FP16, 8, D_, KERNEL_, __VA_ARGS__);                                                                         \
+  } while (0)
+#define BY_EVEN(DT_, V_, D_, KERNEL_, ...)                                                                                      \
+  do {                                                                                                                          \
+    if ((D_) % V_ == 0) hipLaunchKernelGGL((KERNEL_<DT_, V_, true>), __VA_ARGS__);                                              \
+    else hipLaunchKernelGGL((KERNEL_<DT_, V_, false>), __VA_ARGS__);                                                            \
   } while (0)
 
 extern "C" {
@@ -497,7 +545,7 @@ int cogaim_layernorm_bwd(const void* dy, int dy_dtype, long long lddy, const voi
 int cogaim_pack8(const void* x, int x_dtype, long long ldx, void* codes, void* exponents, int M, int D, void* stream) {
   if (M <= 0 || D <= 0 || !dt_ok(x_dtype) || ldx < D || !x || !codes || !exponents || !aligned(x, dt_size(x_dtype)))
     return COGAIM_EINVAL;
-  BY_TYPE(x_dtype, pack8_kernel, dim3(blocks_for((unsigned long long)M * groups_of(D) * 4)), dim3(256), 0, (hipStream_t)stream, x, ldx,
+  BY_TYPE(x_dtype, D, pack8_kernel, dim3(blocks_for((unsigned long long)M * groups_of(D) * (x_dtype == DT_FP32 ? 8 : 4))), dim3(256), 0, (hipStream_t)stream, x, ldx,
           (signed char*)codes, (unsigned char*)exponents, M, D);
   return COGAIM_LAUNCH_CHECK();
 }
@@ -507,7 +555,7 @@ int cogaim_unpack8(const void* codes, const void* exponents, void* out, int out_
   if (M <= 0 || D <= 0 || width < D || !dt_ok(out_dtype) || ldo < width || !codes || !exponents || !out ||
       !aligned(out, dt_size(out_dtype)))
     return COGAIM_EINVAL;
-  BY_TYPE(out_dtype, unpack8_kernel, dim3(blocks_for((unsigned long long)M * ((width + 7LL) / 8))), dim3(256), 0, (hipStream_t)stream,
+  BY_TYPE(out_dtype, (D | width), unpack8_kernel, dim3(blocks_for((unsigned long long)M * (width / (out_dtype == DT_FP32 ? 4LL : 8LL) + 1))), dim3(256), 0, (hipStream_t)stream,
           (const signed char*)codes, (const unsigned char*)exponents, out, ldo, M, D, width);
   return COGAIM_LAUNCH_CHECK();
 }
@@ -518,7 +566,7 @@ int cogaim_activation_bwd(const void* dy, int dy_dtype, long long lddy, const vo
       !du || (activation != ACT_RELU && activation != ACT_GELU) || !aligned(dy, dt_size(dy_dtype)) ||
       !aligned(du, dt_size(du_dtype)))
     return COGAIM_EINVAL;
-  BY_TYPE(dy_dtype, act_bwd_kernel, dim3(blocks_for((unsigned long long)M * ((D + 7LL) / 8))), dim3(256), 0, (hipStream_t)stream, dy, lddy,
+  BY_TYPE(dy_dtype, D, act_bwd_kernel, dim3(blocks_for((unsigned long long)M * (D / (dy_dtype == DT_FP32 ? 4LL : 8LL) + 1))), dim3(256), 0, (hipStream_t)stream, dy, lddy,
           (const signed char*)codes, (const unsigned char*)exponents, du, du_dtype, lddu, activation, M, D);
   return COGAIM_LAUNCH_CHECK();
 }
