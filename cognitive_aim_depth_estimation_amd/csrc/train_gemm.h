@@ -60,15 +60,26 @@ template <int R, int NW, bool KC, bool WIDE, int SPLIT> struct Stager {
   unsigned long long base; long long left, step;      // next K-tile's first byte, bytes of the operand from there
   int k_left;                                         // k from there to the operand's end
   u32x4v rsrc;
+  // piece i of a wave: the first-released half of the K-tile is dealt to the waves ahead of the second.  Where the count is
+  // odd, the middle piece of the lower half of the waves still belongs to the first half, of the others to the second.
+  static constexpr int EARLY = PIECES / 2;            // pieces that lie in the first half for every wave
   __device__ __forceinline__ static int piece_of(int wave, int i) {
-    constexpr int H = PIECES / 2 < 1 ? 1 : PIECES / 2;
-    const int second = i / H, e = wave * H + i % H;   // place among the pieces of its half
+    constexpr int ALL = R / 8, HALF = ALL / 2;
+    int second, e;                                    // half, and place among its pieces
+    if constexpr (PIECES == 1) { second = wave >= NW / 2; e = second ? wave - NW / 2 : wave; }
+    else if constexpr (PIECES % 2 == 0) { second = i >= EARLY; e = wave * EARLY + (second ? i - EARLY : i); }
+    else {
+      second = i > EARLY || (i == EARLY && wave >= NW / 2);
+      if (i < EARLY) e = wave * EARLY + i;
+      else if (i == EARLY) e = second ? NW * EARLY + wave - NW / 2 : NW * EARLY + wave;
+      else e = wave * EARLY + i - EARLY - 1;
+    }
     if constexpr (KC) {
       constexpr int P = SPLIT / 16;                   // pieces (8 rows) in half a strip
-      const int in_strip = e / P * (2 * P) + e % P;   // the first half of the strips
+      const int in_strip = e / P * (2 * P) + e % P;   // the lower halves of the strips
       return in_strip + ((second ^ (WIDE ? 0 : 1)) ? P : 0);
     } else {
-      return e + second * (R / 16);
+      return e + second * HALF;
     }
   }
   __device__ __forceinline__ void init(const void* p, long long ld, int first, int count, int K, int k0, int wave, int lane, unsigned lds) {
@@ -223,7 +234,7 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
   // that share them; only the blocks of the first tile column
   constexpr bool SUMS = !AKC;
   constexpr int NS = SUMS ? MI / TL::WN : 1;
-  static_assert(!SUMS || MI % TL::WN == 0, "row fragments are dealt evenly");
+  static_assert(!SUMS || (MI % TL::WN == 0 && (BM & (BM - 1)) == 0), "row fragments are dealt evenly; rows across k in powers of two");
   f32x4 sums[NS];
   const bool with_sums = SUMS && g.col_sum && tn == 0;
   if constexpr (SUMS) {
@@ -247,35 +258,36 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
     // a step changes one operand; the fragments of a step are read between the MFMAs of the one before it, and the
     // eight DMA pieces that a wave owes the K-tile after the next go out one per step, in the order in which the stage's
     // halves fall free: the first half behind the barrier in mid-tile, the second behind the one at its end.
-    static_assert(MI == 8 && NJ == 4 && ST == 2 && decltype(sa)::PIECES == 4 && decltype(sb)::PIECES == 4, "written for 128 x 64 a wave");
-    v8 ax[4], ay[4], wa[2], wb[2];
+    static_assert(NJ == 4 && ST == 2 && MI % 2 == 0, "written for strips of 64 columns");
+    constexpr int MH = MI / 2, PA = decltype(sa)::PIECES, EA = decltype(sa)::EARLY, LATE = PA - EA;
+    static_assert(decltype(sb)::PIECES == 4 && PA >= 2 && PA <= 4, "six to eight pieces a wave and K-tile");
+    v8 ax[MH], ay[MH], wa[2], wb[2];
     unsigned fill = 0;                                       // stage the DMA fills
+    // order: A's early pieces, B's two early ones | the late ones.  At most four early: three go out in steps 5 to 7
     auto piece = [&](int q) __attribute__((always_inline)) {
-      if (q == 0) sa.piece(0, fill);
-      if (q == 1) sa.piece(1, fill);
-      if (q == 2) sb.piece(0, fill);
-      if (q == 3) sb.piece(1, fill);
-      if (q == 4) sa.piece(2, fill);
-      if (q == 5) sa.piece(3, fill);
-      if (q == 6) sb.piece(2, fill);
-      if (q == 7) { sb.piece(3, fill); advance(); fill ^= TL::STAGE; }
+      if (q < EA) sa.piece(q, fill);
+      else if (q < EA + 2) sb.piece(q - EA, fill);
+      else if (q < EA + 2 + LATE) sa.piece(q - 2, fill);
+      else if (q < PA + 4) sb.piece(q - PA, fill);
+      if (q == PA + 3) { advance(); fill ^= TL::STAGE; }
     };
+    constexpr int NP = PA + 4;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) piece(q);
+    for (int q = 0; q < NP; ++q) piece(q);
 #pragma unroll
     for (int q = 0; q < 4; ++q) piece(q);
     asm volatile("s_waitcnt vmcnt(4)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ax[i] = ra.read(smem, i, 0);
+    for (int i = 0; i < MH; ++i) ax[i] = ra.read(smem, i, 0);
 #pragma unroll
     for (int j = 0; j < 2; ++j) wa[j] = rb.read(smem + BM * TK * 2, j, 0);
-// one step: MFMAs of rows 4 mh_.., columns 2 nh_..; reads `load_(k)` behind the first nl_ of them, piece q_ behind the sixth
+// one step: MFMAs of rows MH mh_.., columns 2 nh_..; reads `load_(k)` behind the first nl_ of them, piece q_ ahead of the last
 #define TRAIN_STEP(af_, wf_, mh_, nh_, nl_, load_, q_)                                                                  \
-  _Pragma("unroll") for (int k_ = 0; k_ < 8; ++k_) {                                                                    \
-    acc[(mh_) * 4 + (k_ >> 1)][(nh_) * 2 + (k_ & 1)] =                                                                  \
-        H::mfma16(wf_[k_ & 1], af_[k_ >> 1], acc[(mh_) * 4 + (k_ >> 1)][(nh_) * 2 + (k_ & 1)]);                         \
+  _Pragma("unroll") for (int k_ = 0; k_ < 2 * MH; ++k_) {                                                               \
+    acc[(mh_) * MH + (k_ >> 1)][(nh_) * 2 + (k_ & 1)] =                                                                 \
+        H::mfma16(wf_[k_ & 1], af_[k_ >> 1], acc[(mh_) * MH + (k_ >> 1)][(nh_) * 2 + (k_ & 1)]);                        \
     if (k_ < (nl_)) { load_; }                                                                                          \
-    if (k_ == 6) piece(q_);                                                                                             \
+    if (k_ == 2 * MH - 2 && (q_) < NP) piece(q_);                                                                       \
     __builtin_amdgcn_sched_barrier(0);                                                                                  \
   }
     auto ktile = [&](auto stage_c) __attribute__((always_inline)) {
@@ -287,18 +299,18 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
       __builtin_amdgcn_sched_barrier(0);
       TRAIN_STEP(ax, wa, 0, 0, 2, wb[k_] = rb.read(bs, 2 + k_, 0), 4)
       add_sums(as, 0);
-      TRAIN_STEP(ax, wb, 0, 1, 4, ay[k_] = ra.read(as, 4 + k_, 0), 5)
-      TRAIN_STEP(ay, wb, 1, 1, 4, ax[k_] = ra.read(as, 4 + k_, 1), 6)
+      TRAIN_STEP(ax, wb, 0, 1, MH, ay[k_] = ra.read(as, MH + k_, 0), 5)
+      TRAIN_STEP(ay, wb, 1, 1, MH, ax[k_] = ra.read(as, MH + k_, 1), 6)
       TRAIN_STEP(ay, wa, 1, 0, 2, wb[k_] = rb.read(bs, k_, 1), 7)
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
       TRAIN_STEP(ax, wb, 1, 0, 2, wa[k_] = rb.read(bs, 2 + k_, 1), 0)
       add_sums(as, 1);
-      TRAIN_STEP(ax, wa, 1, 1, 4, ay[k_] = ra.read(as, k_, 1), 1)
+      TRAIN_STEP(ax, wa, 1, 1, MH, ay[k_] = ra.read(as, k_, 1), 1)
       TRAIN_STEP(ay, wa, 0, 1, 0, , 2)
       asm volatile("s_waitcnt vmcnt(3) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
-      TRAIN_STEP(ay, wb, 0, 0, 6, if (k_ < 4) ax[k_ & 3] = ra.read(an, k_, 0); else wa[k_ & 1] = rb.read(bn, k_ & 1, 0), 3)
+      TRAIN_STEP(ay, wb, 0, 0, 4, if (k_ < MH) ax[k_ < MH ? k_ : 0] = ra.read(an, k_, 0); if (k_ < 2) wa[k_ & 1] = rb.read(bn, k_ & 1, 0), 3)
     };
     for (int kt = 0; kt < nk; kt += 2) {
       ktile(std::integral_constant<int, 0>{});

@@ -259,28 +259,56 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(const unsigned short* __
 
 // ---- plans -------------------------------------------------------------------------------------------------------
 using T256 = Tile<256, 256, 2, 4, 2, true>;
+using T192 = Tile<192, 256, 2, 4, 2, true>;        // A contiguous along k only: its 192 columns across k have no XOR swizzle
+using T128W = Tile<128, 256, 2, 4, 2, true>;
 using T128 = Tile<128, 128, 2, 2, 2, false>;
 using T64 = Tile<64, 64, 2, 2, 4, false>;
+enum { TILE_256, TILE_192, TILE_128W, TILE_128, TILE_64, TILES };
+// What a launch takes, in us, measured on MI355X over 14 shapes from 5 x 1024 x 1024 to 21920 x 768 x 768 and each of the
+// three layouts: `slots` blocks run at a time and a round of them takes per_k for each K-tile of 64 and `fixed` for
+// its first loads and its stores; when at most half the slots are taken, a K-tile takes alone_k (less traffic, higher
+// clock).  A wide tile reads the fewest bytes per product, a small one leaves fewer compute units idle in the last
+// round: 5480 x 4096 x 1024 takes 58 us in 256 x 256 tiles (352 on 256 units), 50 in 192 x 256 (464), 53 in 128 x 256,
+// 58 in 128 x 128 and 99 in 64 x 64; 1370 x 768 x 768 takes 22, 18, 15, 13 and 9.5; 10960 x 4096 x 1024 takes 93, 99,
+// 104, 106 and 195.
+struct TileCost { int m, n, slots; float per_k, fixed, alone_k; };
+const TileCost TILE_COST[TILES] = {{256, 256, 256, 1.50f, 4.5f, 1.20f}, {192, 256, 256, 1.33f, 4.0f, 1.00f}, {128, 256, 256, 0.87f, 4.0f, 0.75f},
+                                   {128, 128, 512, 0.98f, 2.2f, 0.80f}, {64, 64, 512, 0.43f, 2.5f, 0.35f}};
+// Splitting the sum over k takes another kernel: about 5 us of launch and latency, and each partial sum written and
+// read back once at 5 TB/s.
+constexpr float JOIN_FIXED = 5.f, JOIN_PER_BYTE = 1.f / 5.0e6f;
 
-struct Shape { int tile, tiles_m, tiles_n, splits, kt_per_split; };      // tile: 256, 128 or 64
+struct Shape { int tile, tiles_m, tiles_n, splits, kt_per_split; };
 
-Shape shape_of(int M, int N, int K) {
+// `joined`: the second kernel runs whether or not the sum is split
+Shape shape_of(int M, int N, int K, bool a_along_k, bool joined) {
   const int nk = (K + TK - 1) / TK;
-  auto tiles = [&](int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); };
-  Shape s;
-  if (tiles(256) >= 160 || (tiles(256) >= 32 && nk >= 64)) s.tile = 256;
-  else if (tiles(128) >= 64) s.tile = 128;
-  else s.tile = 64;
-  s.tiles_m = (M + s.tile - 1) / s.tile; s.tiles_n = (N + s.tile - 1) / s.tile;
-  const long long t = (long long)s.tiles_m * s.tiles_n;
-  const long long room = s.tile == 256 ? 256 : 512;                      // blocks that run at a time
-  long long want = t >= room ? 1 : room / t;
-  const int least = s.tile == 256 ? 8 : 4;                               // K-tiles a part needs to be worth its partial sums
-  if (want > nk / least) want = nk / least;
-  if (want < 1) want = 1;
-  s.kt_per_split = (int)((nk + want - 1) / want);
-  s.splits = (nk + s.kt_per_split - 1) / s.kt_per_split;                 // no part is empty
-  return s;
+  Shape best{};
+  float least = 0.f;
+  for (int t = 0; t < TILES; ++t) {
+#ifdef FORCE
+    if (t != (FORCE == TILE_192 && !a_along_k ? TILE_256 : FORCE)) continue;
+#endif
+    if (t == TILE_192 && !a_along_k) continue;
+    const TileCost& c = TILE_COST[t];
+    const int tm = (M + c.m - 1) / c.m, tn = (N + c.n - 1) / c.n;
+    for (int want = 1; want <= 64; want += want < 4 ? 1 : want / 2) {
+#ifdef FORCE
+      if (want > 1) break;
+#endif
+      if (want > 1 && nk < 2 * want) break;
+      const int per = (nk + want - 1) / want, splits = (nk + per - 1) / per;            // no part is empty
+      const double blocks = (double)tm * tn * splits;
+      const double rounds = blocks <= c.slots ? 1.0 : (double)((long long)((blocks + c.slots - 1) / c.slots));
+      float us = (float)rounds * (c.fixed + per * (blocks * 2 <= c.slots ? c.alone_k : c.per_k));
+      if (splits > 1 || joined) us += JOIN_FIXED + JOIN_PER_BYTE * 8.f * splits * (float)M * (float)N;
+      if (best.splits == 0 || us < least) {
+        least = us;
+        best = Shape{t, tm, tn, splits, per};
+      }
+    }
+  }
+  return best;
 }
 
 long long round256(long long v) { return (v + 255) / 256 * 256; }
@@ -311,9 +339,15 @@ template <class T, bool AKC, bool BKC, class Epi>
 int launch_gemm(const Operands& g, int tile, const Epi& e, hipStream_t st) {
   const long long blocks = (long long)g.tiles_m * g.tiles_n * g.splits;
   if (blocks <= 0 || blocks >= (1LL << 31)) return COGAIM_EINVAL;
-  if (tile == 256) hipLaunchKernelGGL((train_gemm_kernel<T, AKC, BKC, T256, Epi>), dim3((unsigned)blocks), dim3(512), 0, st, g, e);
-  else if (tile == 128) hipLaunchKernelGGL((train_gemm_kernel<T, AKC, BKC, T128, Epi>), dim3((unsigned)blocks), dim3(256), 0, st, g, e);
-  else hipLaunchKernelGGL((train_gemm_kernel<T, AKC, BKC, T64, Epi>), dim3((unsigned)blocks), dim3(256), 0, st, g, e);
+#define TRAIN_LAUNCH(TL_) hipLaunchKernelGGL((train_gemm_kernel<T, AKC, BKC, TL_, Epi>), dim3((unsigned)blocks), dim3(TL_::NW * 64), 0, st, g, e)
+  if (tile == TILE_256) TRAIN_LAUNCH(T256);
+  else if (tile == TILE_192) {
+    if constexpr (AKC) TRAIN_LAUNCH(T192);
+    else return COGAIM_EINVAL;
+  } else if (tile == TILE_128W) TRAIN_LAUNCH(T128W);
+  else if (tile == TILE_128) TRAIN_LAUNCH(T128);
+  else TRAIN_LAUNCH(T64);
+#undef TRAIN_LAUNCH
   return COGAIM_LAUNCH_CHECK();
 }
 
@@ -387,7 +421,7 @@ extern "C" {
 
 long long cogaim_linear_fwd_workspace_bytes(const cogaim_linear_fwd_desc* d) {
   if (!forward_ok(d)) return COGAIM_EINVAL;
-  const Shape s = shape_of(d->M, d->N, d->K);
+  const Shape s = shape_of(d->M, d->N, d->K, true, !forward_epi<ACT_NONE>(d).fast());
   return copy_bytes(side(d->x, d->ldx, d->M, d->K)) + copy_bytes(side(d->w, d->ldw, d->N, d->K)) +
          (joins(s, forward_epi<ACT_NONE>(d)) ? (long long)s.splits * d->M * round8(d->N) * 4 : 0);
 }
@@ -396,7 +430,7 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long lon
   const long long need = cogaim_linear_fwd_workspace_bytes(d);
   if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  const Shape s = shape_of(d->M, d->N, d->K);
+  const Shape s = shape_of(d->M, d->N, d->K, true, !forward_epi<ACT_NONE>(d).fast());
   Side a = side(d->x, d->ldx, d->M, d->K), b = side(d->w, d->ldw, d->N, d->K);
   char* ws = (char*)workspace;
   int rc = run_copy(a, d->dtype, ws, st);
@@ -412,7 +446,7 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long lon
 
 long long cogaim_linear_bwd_input_workspace_bytes(const cogaim_linear_bwd_input_desc* d) {
   if (!input_ok(d)) return COGAIM_EINVAL;
-  const Shape s = shape_of(d->M, d->K, d->N);
+  const Shape s = shape_of(d->M, d->K, d->N, true, !input_epi<ACT_NONE>(d).fast());
   return copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + copy_bytes(side(d->w, d->ldw, d->N, d->K, d->scale)) +
          (joins(s, input_epi<ACT_NONE>(d)) ? (long long)s.splits * d->M * round8(d->K) * 4 : 0);
 }
@@ -421,7 +455,7 @@ int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspa
   const long long need = cogaim_linear_bwd_input_workspace_bytes(d);
   if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  const Shape s = shape_of(d->M, d->K, d->N);
+  const Shape s = shape_of(d->M, d->K, d->N, true, !input_epi<ACT_NONE>(d).fast());
   Side a = side(d->dy, d->lddy, d->M, d->N), b = side(d->w, d->ldw, d->N, d->K, d->scale);
   char* ws = (char*)workspace;
   int rc = run_copy(a, d->dtype, ws, st);
@@ -435,14 +469,15 @@ int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspa
   return d->dtype == DT_BF16 ? IN_RUN(__bf16) : IN_RUN(_Float16);
 }
 
-// whether the row-wise second kernel runs (parts to add, or something to put on the finished sums)
-static bool weight_needs_finish(const cogaim_linear_bwd_weight_desc* d, const Shape& s) {
-  return s.splits > 1 || d->x_scale || d->x_shift || d->scale || (d->K & 7) || !vec_ok(d->dw, d->lddw);
+// something to put on the finished sums, or a result that 16-byte stores cannot reach: the row-wise second kernel runs
+static bool weight_has_more(const cogaim_linear_bwd_weight_desc* d) {
+  return d->x_scale || d->x_shift || d->scale || (d->K & 7) || !vec_ok(d->dw, d->lddw);
 }
+static bool weight_needs_finish(const cogaim_linear_bwd_weight_desc* d, const Shape& s) { return s.splits > 1 || weight_has_more(d); }
 
 long long cogaim_linear_bwd_weight_workspace_bytes(const cogaim_linear_bwd_weight_desc* d) {
   if (!weight_ok(d)) return COGAIM_EINVAL;
-  const Shape s = shape_of(d->N, d->K, d->M);
+  const Shape s = shape_of(d->N, d->K, d->M, false, weight_has_more(d));
   const long long x = d->codes ? round256((long long)d->M * round8(d->K) * 2) : copy_bytes(side(d->x, d->ldx, d->M, d->K));
   const long long part = weight_needs_finish(d, s) ? round256((long long)s.splits * d->N * round8(d->K) * 4) + (long long)s.splits * d->N * 4 : 0;
   return copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + x + part;
@@ -452,7 +487,7 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
   const long long need = cogaim_linear_bwd_weight_workspace_bytes(d);
   if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  const Shape s = shape_of(d->N, d->K, d->M);
+  const Shape s = shape_of(d->N, d->K, d->M, false, weight_has_more(d));
   char* ws = (char*)workspace;
   Side a = side(d->dy, d->lddy, d->M, d->N), b{};
   int rc = run_copy(a, d->dtype, ws, st);

@@ -24,6 +24,7 @@ There is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -121,48 +122,53 @@ def _act(name):
     return _ACTIVATIONS[name]
 
 
-class _On:
-    """The tensors' device made current for a call, and the handle of its current stream."""
-    __slots__ = ("index", "before")
-
-    def __init__(self, device):
-        if device.type != "cuda":
-            raise RuntimeError("the training operators run only on a ROCm device (no CPU path)")
-        self.index = device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _new_checkpoint(lead, D, device):
-    return Checkpoint8(torch.empty(*lead, D, device=device, dtype=torch.int8),
-                       torch.empty(*lead, (D + GROUP - 1) // GROUP, device=device, dtype=torch.uint8))
+def _stream(device):
+    """Handle of the current stream of a tensor's device."""
+    if device.type != "cuda":
+        raise RuntimeError("the training operators run only on a ROCm device (no CPU path)")
+    # (the handle without the Python object around it, where torch offers that: 0.1 us instead of 2.8 of a call's ten)
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes > 0 else None
+def _on_device(fn):
+    """The device of the first argument made current for a call, when it is not."""
+    @functools.wraps(fn)
+    def run(first, *args, **kwargs):
+        t = first.codes if type(first) is Checkpoint8 else first
+        if isinstance(t, Tensor) and t.is_cuda and t.get_device() != torch.cuda.current_device():
+            with torch.cuda.device(t.device):
+                return fn(first, *args, **kwargs)
+        return fn(first, *args, **kwargs)
+    return run
+
+
+def _new(like, shape, dtype):
+    """An empty tensor on the device of `like`."""
+    return like.new_empty(shape, dtype=dtype)
+
+
+def _new_checkpoint(like, lead, D):
+    return Checkpoint8(_new(like, (*lead, D), torch.int8), _new(like, (*lead, (D + GROUP - 1) // GROUP), torch.uint8))
 
 
 # ---- 8-bit activations -------------------------------------------------------------------------------------------
+@_on_device
 def pack8(x: Tensor) -> Checkpoint8:
     """``x [..., D]`` (bf16, fp16 or fp32) in 8 bits."""
     _float(x, "x")
-    with _On(x.device) as stream:
-        out = _new_checkpoint(x.shape[:-1], x.shape[-1], x.device)
-        v, ld = _rows(x)
-        if v.shape[0]:
-            call("cogaim_pack8", v.data_ptr(), _CODE[x.dtype], ld, out.codes.data_ptr(), out.exponents.data_ptr(), v.shape[0],
-                 v.shape[1], stream)
+    stream = _stream(x.device)
+    out = _new_checkpoint(x, x.shape[:-1], x.shape[-1])
+    v, ld = _rows(x)
+    if v.shape[0]:
+        call("cogaim_pack8", v.data_ptr(), _CODE[x.dtype], ld, out.codes.data_ptr(), out.exponents.data_ptr(), v.shape[0],
+             v.shape[1], stream)
     return out
 
 
+@_on_device
 def unpack8(saved: Checkpoint8, dtype: torch.dtype = torch.float32) -> Tensor:
     """The values of an 8-bit copy: exact in fp32 and bf16, rounded once (and held at +-65504) in fp16."""
     if not isinstance(saved, Checkpoint8):
@@ -172,15 +178,16 @@ def unpack8(saved: Checkpoint8, dtype: torch.dtype = torch.float32) -> Tensor:
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError("saved needs at least one column")
     codes, exponents = _checkpoint(saved, "saved", shape, saved.codes.device)
-    with _On(codes.device) as stream:
-        out = torch.empty(shape, device=codes.device, dtype=dtype)
-        D = shape[-1]
-        M = codes.numel() // D
-        if M:
-            call("cogaim_unpack8", codes.data_ptr(), exponents.data_ptr(), out.data_ptr(), _CODE[dtype], D, M, D, D, stream)
+    stream = _stream(codes.device)
+    out = _new(codes, shape, dtype)
+    D = shape[-1]
+    M = codes.numel() // D
+    if M:
+        call("cogaim_unpack8", codes.data_ptr(), exponents.data_ptr(), out.data_ptr(), _CODE[dtype], D, M, D, D, stream)
     return out
 
 
+@_on_device
 def activation_backward(dy: Tensor, saved: Checkpoint8, activation: str, out_dtype: Optional[torch.dtype] = None) -> Tensor:
     """``dy * act'(u)`` with ``u`` kept in 8 bits; activation "relu" or "gelu"."""
     _float(dy, "dy")
@@ -189,17 +196,18 @@ def activation_backward(dy: Tensor, saved: Checkpoint8, activation: str, out_dty
         raise ValueError("activation must be 'relu' or 'gelu'")
     out_dtype = _out_dtype(out_dtype, dy.dtype)
     codes, exponents = _checkpoint(saved, "saved", dy.shape, dy.device)
-    with _On(dy.device) as stream:
-        out = torch.empty(dy.shape, device=dy.device, dtype=out_dtype)
-        v, ld = _rows(dy)
-        M, D = v.shape
-        if M:
-            call("cogaim_activation_bwd", v.data_ptr(), _CODE[dy.dtype], ld, codes.data_ptr(), exponents.data_ptr(),
-                 out.data_ptr(), _CODE[out_dtype], D, act, M, D, stream)
+    stream = _stream(dy.device)
+    out = _new(dy, dy.shape, out_dtype)
+    v, ld = _rows(dy)
+    M, D = v.shape
+    if M:
+        call("cogaim_activation_bwd", v.data_ptr(), _CODE[dy.dtype], ld, codes.data_ptr(), exponents.data_ptr(),
+             out.data_ptr(), _CODE[out_dtype], D, act, M, D, stream)
     return out
 
 
 # ---- layer norm --------------------------------------------------------------------------------------------------
+@_on_device
 def layer_norm_forward(x: Tensor, weight: Tensor, bias: Tensor, eps: float = 1e-6, out_dtype: Optional[torch.dtype] = None,
                        checkpoint: bool = False) -> Tuple[Tensor, Tensor, Tensor, Optional[Checkpoint8]]:
     """``(y, mean, rstd, saved)``: ``y = (x - mean) * rstd * weight + bias`` of type ``out_dtype`` (default: x's), the fp32
@@ -215,20 +223,21 @@ def layer_norm_forward(x: Tensor, weight: Tensor, bias: Tensor, eps: float = 1e-
     if weight is None or bias is None:
         raise ValueError("weight and bias are needed")
     out_dtype = _out_dtype(out_dtype, x.dtype)
-    with _On(dev) as stream:
-        lead = x.shape[:-1]
-        y = torch.empty(x.shape, device=dev, dtype=out_dtype)
-        stats = torch.empty((2,) + tuple(lead), device=dev, dtype=torch.float32)
-        mean, rstd = stats[0], stats[1]
-        saved = _new_checkpoint(lead, D, dev) if checkpoint else None
-        v, ld = _rows(x)
-        if v.shape[0]:
-            call("cogaim_layernorm_train_fwd", v.data_ptr(), _CODE[x.dtype], ld, weight.data_ptr(), bias.data_ptr(), y.data_ptr(),
-                 _CODE[out_dtype], D, mean.data_ptr(), rstd.data_ptr(), ptr(saved.codes) if saved else None,
-                 ptr(saved.exponents) if saved else None, v.shape[0], D, eps, stream)
+    stream = _stream(dev)
+    lead = x.shape[:-1]
+    y = _new(x, x.shape, out_dtype)
+    mean = _new(x, lead, torch.float32)
+    rstd = torch.empty_like(mean)
+    saved = _new_checkpoint(x, lead, D) if checkpoint else None
+    v, ld = _rows(x)
+    if v.shape[0]:
+        call("cogaim_layernorm_train_fwd", v.data_ptr(), _CODE[x.dtype], ld, weight.data_ptr(), bias.data_ptr(), y.data_ptr(),
+             _CODE[out_dtype], D, mean.data_ptr(), rstd.data_ptr(), ptr(saved.codes) if saved else None,
+             ptr(saved.exponents) if saved else None, v.shape[0], D, eps, stream)
     return y, mean, rstd, saved
 
 
+@_on_device
 def layer_norm_backward(dy: Tensor, saved: Union[Tensor, Checkpoint8], mean: Optional[Tensor], rstd: Tensor, weight: Tensor,
                         add: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor, Tensor]:
     """``(dx, dweight, dbias)`` from ``dy`` and either the norm's input with its ``mean`` or its rows in 8 bits (``mean`` is
@@ -261,22 +270,22 @@ def layer_norm_backward(dy: Tensor, saved: Union[Tensor, Checkpoint8], mean: Opt
     if add is not None:
         _float(add, "add")
         _same(add, "add", dy.shape, dev)
-    with _On(dev) as stream:
-        dx = torch.empty(dy.shape, device=dev, dtype=out_dtype)
-        v, ld = _rows(dy)
-        M = v.shape[0]
-        if not M:
-            return dx, torch.zeros(D, device=dev), torch.zeros(D, device=dev)
-        grads = torch.empty(2, D, device=dev, dtype=torch.float32)
-        dweight, dbias = grads[0], grads[1]
-        nbytes = call("cogaim_layernorm_bwd_workspace_bytes", M, D)
-        ws = _workspace(nbytes, dev)
-        xv, ldx = _rows(x) if x is not None else (None, 0)
-        av, lda = _rows(add) if add is not None else (None, 0)
-        call("cogaim_layernorm_bwd", v.data_ptr(), _CODE[dy.dtype], ld, ptr(xv), _CODE[x.dtype] if x is not None else 0, ldx,
-             ptr(codes), ptr(exponents), ptr(mean) if x is not None else None, rstd.data_ptr(), weight.data_ptr(), ptr(av),
-             _CODE[add.dtype] if add is not None else 0, lda, dx.data_ptr(), _CODE[out_dtype], D, dweight.data_ptr(),
-             dbias.data_ptr(), M, D, ws.data_ptr(), nbytes, stream)
+    stream = _stream(dev)
+    dx = _new(dy, dy.shape, out_dtype)
+    v, ld = _rows(dy)
+    M = v.shape[0]
+    if not M:
+        return dx, torch.zeros(D, device=dev), torch.zeros(D, device=dev)
+    dweight = torch.empty_like(weight)
+    dbias = torch.empty_like(weight)
+    nbytes = call("cogaim_layernorm_bwd_workspace_bytes", M, D)
+    ws = _new(dy, nbytes, torch.uint8)
+    xv, ldx = _rows(x) if x is not None else (None, 0)
+    av, lda = _rows(add) if add is not None else (None, 0)
+    call("cogaim_layernorm_bwd", v.data_ptr(), _CODE[dy.dtype], ld, ptr(xv), _CODE[x.dtype] if x is not None else 0, ldx,
+         ptr(codes), ptr(exponents), ptr(mean) if x is not None else None, rstd.data_ptr(), weight.data_ptr(), ptr(av),
+         _CODE[add.dtype] if add is not None else 0, lda, dx.data_ptr(), _CODE[out_dtype], D, dweight.data_ptr(),
+         dbias.data_ptr(), M, D, ws.data_ptr(), nbytes, stream)
     return dx, dweight, dbias
 
 
@@ -294,14 +303,16 @@ def _leading(ld, name):
     return ld
 
 
-def _run_linear(name, desc, device, stream):
-    nbytes = call(name + "_workspace_bytes", C.byref(desc))
+def _run_linear(name, desc, like, stream):
+    desc = C.byref(desc)
+    nbytes = call(name + "_workspace_bytes", desc)
     if nbytes < 0:
         raise ValueError(f"{name}: arguments the kernels do not take")
-    ws = _workspace(nbytes, device)
-    call(name, C.byref(desc), ptr(ws), nbytes, stream)
+    ws = _new(like, nbytes, torch.uint8) if nbytes else None
+    call(name, desc, ptr(ws), nbytes, stream)
 
 
+@_on_device
 def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: str = "none",
                    scale: Optional[Tensor] = None, residual: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None,
                    checkpoint: bool = False) -> Tuple[Tensor, Optional[Checkpoint8]]:
@@ -322,22 +333,23 @@ def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act
     if residual is not None:
         _float(residual, "residual")
         _same(residual, "residual", tuple(lead) + (N,), dev)
-    with _On(dev) as stream:
-        y = torch.empty(*lead, N, device=dev, dtype=out_dtype)
-        saved = _new_checkpoint(lead, N, dev) if checkpoint else None
-        xv, ldx = _rows(x)
-        M = xv.shape[0]
-        if M:
-            wv, ldw = _rows(weight)
-            rv, ldr = _rows(residual) if residual is not None else (None, 0)
-            desc = LinearFwdDesc(xv.data_ptr(), wv.data_ptr(), ptr(bias), ptr(scale), ptr(rv), y.data_ptr(),
-                                 ptr(saved.codes) if saved else None, ptr(saved.exponents) if saved else None,
-                                 _leading(ldx, "x"), _leading(ldw, "weight"), _leading(ldr, "residual"), _leading(N, "y"), M, N, K,
-                                 _CODE[x.dtype], _CODE[residual.dtype] if residual is not None else 0, _CODE[out_dtype], act, 0)
-            _run_linear("cogaim_linear_fwd", desc, dev, stream)
+    stream = _stream(dev)
+    y = _new(x, (*lead, N), out_dtype)
+    saved = _new_checkpoint(x, lead, N) if checkpoint else None
+    xv, ldx = _rows(x)
+    M = xv.shape[0]
+    if M:
+        wv, ldw = _rows(weight)
+        rv, ldr = _rows(residual) if residual is not None else (None, 0)
+        desc = LinearFwdDesc(xv.data_ptr(), wv.data_ptr(), ptr(bias), ptr(scale), ptr(rv), y.data_ptr(),
+                             ptr(saved.codes) if saved else None, ptr(saved.exponents) if saved else None,
+                             _leading(ldx, "x"), _leading(ldw, "weight"), _leading(ldr, "residual"), _leading(N, "y"), M, N, K,
+                             _CODE[x.dtype], _CODE[residual.dtype] if residual is not None else 0, _CODE[out_dtype], act, 0)
+        _run_linear("cogaim_linear_fwd", desc, x, stream)
     return y, saved
 
 
+@_on_device
 def linear_backward_input(dy: Tensor, weight: Tensor, activation: str = "none", saved: Optional[Checkpoint8] = None,
                           scale: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None,
                           want_activation: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
@@ -361,20 +373,21 @@ def linear_backward_input(dy: Tensor, weight: Tensor, activation: str = "none", 
     codes = exponents = None
     if act:
         codes, exponents = _checkpoint(saved, "saved", tuple(lead) + (K,), dev)
-    with _On(dev) as stream:
-        dx = torch.empty(*lead, K, device=dev, dtype=out_dtype)
-        a = torch.empty(*lead, K, device=dev, dtype=dy.dtype) if want_activation else None
-        v, ld = _rows(dy)
-        M = v.shape[0]
-        if M:
-            wv, ldw = _rows(weight)
-            desc = LinearBwdInputDesc(v.data_ptr(), wv.data_ptr(), ptr(scale), ptr(codes), ptr(exponents), dx.data_ptr(), ptr(a),
-                                      _leading(ld, "dy"), _leading(ldw, "weight"), _leading(K, "dx"), K, M, N, K, _CODE[dy.dtype],
-                                      _CODE[out_dtype], act)
-            _run_linear("cogaim_linear_bwd_input", desc, dev, stream)
+    stream = _stream(dev)
+    dx = _new(dy, (*lead, K), out_dtype)
+    a = _new(dy, (*lead, K), dy.dtype) if want_activation else None
+    v, ld = _rows(dy)
+    M = v.shape[0]
+    if M:
+        wv, ldw = _rows(weight)
+        desc = LinearBwdInputDesc(v.data_ptr(), wv.data_ptr(), ptr(scale), ptr(codes), ptr(exponents), dx.data_ptr(), ptr(a),
+                                  _leading(ld, "dy"), _leading(ldw, "weight"), _leading(K, "dx"), K, M, N, K, _CODE[dy.dtype],
+                                  _CODE[out_dtype], act)
+        _run_linear("cogaim_linear_bwd_input", desc, dy, stream)
     return dx, a
 
 
+@_on_device
 def linear_backward_weight(dy: Tensor, x: Union[Tensor, Checkpoint8], weight: Optional[Tensor] = None,
                            bias: Optional[Tensor] = None, scale: Optional[Tensor] = None, x_scale: Optional[Tensor] = None,
                            x_shift: Optional[Tensor] = None,
@@ -414,21 +427,23 @@ def linear_backward_weight(dy: Tensor, x: Union[Tensor, Checkpoint8], weight: Op
     elif weight is not None or bias is not None:
         raise ValueError("weight and bias go with scale")
     out_dtype = _out_dtype(out_dtype, torch.float32)
-    with _On(dev) as stream:
-        v, ld = _rows(dy)
-        M = v.shape[0]
-        make = torch.empty if M else torch.zeros
-        dw = make(N, K, device=dev, dtype=out_dtype)
-        db = make(N, device=dev, dtype=torch.float32)
-        ds = make(N, device=dev, dtype=torch.float32) if scale is not None else None
-        if M:
-            xv, ldx = _rows(x) if x is not None else (None, 0)
-            wv, ldw = _rows(weight) if scale is not None else (None, 0)
-            desc = LinearBwdWeightDesc(v.data_ptr(), ptr(xv), ptr(codes), ptr(exponents), ptr(x_scale), ptr(x_shift), ptr(wv),
-                                       ptr(bias), ptr(scale), dw.data_ptr(), db.data_ptr(), ptr(ds), _leading(ld, "dy"),
-                                       _leading(ldx, "x"), _leading(ldw, "weight"), _leading(K, "dW"), M, N, K, _CODE[dy.dtype],
-                                       _CODE[out_dtype], 0)
-            _run_linear("cogaim_linear_bwd_weight", desc, dev, stream)
+    stream = _stream(dev)
+    v, ld = _rows(dy)
+    M = v.shape[0]
+    make = dy.new_empty if M else dy.new_zeros
+    dw = make((N, K), dtype=out_dtype)
+    db = make(N, dtype=torch.float32)
+    ds = torch.empty_like(db) if scale is not None else None
+    if ds is not None and not M:
+        ds.zero_()
+    if M:
+        xv, ldx = _rows(x) if x is not None else (None, 0)
+        wv, ldw = _rows(weight) if scale is not None else (None, 0)
+        desc = LinearBwdWeightDesc(v.data_ptr(), ptr(xv), ptr(codes), ptr(exponents), ptr(x_scale), ptr(x_shift), ptr(wv),
+                                   ptr(bias), ptr(scale), dw.data_ptr(), db.data_ptr(), ptr(ds), _leading(ld, "dy"),
+                                   _leading(ldx, "x"), _leading(ldw, "weight"), _leading(K, "dW"), M, N, K, _CODE[dy.dtype],
+                                   _CODE[out_dtype], 0)
+        _run_linear("cogaim_linear_bwd_weight", desc, dy, stream)
     return dw, db, ds
 
 
