@@ -190,7 +190,8 @@ template <class T, bool AKC, bool BKC, class TL, class Epi>
 __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, Epi epi) {
   constexpr int BM = TL::BM, BN = TL::BN, MI = TL::MI, NJ = TL::NJ, ST = TL::STAGES;
   constexpr int PER_STAGE = (BM + BN) / 8 / TL::NW;                   // DMA instructions a wave issues per K-tile
-  __shared__ __attribute__((aligned(1024))) char smem[ST * TL::STAGE];
+  __shared__ __attribute__((aligned(1024))) char smem[ST * TL::STAGE + Epi::TABLE * sizeof(float2)];
+  float2* const table = reinterpret_cast<float2*>(smem + ST * TL::STAGE);      // the epilogue's own, complete behind the first barrier below
   using H = Half<T>;
   using v8 = typename H::v8;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -276,7 +277,8 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
     for (int q = 0; q < NP; ++q) piece(q);
 #pragma unroll
     for (int q = 0; q < 4; ++q) piece(q);
-    asm volatile("s_waitcnt vmcnt(4)\n\ts_barrier" ::: "memory");
+    epi.fill(table, threadIdx.x, TL::NW * 64);
+    asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int i = 0; i < MH; ++i) ax[i] = ra.read(smem, i, 0);
 #pragma unroll
@@ -327,6 +329,7 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
     };
 #pragma unroll
     for (int p = 0; p < ST - 1; ++p) stage_all(p);
+    epi.fill(table, threadIdx.x, TL::NW * 64);
     int slot = 0;
     for (int kt = 0; kt < nk; ++kt) {
       // this K-tile has landed (the ST - 2 younger ones may still be in flight) and this wave's reads of the slot that is
@@ -376,7 +379,7 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
       float v[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) { v[e] = acc[i][2 * h][e]; v[4 + e] = acc[i][2 * h + 1][e]; }
-      epi.template finish<true, 16, 32>(split, mw + 16 * i, n, v, col, row[i]);
+      epi.template finish<true, 16, 32>(split, mw + 16 * i, n, v, col, row[i], table);
     }
   }
 }

@@ -33,6 +33,8 @@ template <int ACT>
 struct EpiForward {                          // y = act(acc + bias) * scale + residual, codes of acc + bias
   const float* bias; const float* scale; const void* res; void* y; signed char* codes; unsigned char* bytes;
   long long ldr, ldy; int M, N, res_dt, y_dt; bool res_vec, y_vec, code_vec;
+  static constexpr int TABLE = 0;            // float2 entries of LDS the epilogue wants
+  __device__ __forceinline__ void fill(float2*, int, int) const {}
   bool fast() const { return (N & 7) == 0 && y_vec && (!res || res_vec) && (!codes || code_vec); }
   struct Columns { float b[8], s[8]; };
   struct Row { Raw8 r; };
@@ -49,7 +51,7 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
     if (res && (FAST || (res_vec && n + 8 <= N)) && m < M && n < N) r.r = load_raw8(res, res_dt, (size_t)m * ldr + n);
   }
   template <bool FAST, int X1, int X2>
-  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns& c, const Row& r) const {
+  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns& c, const Row& r, const float2*) const {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += c.b[j];
     if (codes) {
@@ -94,10 +96,26 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
   }
 };
 
+// dx = acc * act'(u), a = act(u), u from its 8-bit copy.  GELU and its derivative take about 30 instructions an element,
+// during which the matrix pipe stands: two fifths of the launch at 5480 x 1024 x 4096.  But a code has 256 values and
+// few steps occur, so the main loop's blocks hold both functions of every code at the eight steps 2^-9 .. 2^-2 (groups
+// whose largest magnitude lies between 1/8 and 32) in 16 KB of LDS, filled while their first loads are in flight;
+// other groups are computed.  Both ways give the same bits.  @TABLE@
+constexpr unsigned TABLE_FIRST = 118;        // exponent byte of 2^-9
+constexpr int TABLE_STEPS = 8;
 template <int ACT>
-struct EpiInput {                            // dx = acc * act'(u), a = act(u), u from its 8-bit copy
+struct EpiInput {
   const signed char* codes; const unsigned char* bytes; void* dx; void* a; long long lddx, lda;
   int M, N, dx_dt, a_dt; bool dx_vec, a_vec, code_vec;
+  static constexpr int TABLE = ACT == ACT_GELU ? TABLE_STEPS * 256 : 0;
+  __device__ __forceinline__ void fill(float2* table, int tid, int threads) const {
+    if constexpr (ACT == ACT_GELU)
+      for (int i = tid; i < TABLE; i += threads) {
+        float2 f;
+        gelu_both((float)((i & 255) - 128) * group_step(TABLE_FIRST + (i >> 8)), f.x, f.y);
+        table[i] = f;
+      }
+  }
   bool fast() const { return (N & 7) == 0 && dx_vec && (!a || a_vec) && (!codes || code_vec); }
   struct Columns {};
   struct Row { u32x2 q; unsigned byte; };
@@ -119,18 +137,29 @@ struct EpiInput {                            // dx = acc * act'(u), a = act(u), 
     }
   }
   template <bool FAST, int X1, int X2>
-  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row& r) const {
+  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row& r, const float2* table) const {
     if (m >= M || n >= N) return;
     if constexpr (ACT != ACT_NONE) {
       float u[8];
-      decode8(r.q, group_step(r.byte), u);
+      const bool listed = ACT == ACT_GELU && FAST && r.byte - TABLE_FIRST < (unsigned)TABLE_STEPS;
+      if (ACT == ACT_GELU && FAST && __all(listed)) {
+        const float2* t = table + ((r.byte - TABLE_FIRST) << 8);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float value, slope;
-        if constexpr (ACT == ACT_GELU) gelu_both(u[j], value, slope);
-        else { value = relu_of(u[j]); slope = relu_slope(u[j]); }
-        v[j] *= slope;
-        u[j] = value;
+        for (int j = 0; j < 8; ++j) {
+          const float2 f = t[(r.q[j >> 2] ^ 0x80808080u) >> (8 * (j & 3)) & 255u];
+          u[j] = f.x;
+          v[j] *= f.y;
+        }
+      } else {
+        decode8(r.q, group_step(r.byte), u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float value, slope;
+          if constexpr (ACT == ACT_GELU) gelu_both(u[j], value, slope);
+          else { value = relu_of(u[j]); slope = relu_slope(u[j]); }
+          v[j] *= slope;
+          u[j] = value;
+        }
       }
       if (a) store_run8<FAST>(a, a_dt, lda, a_vec, m, n, N, u);
     }
@@ -140,26 +169,30 @@ struct EpiInput {                            // dx = acc * act'(u), a = act(u), 
 
 struct EpiPlain {                            // the product itself
   void* out; long long ld; int M, N, dt; bool vec;
+  static constexpr int TABLE = 0;
+  __device__ __forceinline__ void fill(float2*, int, int) const {}
   struct Columns {};
   struct Row {};
   __device__ __forceinline__ void columns(int, Columns&) const {}
   template <bool FAST>
   __device__ __forceinline__ void fetch(int, int, Row&) const {}
   template <bool FAST, int X1, int X2>
-  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row&) const {
+  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row&, const float2*) const {
     if (m < M && n < N) store_run8<FAST>(out, dt, ld, vec, m, n, N, v);
   }
 };
 
 struct EpiPart {                             // fp32 partial sums [split][M][Np], Np = N rounded up to 8
   float* part; int M, Np;
+  static constexpr int TABLE = 0;
+  __device__ __forceinline__ void fill(float2*, int, int) const {}
   struct Columns {};
   struct Row {};
   __device__ __forceinline__ void columns(int, Columns&) const {}
   template <bool FAST>
   __device__ __forceinline__ void fetch(int, int, Row&) const {}
   template <bool FAST, int X1, int X2>
-  __device__ __forceinline__ void finish(int split, int m, int n, float (&v)[8], const Columns&, const Row&) const {
+  __device__ __forceinline__ void finish(int split, int m, int n, float (&v)[8], const Columns&, const Row&, const float2*) const {
     if (m < M && n < Np) store_vec8(part, DT_FP32, ((size_t)split * M + m) * Np + n, v);
   }
 };
@@ -186,7 +219,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
       v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
     }
   }
-  epi.template finish<false, 1, 2>(0, m, n, v, col, r);
+  epi.template finish<false, 1, 2>(0, m, n, v, col, r, nullptr);
 }
 
 // One block per row n of the weight's gradient:  G = sum of the parts, with x = xh * xs + xt put back

@@ -277,6 +277,27 @@ def test_linear_backward_input_large(M, K, N):
     check_input(M, N, K, "bf16", "gelu", False, "bf16")
 
 
+@pytest.mark.parametrize("M,N,K", [(200, 128, 264), (2600, 264, 4096)])
+def test_linear_backward_input_any_step(M, N, K):
+    """Pre-activations whose groups span many steps: those the GELU table holds, smaller and larger ones, zeros and NaN,
+    in one matrix; a group's result does not depend on the others of its wave."""
+    u = rnd(M, K) * torch.exp2(torch.randint(-14, 8, (M, 1), device="cuda").float()) * torch.exp2(torch.randint(-2, 3, (1, K), device="cuda").float())
+    u[5] = 0
+    u[7, 40] = float("nan")
+    saved = T.pack8(u)
+    dy, w = rnd(M, N, dtype=torch.bfloat16), rnd(N, K, dtype=torch.bfloat16, scale=N ** -0.5)
+    dx, a = T.linear_backward_input(dy, w, "gelu", saved, out_dtype=torch.float32, want_activation=True)
+    v = decode(saved.codes, saved.exponents)
+    ok = torch.isfinite(v)
+    assert torch.equal(torch.isnan(dx), ~ok) and torch.equal(torch.isnan(a), ~ok) and int((~ok).sum()) == 32
+    v = torch.where(ok, v, torch.zeros_like(v))
+    G, f = dy.double() @ w.double(), slope(v, "gelu")
+    bound = (N + 8) * 2 * U32 * (dy.double().abs() @ w.double().abs()) * f.abs() + G.abs() * (3e-7 + 4 * U32) + 2 * U32 * (G * f).abs()
+    within(torch.where(ok, dx.double(), torch.zeros_like(v)), torch.where(ok, G * f, torch.zeros_like(v)), bound, "dx")
+    value = act(v, "gelu")
+    within(torch.where(ok, a.double(), torch.zeros_like(v)), torch.where(ok, value, torch.zeros_like(v)), 2e-7 + (half_step(torch.bfloat16) + 4 * U32) * value.abs() + least(torch.bfloat16), "a")
+
+
 @pytest.mark.parametrize("layout", ["padded", "odd", "offset"])
 def test_linear_backward_input_layouts(layout):
     check_input(150, 136, 264, "bf16", "gelu", True, "bf16", layout)
