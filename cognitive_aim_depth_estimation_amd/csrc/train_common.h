@@ -61,16 +61,21 @@ template <int V> __device__ __forceinline__ void pack_half(const float (&y)[V], 
   if (dt == DT_BF16) { const bv h = __builtin_convertvector(v, bv); __builtin_memcpy(to, &h, 2 * V); }
   else { const hv h = __builtin_convertvector(v, hv); __builtin_memcpy(to, &h, 2 * V); }
 }
+template <bool STREAM = false>
 __device__ __forceinline__ void store_vec8(void* p, int dt, size_t off, const float (&y)[8]) {   // 16-byte aligned
   if (dt == DT_FP32) {
-    float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + off);
-    q[0] = make_float4(y[0], y[1], y[2], y[3]); q[1] = make_float4(y[4], y[5], y[6], y[7]);
+    f32x4* q = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + off);
+    const f32x4 a = {y[0], y[1], y[2], y[3]}, b = {y[4], y[5], y[6], y[7]};
+    if constexpr (STREAM) { __builtin_nontemporal_store(a, q); __builtin_nontemporal_store(b, q + 1); }
+    else { q[0] = a; q[1] = b; }
   } else {
     const f32x8 v = {y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
     u32x4v w;
     if (dt == DT_BF16) w = __builtin_bit_cast(u32x4v, __builtin_convertvector(v, bf16x8));
     else w = __builtin_bit_cast(u32x4v, __builtin_convertvector(v, f16x8));
-    *reinterpret_cast<u32x4v*>(reinterpret_cast<unsigned short*>(p) + off) = w;
+    u32x4v* q = reinterpret_cast<u32x4v*>(reinterpret_cast<unsigned short*>(p) + off);
+    if constexpr (STREAM) __builtin_nontemporal_store(w, q);
+    else *q = w;
   }
 }
 __device__ __forceinline__ float load_one(const void* p, int dt, size_t off) {

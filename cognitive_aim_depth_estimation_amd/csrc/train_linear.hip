@@ -16,12 +16,12 @@ constexpr long long MAX_LD = 1 << 21;      // a tile's 256 rows stay inside a bu
 // ---- epilogues ---------------------------------------------------------------------------------------------------
 // finish<FAST, X1, X2>: eight columns [n, n + 8) of row m; the four lanes that hold a group of 32 are X1 and X2 apart.
 // Every lane of the wave calls it (the 8-bit group maximum crosses lanes); rows and columns past the matrix are dropped
-// here.  FAST: the width is a multiple of eight and every array takes 16-byte accesses (`fast()`); the main loop carries
+// here.  FAST (stores past the caches: another pass reads them, and 2 % of the launch is saved for the operands' lines): the width is a multiple of eight and every array takes 16-byte accesses (`fast()`); the main loop carries
 // only that form, sixteen times unrolled, and leaves any other result to the join kernel.
 template <bool FAST>
 __device__ __forceinline__ void store_run8(void* p, int dt, long long ld, bool vec, int m, int n, int N, const float (&y)[8]) {
   const size_t at = (size_t)m * ld + n;
-  if (FAST || (vec && n + 8 <= N)) store_vec8(p, dt, at, y);
+  if (FAST || (vec && n + 8 <= N)) store_vec8<FAST>(p, dt, at, y);
   else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
