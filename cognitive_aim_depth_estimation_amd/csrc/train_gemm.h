@@ -226,11 +226,30 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
   ra.init(wm * (BM / TL::WM), lane);
   rb.init(wn * (BN / TL::WN), lane);
 
+  // sums begin at the bias (a lane's columns are the same for all its rows)
+  const int fr = lane & 15, fq = lane >> 4;
+  const int mw = m0 + wm * (BM / TL::WM) + fr, nw = n0 + wn * (BN / TL::WN) + 8 * fq;
   f32x4 acc[MI][NJ];
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+  for (int h = 0; h < NJ / 2; ++h) {
+    float b[8];
+    epi.start(nw + 32 * h, b);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < MI; ++i) {
+      acc[i][2 * h] = f32x4{b[0], b[1], b[2], b[3]};
+      acc[i][2 * h + 1] = f32x4{b[4], b[5], b[6], b[7]};
+    }
+  }
+  // what the epilogue reads (residual, 8-bit codes), requested here where the registers allow: its latency lies under the
+  // main loop then
+  constexpr bool FETCH_AHEAD = MI * NJ * 4 <= 64;
+  typename Epi::Row row[FETCH_AHEAD ? NJ / 2 : 1][MI];
+  if constexpr (FETCH_AHEAD) {
+#pragma unroll
+    for (int h = 0; h < NJ / 2; ++h)
+#pragma unroll
+      for (int i = 0; i < MI; ++i) epi.template fetch<true>(mw + 16 * i, nw + 32 * h, row[h][i]);
+  }
   // sums of A over k for the bias' gradient: products with a fragment of ones, the row fragments dealt to the WN waves
   // that share them; only the blocks of the first tile column
   constexpr bool SUMS = !AKC;
@@ -355,8 +374,6 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // the dropped loads past the end
-  const int fr = lane & 15, fq = lane >> 4;
-  const int mw = m0 + wm * (BM / TL::WM) + fr, nw = n0 + wn * (BN / TL::WN) + 8 * fq;
   if constexpr (SUMS) {
     if (with_sums && fq == 0) {
 #pragma unroll
@@ -371,15 +388,17 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
     const int n = nw + 32 * h;
     typename Epi::Columns col;
     epi.columns(n, col);
-    typename Epi::Row row[MI];                               // all reads of the strip ahead of its first store
+    typename Epi::Row (&now)[MI] = row[FETCH_AHEAD ? h : 0];
+    if constexpr (!FETCH_AHEAD) {                            // all reads of the strip ahead of its first store
 #pragma unroll
-    for (int i = 0; i < MI; ++i) epi.template fetch<true>(mw + 16 * i, n, row[i]);
+      for (int i = 0; i < MI; ++i) epi.template fetch<true>(mw + 16 * i, n, now[i]);
+    }
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       float v[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) { v[e] = acc[i][2 * h][e]; v[4 + e] = acc[i][2 * h + 1][e]; }
-      epi.template finish<true, 16, 32>(split, mw + 16 * i, n, v, col, row[i], table);
+      epi.template finish<true, 16, 32>(split, mw + 16 * i, n, v, col, now[i], table);
     }
   }
 }

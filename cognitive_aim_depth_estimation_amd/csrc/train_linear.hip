@@ -29,6 +29,20 @@ __device__ __forceinline__ void store_run8(void* p, int dt, long long ld, bool v
   }
 }
 
+// largest of the four lanes X1 and X2 apart: row swaps (16, 32) or quad permutations (1, 2), not the LDS permute's round trip
+template <int X1, int X2> __device__ __forceinline__ unsigned max_of_four(unsigned u) {
+  static_assert((X1 == 16 && X2 == 32) || (X1 == 1 && X2 == 2), "the two layouts of a group");
+  if constexpr (X1 == 16) {
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    u = umax(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return umax(b[0], b[1]);
+  } else {
+    u = umax(u, (unsigned)__builtin_amdgcn_mov_dpp((int)u, 0xB1 /* quad_perm [1,0,3,2] */, 0xf, 0xf, true));
+    return umax(u, (unsigned)__builtin_amdgcn_mov_dpp((int)u, 0x4E /* quad_perm [2,3,0,1] */, 0xf, 0xf, true));
+  }
+}
+
 template <int ACT>
 struct EpiForward {                          // y = act(acc + bias) * scale + residual, codes of acc + bias
   const float* bias; const float* scale; const void* res; void* y; signed char* codes; unsigned char* bytes;
@@ -36,13 +50,17 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
   static constexpr int TABLE = 0;            // float2 entries of LDS the epilogue wants
   __device__ __forceinline__ void fill(float2*, int, int) const {}
   bool fast() const { return (N & 7) == 0 && y_vec && (!res || res_vec) && (!codes || code_vec); }
-  struct Columns { float b[8], s[8]; };
+  struct Columns { float s[8]; };
   struct Row { Raw8 r; };
+  // where the sums of columns n .. n + 7 begin
+  __device__ __forceinline__ void start(int n, float (&b)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = bias ? bias[n + j < N ? n + j : N - 1] : 0.f;
+  }
   __device__ __forceinline__ void columns(int n, Columns& c) const {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int at = n + j < N ? n + j : N - 1;
-      c.b[j] = bias ? bias[at] : 0.f;
       c.s[j] = ACT == ACT_NONE && scale ? scale[at] : 1.f;
     }
   }
@@ -52,16 +70,13 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
   }
   template <bool FAST, int X1, int X2>
   __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns& c, const Row& r, const float2*) const {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += c.b[j];
     if (codes) {
       if constexpr (!FAST) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = n + j < N ? v[j] : 0.f;
       }
       unsigned top = n < N ? top_bits<8>(v) : 0u;
-      top = umax(top, (unsigned)__shfl_xor((int)top, X1, 64));
-      top = umax(top, (unsigned)__shfl_xor((int)top, X2, 64));
+      top = max_of_four<X1, X2>(top);
       if (m < M && n < N) {
         const unsigned byte = group_byte(top);
         const u32x2 q = pack_codes(v, byte);
@@ -119,6 +134,10 @@ struct EpiInput {
   bool fast() const { return (N & 7) == 0 && dx_vec && (!a || a_vec) && (!codes || code_vec); }
   struct Columns {};
   struct Row { u32x2 q; unsigned byte; };
+  __device__ __forceinline__ void start(int, float (&b)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = 0.f;
+  }
   __device__ __forceinline__ void columns(int, Columns&) const {}
   template <bool FAST>
   __device__ __forceinline__ void fetch(int m, int n, Row& r) const {
@@ -173,6 +192,10 @@ struct EpiPlain {                            // the product itself
   __device__ __forceinline__ void fill(float2*, int, int) const {}
   struct Columns {};
   struct Row {};
+  __device__ __forceinline__ void start(int, float (&b)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = 0.f;
+  }
   __device__ __forceinline__ void columns(int, Columns&) const {}
   template <bool FAST>
   __device__ __forceinline__ void fetch(int, int, Row&) const {}
@@ -188,6 +211,10 @@ struct EpiPart {                             // fp32 partial sums [split][M][Np]
   __device__ __forceinline__ void fill(float2*, int, int) const {}
   struct Columns {};
   struct Row {};
+  __device__ __forceinline__ void start(int, float (&b)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = 0.f;
+  }
   __device__ __forceinline__ void columns(int, Columns&) const {}
   template <bool FAST>
   __device__ __forceinline__ void fetch(int, int, Row&) const {}
@@ -210,8 +237,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
   typename Epi::Row r;
   epi.template fetch<false>(m, n, r);
   float v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  epi.start(n < N ? n : 0, v);
   if (m < M && n < N) {
     for (int s = 0; s < splits; ++s) {
       const float4* p = reinterpret_cast<const float4*>(part + ((size_t)s * M + m) * Np + n);
@@ -222,71 +248,131 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
   epi.template finish<false, 1, 2>(0, m, n, v, col, r, nullptr);
 }
 
-// One block per row n of the weight's gradient:  G = sum of the parts, with x = xh * xs + xt put back
-// (sum_m dy (xh xs + xt) = (dy^T xh) xs + (sum_m dy) xt);  dW = s G, db = s sum dy, ds = sum_k W G + b sum dy.
+// ROWS rows n of the weight's gradient to a block (their loads in flight together):  G = sum of the parts, with
+// x = xh * xs + xt put back  (sum_m dy (xh xs + xt) = (dy^T xh) xs + (sum_m dy) xt);  dW = s G, db = s sum dy,
+// ds = sum_k W G + b sum dy.  Four rows where they still make 512 blocks (12 against 17 us at 4096 x 1024 in two
+// parts); one row, for more blocks, below.
 struct WeightFinish {
-  const float* part; const float* col_sum; const float* xs; const float* xt; const float* scale; const void* W; const float* bias;
-  void* dW; float* db; float* ds; long long ldw, lddw; int N, K, Kp, splits, dt, dw_dt; bool vec;
+  const float* part; const float* col_sum; const float* xs; const float* xt; const float* scale; const unsigned short* W;
+  const float* bias; void* dW; float* db; float* ds; long long ldw, lddw; int N, K, Kp, splits, dt, dw_dt; bool vec;
 };
+template <int ROWS>
 __global__ __launch_bounds__(256) void weight_finish_kernel(WeightFinish a) {
-  __shared__ float red[4];
-  const int n = blockIdx.x;
-  float total = 0.f;
-  for (int s = 0; s < a.splits; ++s) total += a.col_sum[(size_t)s * a.N + n];
-  const float sc = a.scale ? a.scale[n] : 1.f;
-  float dot = 0.f;
+  __shared__ float red[ROWS][4];
+  const int n0 = blockIdx.x * ROWS;
+  int row[ROWS];
+  float total[ROWS], sc[ROWS], dot[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    row[r] = n0 + r < a.N ? n0 + r : a.N - 1;
+    total[r] = 0.f; dot[r] = 0.f;
+    sc[r] = a.scale ? a.scale[row[r]] : 1.f;
+  }
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) total[r] += a.col_sum[(size_t)s * a.N + row[r]];
   for (int k = threadIdx.x * 4; k < a.K; k += 1024) {
-    float g[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-      const float4 p = *reinterpret_cast<const float4*>(a.part + ((size_t)s * a.N + n) * a.Kp + k);
-      g[0] += p.x; g[1] += p.y; g[2] += p.z; g[3] += p.w;
+    f32x4 g[ROWS];
+    float w[ROWS][4];
+    if (a.ds) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const unsigned short* q = a.W + (size_t)row[r] * a.ldw + k;
+        unsigned short h[4] = {0, 0, 0, 0};
+        if (k + 4 <= a.K) __builtin_memcpy(h, q, 8);
+        else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) if (k + j < a.K) h[j] = q[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[r][j] = a.dt == DT_BF16 ? __uint_as_float((unsigned)h[j] << 16) : half_bits(h[j]);
+      }
     }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) g[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const f32x4 p = *reinterpret_cast<const f32x4*>(a.part + ((size_t)s * a.N + row[r]) * a.Kp + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) g[r][j] += p[j];
+      }
+    float xs[4], xt[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (k + j >= a.K) continue;
-      if (a.xs) g[j] *= a.xs[k + j];
-      if (a.xt) g[j] = __builtin_fmaf(total, a.xt[k + j], g[j]);
-      if (a.ds) dot = __builtin_fmaf(load_one(a.W, a.dt, (size_t)n * a.ldw + k + j), g[j], dot);
-      g[j] *= sc;
+      const int at = k + j < a.K ? k + j : a.K - 1;
+      xs[j] = a.xs ? a.xs[at] : 1.f;
+      xt[j] = a.xt ? a.xt[at] : 0.f;
     }
-    const size_t at = (size_t)n * a.lddw + k;
-    if (a.vec && k + 4 <= a.K && a.dw_dt == DT_FP32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.dW) + at) = make_float4(g[0], g[1], g[2], g[3]);
-    else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (k + j < a.K) store_one(a.dW, a.dw_dt, at + j, g[j]);
+    for (int r = 0; r < ROWS; ++r) {
+      if (n0 + r >= a.N) break;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (a.xs) g[r][j] *= xs[j];
+        if (a.xt) g[r][j] = __builtin_fmaf(total[r], xt[j], g[r][j]);
+        if (a.ds && k + j < a.K) dot[r] = __builtin_fmaf(w[r][j], g[r][j], dot[r]);
+        g[r][j] *= sc[r];
+      }
+      const size_t at = (size_t)row[r] * a.lddw + k;
+      if (a.vec && k + 4 <= a.K && a.dw_dt == DT_FP32) *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.dW) + at) = g[r];
+      else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (k + j < a.K) store_one(a.dW, a.dw_dt, at + j, g[r][j]);
+      }
     }
   }
   if (a.ds) {
-    dot = block_sum_256(dot, red);
-    if (threadIdx.x == 0) a.ds[n] = dot + (a.bias ? a.bias[n] * total : 0.f);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const float d = wave_sum_dpp(dot[r]);
+      if ((threadIdx.x & 63) == 0) red[r][threadIdx.x >> 6] = d;
+    }
+    __syncthreads();
   }
-  if (a.db && threadIdx.x == 0) a.db[n] = sc * total;
+  if (threadIdx.x < ROWS && n0 + (int)threadIdx.x < a.N) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if ((int)threadIdx.x == r) {
+        if (a.ds) a.ds[n0 + r] = (red[r][0] + red[r][1]) + (red[r][2] + red[r][3]) + (a.bias ? a.bias[n0 + r] * total[r] : 0.f);
+        a.db[n0 + r] = sc[r] * total[r];
+      }
+  }
 }
 
-// Copy of an operand whose rows 16-byte loads cannot address (odd widths, strides or bases), padded with zeros to a
-// multiple of eight columns; with `scale`, row r times scale[r] (rounded once to 16 bits: the matrix cores take it so).
-__global__ __launch_bounds__(256) void copy_rows_kernel(const unsigned short* __restrict__ src, long long ld, int R, int C, int C8,
-                                                        const float* __restrict__ scale, int dt, unsigned short* __restrict__ dst) {
-  const unsigned runs = (unsigned)C8 / 8;
-  const unsigned long long total = (unsigned long long)R * runs;
-  for (unsigned long long i = blockIdx.x * 256ULL + threadIdx.x; i < total; i += 256ULL * gridDim.x) {
-    const unsigned long long r = i / runs;
-    const int c = (int)(i - r * runs) * 8;
+// Copies of operands whose rows the DMA's 16-byte loads cannot address (odd widths, strides or bases), padded with zeros to
+// a multiple of eight columns; with `scale`, row r times scale[r] (rounded once to 16 bits: the matrix cores take it so).
+// Both operands of a product in one launch: blocks [0, blocks0) copy the first.
+struct CopyOne { const unsigned short* src; unsigned short* dst; const float* scale; long long ld; int rows, cols, padded; };
+struct CopyTwo { CopyOne one[2]; unsigned blocks0; int dt; };
+__global__ __launch_bounds__(256) void copy_rows_kernel(CopyTwo a) {
+  const bool second = blockIdx.x >= a.blocks0;
+  const CopyOne& c = a.one[second];
+  const unsigned block = second ? blockIdx.x - a.blocks0 : blockIdx.x, blocks = second ? gridDim.x - a.blocks0 : a.blocks0;
+  const unsigned runs = (unsigned)c.padded / 8;
+  const unsigned long long total = (unsigned long long)c.rows * runs;
+  for (unsigned long long i = block * 256ULL + threadIdx.x; i < total; i += 256ULL * blocks) {
+    const unsigned long long r = total < (1ULL << 32) ? (unsigned)i / runs : i / runs;
+    const int k0 = (int)(i - r * runs) * 8;
+    const unsigned short* src = c.src + r * c.ld + k0;
     u32x4v w;
+    if (k0 + 8 <= c.cols) __builtin_memcpy(&w, src, 16);               // of any alignment
+    else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      unsigned two = 0;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int k = c + 2 * j + e;
-        unsigned h = k < C ? src[r * ld + k] : 0u;
-        if (scale && k < C) h = bits16((dt == DT_BF16 ? __uint_as_float(h << 16) : half_bits((unsigned short)h)) * scale[r], dt);
-        two |= h << (16 * e);
-      }
-      w[j] = two;
+      for (int j = 0; j < 4; ++j) w[j] = (k0 + 2 * j < c.cols ? (unsigned)src[2 * j] : 0u) | (k0 + 2 * j + 1 < c.cols ? (unsigned)src[2 * j + 1] << 16 : 0u);
     }
-    *reinterpret_cast<u32x4v*>(dst + r * C8 + c) = w;
+    if (c.scale) {
+      const float s = c.scale[r];
+      float v[8];
+      cvt_raw8(Raw8{w, w}, a.dt, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = k0 + j < c.cols ? v[j] * s : 0.f;   // the padding stays zero whatever the scale
+      pack_half<8>(v, a.dt, &w);
+    }
+    *reinterpret_cast<u32x4v*>(c.dst + r * c.padded + k0) = w;
   }
 }
 
@@ -294,7 +380,7 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(const unsigned short* __
 using T256 = Tile<256, 256, 2, 4, 2, true>;
 using T192 = Tile<192, 256, 2, 4, 2, true>;        // A contiguous along k only: its 192 columns across k have no XOR swizzle
 using T128W = Tile<128, 256, 2, 4, 2, true>;
-using T128 = Tile<128, 128, 2, 2, 2, false>;
+using T128 = Tile<128, 128, 2, 2, 2, true>;
 using T64 = Tile<64, 64, 2, 2, 4, false>;
 enum { TILE_256, TILE_192, TILE_128W, TILE_128, TILE_64, TILES };
 // What a launch takes, in us, measured on MI355X over 14 shapes from 5 x 1024 x 1024 to 21920 x 768 x 768 and each of the
@@ -302,11 +388,11 @@ enum { TILE_256, TILE_192, TILE_128W, TILE_128, TILE_64, TILES };
 // its first loads and its stores; when at most half the slots are taken, a K-tile takes alone_k (less traffic, higher
 // clock).  A wide tile reads the fewest bytes per product, a small one leaves fewer compute units idle in the last
 // round: 5480 x 4096 x 1024 takes 58 us in 256 x 256 tiles (352 on 256 units), 50 in 192 x 256 (464), 53 in 128 x 256,
-// 58 in 128 x 128 and 99 in 64 x 64; 1370 x 768 x 768 takes 22, 18, 15, 13 and 9.5; 10960 x 4096 x 1024 takes 93, 99,
-// 104, 106 and 195.
+// 54 in 128 x 128 and 99 in 64 x 64; 1370 x 768 x 768 takes 22, 18, 15, 12 and 9.5; 10960 x 4096 x 1024 takes 89, 98,
+// 104, 100 and 195.
 struct TileCost { int m, n, slots; float per_k, fixed, alone_k; };
 const TileCost TILE_COST[TILES] = {{256, 256, 256, 1.50f, 4.5f, 1.20f}, {192, 256, 256, 1.33f, 4.0f, 1.00f}, {128, 256, 256, 0.87f, 4.0f, 0.75f},
-                                   {128, 128, 512, 0.98f, 2.2f, 0.80f}, {64, 64, 512, 0.43f, 2.5f, 0.35f}};
+                                   {128, 128, 512, 0.92f, 2.6f, 0.61f}, {64, 64, 512, 0.43f, 2.5f, 0.35f}};
 // Splitting the sum over k takes another kernel: about 5 us of launch and latency, and each partial sum written and
 // read back once at 5 TB/s.
 constexpr float JOIN_FIXED = 5.f, JOIN_PER_BYTE = 1.f / 5.0e6f;
@@ -355,16 +441,24 @@ Side side(const void* p, long long ld, int rows, int cols, const float* scale = 
 }
 long long copy_bytes(const Side& s) { return s.copy ? round256((long long)s.rows * round8(s.cols) * 2) : 0; }
 
-int run_copy(Side& s, int dt, char*& ws, hipStream_t st) {
-  if (!s.copy) return COGAIM_OK;
-  const int c8 = round8(s.cols);
-  const unsigned long long runs = (unsigned long long)s.rows * (c8 / 8);
-  unsigned long long blocks = (runs + 255) / 256;
-  if (blocks > 256 * 32) blocks = 256 * 32;
-  hipLaunchKernelGGL(copy_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, st, (const unsigned short*)s.p, s.ld, s.rows, s.cols, c8,
-                     s.scale, dt, (unsigned short*)ws);
-  s.p = ws; s.ld = c8; s.cols = c8;
-  ws += round256((long long)s.rows * c8 * 2);
+// copies those of the two operands that need it, moves `ws` behind them
+int run_copies(Side& a, Side& b, int dt, char*& ws, hipStream_t st) {
+  CopyTwo c{};
+  c.dt = dt;
+  unsigned blocks[2] = {0, 0};
+  int n = 0;
+  for (Side* s : {&a, &b}) {
+    if (!s->copy) continue;
+    const int c8 = round8(s->cols);
+    c.one[n] = CopyOne{(const unsigned short*)s->p, (unsigned short*)ws, s->scale, s->ld, s->rows, s->cols, c8};
+    const unsigned long long want = ((unsigned long long)s->rows * (c8 / 8) + 255) / 256;
+    blocks[n++] = (unsigned)(want > 256 * 16 ? 256 * 16 : want);
+    s->p = ws; s->ld = c8; s->cols = c8;
+    ws += round256((long long)s->rows * c8 * 2);
+  }
+  if (n == 0) return COGAIM_OK;
+  c.blocks0 = blocks[0];
+  hipLaunchKernelGGL(copy_rows_kernel, dim3(blocks[0] + blocks[1]), dim3(256), 0, st, c);
   return COGAIM_LAUNCH_CHECK();
 }
 
@@ -466,8 +560,7 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long lon
   const Shape s = shape_of(d->M, d->N, d->K, true, !forward_epi<ACT_NONE>(d).fast());
   Side a = side(d->x, d->ldx, d->M, d->K), b = side(d->w, d->ldw, d->N, d->K);
   char* ws = (char*)workspace;
-  int rc = run_copy(a, d->dtype, ws, st);
-  if (!rc) rc = run_copy(b, d->dtype, ws, st);
+  const int rc = run_copies(a, b, d->dtype, ws, st);
   if (rc) return rc;
   const Operands g = operands(a, b, true, true, d->M, d->N, s);
 #define FWD_RUN(T_)                                                                                                    \
@@ -491,8 +584,7 @@ int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspa
   const Shape s = shape_of(d->M, d->K, d->N, true, !input_epi<ACT_NONE>(d).fast());
   Side a = side(d->dy, d->lddy, d->M, d->N), b = side(d->w, d->ldw, d->N, d->K, d->scale);
   char* ws = (char*)workspace;
-  int rc = run_copy(a, d->dtype, ws, st);
-  if (!rc) rc = run_copy(b, d->dtype, ws, st);
+  const int rc = run_copies(a, b, d->dtype, ws, st);
   if (rc) return rc;
   const Operands g = operands(a, b, true, false, d->M, d->K, s);
 #define IN_RUN(T_)                                                                                                     \
@@ -523,7 +615,8 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
   const Shape s = shape_of(d->N, d->K, d->M, false, weight_has_more(d));
   char* ws = (char*)workspace;
   Side a = side(d->dy, d->lddy, d->M, d->N), b{};
-  int rc = run_copy(a, d->dtype, ws, st);
+  if (!d->codes) b = side(d->x, d->ldx, d->M, d->K);
+  int rc = run_copies(a, b, d->dtype, ws, st);
   if (rc) return rc;
   if (d->codes) {
     // the 8-bit rows as 16-bit values in front of the product (a power-of-two step makes them exact in bf16)
@@ -531,11 +624,8 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
     rc = cogaim_unpack8(d->codes, d->exponents, ws, d->dtype, k8, d->M, d->K, k8, stream);
     b = Side{ws, k8, d->M, k8, false, nullptr};
     ws += round256((long long)d->M * k8 * 2);
-  } else {
-    b = side(d->x, d->ldx, d->M, d->K);
-    rc = run_copy(b, d->dtype, ws, st);
+    if (rc) return rc;
   }
-  if (rc) return rc;
   Operands g = operands(a, b, false, false, d->N, d->K, s);
   if (!weight_needs_finish(d, s)) {
     g.col_sum = d->db;
@@ -549,9 +639,10 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
   const EpiPart e{part, d->N, kp};
   rc = d->dtype == DT_BF16 ? launch_gemm<__bf16, false, false>(g, s.tile, e, st) : launch_gemm<_Float16, false, false>(g, s.tile, e, st);
   if (rc) return rc;
-  const WeightFinish f{part, sums, d->x_scale, d->x_shift, d->scale, d->w, d->bias, d->dw, d->db, d->ds, d->ldw, d->lddw,
+  const WeightFinish f{part, sums, d->x_scale, d->x_shift, d->scale, (const unsigned short*)d->w, d->bias, d->dw, d->db, d->ds, d->ldw, d->lddw,
                        d->N, d->K, kp, s.splits, d->dtype, d->dw_dtype, vec_ok(d->dw, d->lddw)};
-  hipLaunchKernelGGL(weight_finish_kernel, dim3(d->N), dim3(256), 0, st, f);
+  if (d->N >= 4 * 512) hipLaunchKernelGGL(weight_finish_kernel<4>, dim3((d->N + 3) / 4), dim3(256), 0, st, f);
+  else hipLaunchKernelGGL(weight_finish_kernel<1>, dim3(d->N), dim3(256), 0, st, f);
   return COGAIM_LAUNCH_CHECK();
 }
 
