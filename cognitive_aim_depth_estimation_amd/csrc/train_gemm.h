@@ -243,7 +243,7 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
   // what the epilogue reads (residual, 8-bit codes), requested here where the registers allow: its latency lies under the
   // main loop then
   constexpr bool FETCH_AHEAD = MI * NJ * 4 <= 64;
-  typename Epi::Row row[FETCH_AHEAD ? NJ / 2 : 1][MI];
+  typename Epi::Row row[NJ / 2][FETCH_AHEAD ? MI : 2];
   if constexpr (FETCH_AHEAD) {
 #pragma unroll
     for (int h = 0; h < NJ / 2; ++h)
@@ -383,22 +383,24 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
       }
     }
   }
+  typename Epi::Columns col[NJ / 2];
 #pragma unroll
-  for (int h = 0; h < NJ / 2; ++h) {
-    const int n = nw + 32 * h;
-    typename Epi::Columns col;
-    epi.columns(n, col);
-    typename Epi::Row (&now)[MI] = row[FETCH_AHEAD ? h : 0];
-    if constexpr (!FETCH_AHEAD) {                            // all reads of the strip ahead of its first store
+  for (int h = 0; h < NJ / 2; ++h) epi.columns(nw + 32 * h, col[h]);
+  auto fetch_row = [&](int i) __attribute__((always_inline)) {
+    if constexpr (!FETCH_AHEAD)
 #pragma unroll
-      for (int i = 0; i < MI; ++i) epi.template fetch<true>(mw + 16 * i, n, now[i]);
-    }
+      for (int h = 0; h < NJ / 2; ++h) epi.template fetch<true>(mw + 16 * i, nw + 32 * h, row[h][i & 1]);
+  };
+  fetch_row(0);
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
+  for (int i = 0; i < MI; ++i) {
+    if (i + 1 < MI) fetch_row(i + 1);                          // ahead of this row's stores
+#pragma unroll
+    for (int h = 0; h < NJ / 2; ++h) {
       float v[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) { v[e] = acc[i][2 * h][e]; v[4 + e] = acc[i][2 * h + 1][e]; }
-      epi.template finish<true, 16, 32>(split, mw + 16 * i, n, v, col, now[i], table);
+      epi.template finish<true, 16, 32>(split, mw + 16 * i, nw + 32 * h, v, col[h], row[h][FETCH_AHEAD ? i : i & 1], table);
     }
   }
 }

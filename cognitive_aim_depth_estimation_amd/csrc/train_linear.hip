@@ -18,8 +18,39 @@ constexpr long long MAX_LD = 1 << 21;      // a tile's 256 rows stay inside a bu
 // Every lane of the wave calls it (the 8-bit group maximum crosses lanes); rows and columns past the matrix are dropped
 // here.  FAST (stores past the caches: another pass reads them, and 2 % of the launch is saved for the operands' lines): the width is a multiple of eight and every array takes 16-byte accesses (`fast()`); the main loop carries
 // only that form, sixteen times unrolled, and leaves any other result to the join kernel.
-template <bool FAST>
-__device__ __forceinline__ void store_run8(void* p, int dt, long long ld, bool vec, int m, int n, int N, const float (&y)[8]) {
+//
+// fp32 rows: a lane's eight columns are 32 bytes, and a 16-byte access of every lane would touch half of each sector.  The
+// row swap of lane halves turns them (lane bit 5 against the half of the eight): a lane then holds columns
+// 8 (q % 2) + 4 (q / 2) .. + 3 of the first and of the last 16 of its group of 32, and an access covers 64 bytes of a row.
+__device__ __forceinline__ void turn8(float (&y)[8]) {                    // its own inverse
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(y[j]), __float_as_uint(y[4 + j]), false, false);
+    y[j] = __uint_as_float(t[0]); y[4 + j] = __uint_as_float(t[1]);
+  }
+}
+__device__ __forceinline__ int turned_column(int n) {                     // of the first of the two; the other is 16 on
+  const int q = (n >> 3) & 3;
+  return (n & ~(GROUP - 1)) + 8 * (q & 1) + 4 * (q >> 1);
+}
+// FAST calls come from whole waves but for lanes past the last row
+template <bool FAST, bool STREAM = true>
+__device__ __forceinline__ void store_run8(void* p, int dt, long long ld, bool vec, int m, int n, int N, float (&y)[8]) {
+  if (FAST && dt == DT_FP32) {
+    turn8(y);
+    const int c = turned_column(n);
+    f32x4* q = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + (size_t)m * ld + c);
+    const f32x4 lo = {y[0], y[1], y[2], y[3]}, hi = {y[4], y[5], y[6], y[7]};
+    if constexpr (STREAM) {
+      if (c < N) __builtin_nontemporal_store(lo, q);
+      if (c + 16 < N) __builtin_nontemporal_store(hi, q + 4);
+    } else {
+      if (c < N) q[0] = lo;
+      if (c + 16 < N) q[4] = hi;
+    }
+    return;
+  }
+  if (n >= N) return;
   const size_t at = (size_t)m * ld + n;
   if (FAST || (vec && n + 8 <= N)) store_vec8<FAST>(p, dt, at, y);
   else {
@@ -66,7 +97,13 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
   }
   template <bool FAST>
   __device__ __forceinline__ void fetch(int m, int n, Row& r) const {
-    if (res && (FAST || (res_vec && n + 8 <= N)) && m < M && n < N) r.r = load_raw8(res, res_dt, (size_t)m * ldr + n);
+    if (!res || m >= M) return;
+    if (FAST && res_dt == DT_FP32) {
+      const int c = turned_column(n);
+      const u32x4v* q = reinterpret_cast<const u32x4v*>(reinterpret_cast<const float*>(res) + (size_t)m * ldr + c);
+      r.r.a = c < N ? q[0] : u32x4v{0, 0, 0, 0};
+      r.r.b = c + 16 < N ? q[4] : u32x4v{0, 0, 0, 0};
+    } else if ((FAST || (res_vec && n + 8 <= N)) && n < N) r.r = load_raw8(res, res_dt, (size_t)m * ldr + n);
   }
   template <bool FAST, int X1, int X2>
   __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns& c, const Row& r, const float2*) const {
@@ -90,7 +127,7 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
         if ((n & (GROUP - 1)) == 0) bytes[(size_t)m * groups_of(N) + n / GROUP] = (unsigned char)byte;
       }
     }
-    if (m >= M || n >= N) return;
+    if (m >= M) return;                          // lanes of one row leave together
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if constexpr (ACT == ACT_RELU) v[j] = relu_of(v[j]);
@@ -99,8 +136,10 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
     }
     if (res) {
       float a[8];
-      if (FAST || (res_vec && n + 8 <= N)) cvt_raw8(r.r, res_dt, a);
-      else {
+      if (FAST || (res_vec && n + 8 <= N)) {
+        cvt_raw8(r.r, res_dt, a);
+        if (FAST && res_dt == DT_FP32) turn8(a);
+      } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) a[j] = n + j < N ? load_one(res, res_dt, (size_t)m * ldr + n + j) : 0.f;
       }
@@ -141,12 +180,12 @@ struct EpiInput {
   __device__ __forceinline__ void columns(int, Columns&) const {}
   template <bool FAST>
   __device__ __forceinline__ void fetch(int m, int n, Row& r) const {
+    r.q = u32x2{0, 0}; r.byte = 1;
     if constexpr (ACT != ACT_NONE) {
       if (m < M && n < N) {
         const signed char* p = codes + (size_t)m * N + n;
         if (FAST || (code_vec && n + 8 <= N)) r.q = *reinterpret_cast<const u32x2*>(p);
         else {
-          r.q = u32x2{0, 0};
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             if (n + j < N) r.q[j >> 2] |= (unsigned)(unsigned char)p[j] << (8 * (j & 3));
@@ -157,12 +196,12 @@ struct EpiInput {
   }
   template <bool FAST, int X1, int X2>
   __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row& r, const float2* table) const {
-    if (m >= M || n >= N) return;
+    if (m >= M) return;                          // lanes of one row leave together
     if constexpr (ACT != ACT_NONE) {
       float u[8];
-      const bool listed = ACT == ACT_GELU && FAST && r.byte - TABLE_FIRST < (unsigned)TABLE_STEPS;
+      const bool listed = ACT == ACT_GELU && FAST && (n >= N || r.byte - TABLE_FIRST < (unsigned)TABLE_STEPS);
       if (ACT == ACT_GELU && FAST && __all(listed)) {
-        const float2* t = table + ((r.byte - TABLE_FIRST) << 8);
+        const float2* t = table + (n < N ? (r.byte - TABLE_FIRST) << 8 : 0u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float2 f = t[(r.q[j >> 2] ^ 0x80808080u) >> (8 * (j & 3)) & 255u];
@@ -201,7 +240,7 @@ struct EpiPlain {                            // the product itself
   __device__ __forceinline__ void fetch(int, int, Row&) const {}
   template <bool FAST, int X1, int X2>
   __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row&, const float2*) const {
-    if (m < M && n < N) store_run8<FAST>(out, dt, ld, vec, m, n, N, v);
+    if (m < M) store_run8<FAST>(out, dt, ld, vec, m, n, N, v);
   }
 };
 
@@ -220,7 +259,7 @@ struct EpiPart {                             // fp32 partial sums [split][M][Np]
   __device__ __forceinline__ void fetch(int, int, Row&) const {}
   template <bool FAST, int X1, int X2>
   __device__ __forceinline__ void finish(int split, int m, int n, float (&v)[8], const Columns&, const Row&, const float2*) const {
-    if (m < M && n < Np) store_vec8(part, DT_FP32, ((size_t)split * M + m) * Np + n, v);
+    if (m < M) store_run8<true, false>(part + (size_t)split * M * Np, DT_FP32, Np, true, m, n, Np, v);      // read back at once
   }
 };
 
