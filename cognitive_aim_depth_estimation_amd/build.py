@@ -1,4 +1,4 @@
-"""Builds libcogaim.so (hipcc, gfx950 only) in-tree next to the sources."""
+"""Builds libcogaim.so (hipcc, gfx950 only) and the host module of training.py in-tree next to the sources."""
 from __future__ import annotations
 
 import os
@@ -8,6 +8,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcogaim.so")
+HOST = os.path.join(HERE, "_host.so")            # host side of training.py: a Python module on torch's C++ API
 SOURCES = ["gemm.hip", "gemm_rowln.hip", "attention.hip", "rowwise.hip", "focal.hip", "small.hip", "preprocess.hip",
            "train_rows.hip", "train_linear.hip"]
 # attention.hip: without NaN-honouring, fmaxf on MFMA results needs no canonicalising v_max (x3 fewer max ops)
@@ -24,11 +25,22 @@ def _hipcc() -> str:
 
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(HOST):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(HOST))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "cogaim.h")]
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _host_command():
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-I" + os.path.join(root, "include"),
+            "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I/opt/rocm/include",
+            "-I" + sysconfig.get_paths()["include"], os.path.join(CSRC, "host_training.cpp"), "-o", HOST, "-L" + os.path.join(root, "lib"),
+            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"]
 
 
 def build(force: bool = False, verbose: bool = True) -> str:
@@ -45,11 +57,15 @@ def build(force: bool = False, verbose: bool = True) -> str:
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
         objs.append(obj)
+    cmd = _host_command()
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    procs.append(("host_training.cpp", subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     for src, p in procs:
         out, _ = p.communicate()
         if p.returncode != 0:
             sys.stderr.write(out.decode())
-            raise RuntimeError(f"hipcc failed on {src}")
+            raise RuntimeError(f"the compiler failed on {src}")
     cmd = [_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
     if verbose:
         print(" ".join(cmd), flush=True)
