@@ -750,6 +750,20 @@ class CognitiveAimModel(nn.Module):
                         other["pending"] = False
                 raise err
 
+    def encoder_mlp(self, layer: int, hidden: torch.Tensor) -> torch.Tensor:
+        """The MLP half of encoder layer ``layer`` (hf:372-378) on ``hidden [..., D]`` (fp32, bf16 or fp16 residual stream):
+        ``x + layer_scale2 * fc2(gelu(fc1(norm2(x))))``, differentiable in ``hidden`` and in those of the layer's parameters
+        that require a gradient (they do not by default: ``p.requires_grad_()``).  Matrix operands are rounded to
+        ``compute_dtype`` as in the forward; what the backward pass needs is kept in 8 bits (``training.mlp_half``)."""
+        if not 0 <= layer < self.num_layers:
+            raise IndexError(f"encoder layer {layer}: the model has {self.num_layers}")
+        if hidden.shape[-1] != self.feature_dim:
+            raise ValueError(f"hidden has rows of {hidden.shape[-1]}, the encoder is {self.feature_dim} wide")
+        from .training import mlp_half
+        p = getattr(self.backbone.encoder.layer, str(layer))
+        return mlp_half(hidden, p.norm2.weight, p.norm2.bias, p.mlp.fc1.weight, p.mlp.fc1.bias, p.mlp.fc2.weight, p.mlp.fc2.bias,
+                        p.layer_scale2.lambda1, self.layer_norm_eps, _DTYPES[self.compute_dtype][1])
+
     def synchronize(self):
         """Waits for all queued work of this model and raises any deferred device-side condition."""
         torch.cuda.synchronize()

@@ -529,6 +529,42 @@ def test_gradients_against_differences():
         assert abs((val[1] - val[0]) / (2 * e) - want) <= size * (10 * e * e / 6 + 64 * U32 / e), (i, val, want)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_encoder_mlp_trains_a_layer(dtype):
+    """The model's own entry: value and gradients of one layer's MLP half on a residual stream, and the forward that follows
+    an in-place step sees the new weights."""
+    from util import default_exif, synth_model_and_sd
+    model, _ = synth_model_and_sd(layers=2, native_grid=4, dtype=dtype)
+    D = model.feature_dim
+    x = rnd(2, 17, D, scale=1.5).requires_grad_()
+    layer = getattr(model.backbone.encoder.layer, "1")
+    named = [layer.norm2.weight, layer.norm2.bias, layer.mlp.fc1.weight, layer.mlp.fc1.bias, layer.mlp.fc2.weight, layer.mlp.fc2.bias, layer.layer_scale2.lambda1]
+    for p in named:
+        p.requires_grad_()
+    y = model.encoder_mlp(1, x)
+    assert y.shape == x.shape and y.dtype == torch.float32
+    dy = rnd(2, 17, D)
+    grads = torch.autograd.grad(y, [x] + named, dy)
+    q = [v.detach().double().requires_grad_() for v in [x] + named]
+    ref = mlp_plain(q[0], q[1], q[2], q[3], q[4], q[5], q[6], q[7], model.layer_norm_eps)
+    want = torch.autograd.grad(ref, q, dy.double())
+    assert float((y.detach().double() - ref.detach()).norm() / ref.detach().norm()) <= 4 * half_step(DT[dtype])
+    bound = 2 * (0.0136 * 1.8 + 5 * half_step(torch.bfloat16))          # as in test_mlp_half_gradients
+    for g, r in zip(grads, want):
+        assert float((g.double() - r).norm() / r.norm()) <= bound
+    images, exif = torch.randn(2, 3, 56, 56, device="cuda"), default_exif(2, "cuda")
+    with torch.no_grad():
+        before = model(images, exif)[0].clone()
+        for p, g in zip(named, grads[1:]):
+            p.add_(g, alpha=-0.05)
+        after = model(images, exif)[0]
+    assert bool(torch.isfinite(after).all()) and not torch.equal(before, after)
+    with pytest.raises(IndexError):
+        model.encoder_mlp(2, x)
+    with pytest.raises(ValueError):
+        model.encoder_mlp(0, x[..., :64])
+
+
 def test_only_wanted_gradients_and_leading_dims():
     p = mlp_tensors(2 * 15, 64, 96)
     x = p[0].detach().view(2, 15, 64)
