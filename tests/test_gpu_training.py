@@ -18,7 +18,8 @@ DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 def _dev():
     assert torch.cuda.is_available(), "these tests need the MI355X"
     torch.manual_seed(0)
-    yield
+    with torch.enable_grad():            # other test modules switch gradients off for the whole process
+        yield
     torch.cuda.synchronize()
 
 
