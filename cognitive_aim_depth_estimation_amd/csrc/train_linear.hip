@@ -6,6 +6,7 @@
 // the parts leave fp32 partial tiles in the workspace and a join kernel adds them in order and applies the epilogue
 // (no atomics: results do not depend on timing).
 #include "train_gemm.h"
+#include "train_few.h"
 #include "../../include/cogaim.h"
 
 namespace {
@@ -571,6 +572,9 @@ bool weight_ok(const cogaim_linear_bwd_weight_desc* d) {
 }
 }  // namespace
 
+#ifdef NOFEW
+#define few_rows(...) false
+#endif
 // the epilogues of a descriptor
 template <int ACT> EpiForward<ACT> forward_epi(const cogaim_linear_fwd_desc* d) {
   return EpiForward<ACT>{d->bias, d->scale, d->residual, d->y, (signed char*)d->codes, (unsigned char*)d->exponents, d->ldr,
@@ -587,6 +591,7 @@ extern "C" {
 
 long long cogaim_linear_fwd_workspace_bytes(const cogaim_linear_fwd_desc* d) {
   if (!forward_ok(d)) return COGAIM_EINVAL;
+  if (few_rows(d->M, d->N, d->K, true)) return 0;
   const Shape s = shape_of(d->M, d->N, d->K, true, !forward_epi<ACT_NONE>(d).fast());
   return copy_bytes(side(d->x, d->ldx, d->M, d->K)) + copy_bytes(side(d->w, d->ldw, d->N, d->K)) +
          (joins(s, forward_epi<ACT_NONE>(d)) ? (long long)s.splits * d->M * round8(d->N) * 4 : 0);
@@ -596,6 +601,15 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long lon
   const long long need = cogaim_linear_fwd_workspace_bytes(d);
   if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
   hipStream_t st = (hipStream_t)stream;
+  if (few_rows(d->M, d->N, d->K, true)) {
+    const Few f{d->x, d->w, nullptr, d->ldx, d->ldw, d->M, d->N, d->K};
+#define FEW_RUN(T_, DT_)                                                                      \
+  (d->activation == ACT_RELU ? launch_few<T_, DT_, true>(f, forward_epi<ACT_RELU>(d), st)      \
+   : d->activation == ACT_GELU ? launch_few<T_, DT_, true>(f, forward_epi<ACT_GELU>(d), st)    \
+                               : launch_few<T_, DT_, true>(f, forward_epi<ACT_NONE>(d), st))
+    return d->dtype == DT_BF16 ? FEW_RUN(__bf16, DT_BF16) : FEW_RUN(_Float16, DT_FP16);
+#undef FEW_RUN
+  }
   const Shape s = shape_of(d->M, d->N, d->K, true, !forward_epi<ACT_NONE>(d).fast());
   Side a = side(d->x, d->ldx, d->M, d->K), b = side(d->w, d->ldw, d->N, d->K);
   char* ws = (char*)workspace;
@@ -611,6 +625,7 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long lon
 
 long long cogaim_linear_bwd_input_workspace_bytes(const cogaim_linear_bwd_input_desc* d) {
   if (!input_ok(d)) return COGAIM_EINVAL;
+  if (few_rows(d->M, d->K, d->N, false)) return 0;
   const Shape s = shape_of(d->M, d->K, d->N, true, !input_epi<ACT_NONE>(d).fast());
   return copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + copy_bytes(side(d->w, d->ldw, d->N, d->K, d->scale)) +
          (joins(s, input_epi<ACT_NONE>(d)) ? (long long)s.splits * d->M * round8(d->K) * 4 : 0);
@@ -620,6 +635,15 @@ int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspa
   const long long need = cogaim_linear_bwd_input_workspace_bytes(d);
   if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
   hipStream_t st = (hipStream_t)stream;
+  if (few_rows(d->M, d->K, d->N, false)) {
+    const Few f{d->dy, d->w, d->scale, d->lddy, d->ldw, d->M, d->K, d->N};
+#define FEW_RUN(T_, DT_)                                                                      \
+  (d->activation == ACT_RELU ? launch_few<T_, DT_, false>(f, input_epi<ACT_RELU>(d), st)       \
+   : d->activation == ACT_GELU ? launch_few<T_, DT_, false>(f, input_epi<ACT_GELU>(d), st)     \
+                               : launch_few<T_, DT_, false>(f, input_epi<ACT_NONE>(d), st))
+    return d->dtype == DT_BF16 ? FEW_RUN(__bf16, DT_BF16) : FEW_RUN(_Float16, DT_FP16);
+#undef FEW_RUN
+  }
   const Shape s = shape_of(d->M, d->K, d->N, true, !input_epi<ACT_NONE>(d).fast());
   Side a = side(d->dy, d->lddy, d->M, d->N), b = side(d->w, d->ldw, d->N, d->K, d->scale);
   char* ws = (char*)workspace;

@@ -209,7 +209,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_fwd_kernel(LnF
 // kernel, so the result does not depend on timing (no atomics).
 struct LnBwd {
   const void* dy; const void* x; const signed char* codes; const unsigned char* bytes; const float* mean; const float* rstd;
-  const float* gamma; const void* add; void* dx; float* part;
+  const float* gamma; const void* add; void* dx; float* part; float* dgamma; float* dbeta;
   long long lddy, ldx, ldadd, lddx; int M, D, add_dt, dx_dt;
 };
 
@@ -303,10 +303,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnB
       }
     }
   }
-  // the block's partial row: dgamma at part[block][0][.], dbeta at part[block][1][.]
-  float* out = a.part + (size_t)blockIdx.x * 2 * a.D;
+  // the block's partial row: dgamma at part[block][0][.], dbeta at part[block][1][.]; a single block's is the result
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
+    float* out = gridDim.x == 1 ? (which ? a.dbeta : a.dgamma) : a.part + ((size_t)blockIdx.x * 2 + which) * a.D;
     if constexpr (RPB > 1) {
       __syncthreads();
 #pragma unroll
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnB
         float s = acc[at];
 #pragma unroll
         for (int w = 1; w < RPB; ++w) s += acc[w * NCH * V * TPR + at];
-        out[which * a.D + c] = s;
+        out[c] = s;
       }
     } else {
 #pragma unroll
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnB
         const int c = (t + TPR * i) * V;
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (c + j < a.D) out[which * a.D + c + j] = which ? db[i][j] : dg[i][j];
+          if (c + j < a.D) out[c + j] = which ? db[i][j] : dg[i][j];
       }
     }
   }
@@ -532,12 +532,12 @@ int cogaim_layernorm_bwd(const void* dy, int dy_dtype, long long lddy, const voi
       workspace_bytes < cogaim_layernorm_bwd_workspace_bytes(M, D))
     return COGAIM_EINVAL;
   const LnBwd a{dy, x, (const signed char*)codes, (const unsigned char*)exponents, mean, rstd, gamma, add, dx,
-                (float*)workspace, lddy, ldx, ldadd, lddx, M, D, add_dtype, dx_dtype};
+                (float*)workspace, dgamma, dbeta, lddy, ldx, ldadd, lddx, M, D, add_dtype, dx_dtype};
   const int nblk = ln_bwd_blocks(M, D);
   if (dy_dtype == DT_BF16) run_ln_bwd_from<DT_BF16>(a, x_dtype, nblk, (hipStream_t)stream);
   else if (dy_dtype == DT_FP16) run_ln_bwd_from<DT_FP16>(a, x_dtype, nblk, (hipStream_t)stream);
   else run_ln_bwd_from<DT_FP32>(a, x_dtype, nblk, (hipStream_t)stream);
-  hipLaunchKernelGGL(ln_train_reduce_kernel, dim3((2 * D + 31) / 32), dim3(1024), 0, (hipStream_t)stream,
+  if (nblk > 1) hipLaunchKernelGGL(ln_train_reduce_kernel, dim3((2 * D + 31) / 32), dim3(1024), 0, (hipStream_t)stream,
                      (const float*)workspace, dgamma, dbeta, nblk, D);
   return COGAIM_LAUNCH_CHECK();
 }

@@ -187,7 +187,8 @@ def test_layer_norm_non_finite_rows_stay_in_their_row():
 
 # ---- linear layers -----------------------------------------------------------------------------------------------
 SHAPES = [(1, 1, 1), (1, 8, 8), (5, 64, 64), (3, 577, 588), (65, 129, 72), (130, 256, 768), (64, 200, 8), (257, 1000, 264),
-          (31, 24, 4096), (1000, 96, 100), (9, 2048, 1024), (300, 1544, 520)]
+          (31, 24, 4096), (1000, 96, 100), (9, 2048, 1024), (300, 1544, 520), (16, 2052, 1000), (17, 100, 72), (32, 333, 1001),
+          (33, 333, 1001), (2, 7, 30)]
 LARGE = [(2600, 4096, 264), (11000, 1000, 200), (2100, 2048, 4160), (700, 5000, 136)]
 
 
@@ -248,12 +249,12 @@ def check_input(M, N, K, dtype, activation, with_scale, out_dtype, layout="plain
     s = 0.5 + torch.rand(N, device="cuda") if with_scale else None
     saved = T.pack8(1.4 * rnd(M, K)) if activation != "none" else None
     dx, a = T.linear_backward_input(dy, w, activation=activation, saved=saved, scale=s, out_dtype=DT[out_dtype], want_activation=activation != "none")
-    # with a scale the matrix cores take W * scale rounded to 16 bits: half a step of each product
+    # with a scale the matrix cores take W * scale, or (few rows) dy * scale, rounded to 16 bits: half a step of each product
     ws = w.double() * s.double()[:, None] if with_scale else w.double()
     want = dy.double() @ ws
     bound = (N + 8) * 2 * U32 * (dy.double().abs() @ ws.abs())
     if with_scale:
-        bound = bound + 1.01 * dy.double().abs() @ (half_step(t) * ws.abs() + least(t))
+        bound = bound + 1.01 * dy.double().abs() @ (half_step(t) * ws.abs() + least(t)) + least(t) * w.double().abs().sum(0)
     if activation != "none":
         u = decode(saved.codes, saved.exponents)
         f = slope(u, activation)
