@@ -19,14 +19,18 @@ __host__ __device__ inline int dt_size(int dt) { return dt == DT_FP32 ? 4 : 2; }
 // The element type is uniform over a launch: a scalar branch picks the load, and the bits are converted later, so that
 // several loads are in flight before the first conversion waits.
 struct Raw8 { u32x4v a, b; };
+// 16 bytes of any alignment that the element type has (gfx950 takes them)
+typedef unsigned int u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
-__device__ __forceinline__ Raw8 load_raw8(const void* p, int dt, size_t off) {       // 16-byte aligned
+__device__ __forceinline__ Raw8 load_raw8(const void* p, int dt, size_t off) {
   Raw8 r;
   if (dt == DT_FP32) {
-    const u32x4v* q = reinterpret_cast<const u32x4v*>(reinterpret_cast<const float*>(p) + off);
+    const u32x4_any* q = reinterpret_cast<const u32x4_any*>(reinterpret_cast<const float*>(p) + off);
     r.a = q[0]; r.b = q[1];
   } else {
-    r.a = *reinterpret_cast<const u32x4v*>(reinterpret_cast<const unsigned short*>(p) + off);
+    r.a = *reinterpret_cast<const u32x4_any*>(reinterpret_cast<const unsigned short*>(p) + off);
     r.b = u32x4v{0, 0, 0, 0};
   }
   return r;
@@ -62,10 +66,10 @@ template <int V> __device__ __forceinline__ void pack_half(const float (&y)[V], 
   else { const hv h = __builtin_convertvector(v, hv); __builtin_memcpy(to, &h, 2 * V); }
 }
 template <bool STREAM = false>
-__device__ __forceinline__ void store_vec8(void* p, int dt, size_t off, const float (&y)[8]) {   // 16-byte aligned
+__device__ __forceinline__ void store_vec8(void* p, int dt, size_t off, const float (&y)[8]) {
   if (dt == DT_FP32) {
-    f32x4* q = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + off);
-    const f32x4 a = {y[0], y[1], y[2], y[3]}, b = {y[4], y[5], y[6], y[7]};
+    f32x4_any* q = reinterpret_cast<f32x4_any*>(reinterpret_cast<float*>(p) + off);
+    const f32x4_any a = {y[0], y[1], y[2], y[3]}, b = {y[4], y[5], y[6], y[7]};
     if constexpr (STREAM) { __builtin_nontemporal_store(a, q); __builtin_nontemporal_store(b, q + 1); }
     else { q[0] = a; q[1] = b; }
   } else {
@@ -73,8 +77,8 @@ __device__ __forceinline__ void store_vec8(void* p, int dt, size_t off, const fl
     u32x4v w;
     if (dt == DT_BF16) w = __builtin_bit_cast(u32x4v, __builtin_convertvector(v, bf16x8));
     else w = __builtin_bit_cast(u32x4v, __builtin_convertvector(v, f16x8));
-    u32x4v* q = reinterpret_cast<u32x4v*>(reinterpret_cast<unsigned short*>(p) + off);
-    if constexpr (STREAM) __builtin_nontemporal_store(w, q);
+    u32x4_any* q = reinterpret_cast<u32x4_any*>(reinterpret_cast<unsigned short*>(p) + off);
+    if constexpr (STREAM) __builtin_nontemporal_store((u32x4_any)w, q);
     else *q = w;
   }
 }

@@ -186,7 +186,8 @@ template <int BM_, int BN_, int WM_, int WN_, int ST_, bool STEPS_> struct Tile 
   static constexpr int STAGE = (BM_ + BN_) * TK * 2;
 };
 
-template <class T, bool AKC, bool BKC, class TL, class Epi>
+// FAST: the result's width is a multiple of eight (Epi::fast()); the other form only in the smallest tile, whose epilogue is short
+template <class T, bool AKC, bool BKC, class TL, class Epi, bool FAST>
 __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, Epi epi) {
   constexpr int BM = TL::BM, BN = TL::BN, MI = TL::MI, NJ = TL::NJ, ST = TL::STAGES;
   constexpr int PER_STAGE = (BM + BN) / 8 / TL::NW;                   // DMA instructions a wave issues per K-tile
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
 #pragma unroll
     for (int h = 0; h < NJ / 2; ++h)
 #pragma unroll
-      for (int i = 0; i < MI; ++i) epi.template fetch<true>(mw + 16 * i, nw + 32 * h, row[h][i]);
+      for (int i = 0; i < MI; ++i) epi.template fetch<FAST>(mw + 16 * i, nw + 32 * h, row[h][i]);
   }
   // sums of A over k for the bias' gradient: products with a fragment of ones, the row fragments dealt to the WN waves
   // that share them; only the blocks of the first tile column
@@ -389,7 +390,7 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
   auto fetch_row = [&](int i) __attribute__((always_inline)) {
     if constexpr (!FETCH_AHEAD)
 #pragma unroll
-      for (int h = 0; h < NJ / 2; ++h) epi.template fetch<true>(mw + 16 * i, nw + 32 * h, row[h][i & 1]);
+      for (int h = 0; h < NJ / 2; ++h) epi.template fetch<FAST>(mw + 16 * i, nw + 32 * h, row[h][i & 1]);
   };
   fetch_row(0);
 #pragma unroll
@@ -400,7 +401,7 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
       float v[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) { v[e] = acc[i][2 * h][e]; v[4 + e] = acc[i][2 * h + 1][e]; }
-      epi.template finish<true, 16, 32>(split, mw + 16 * i, nw + 32 * h, v, col[h], row[h][FETCH_AHEAD ? i : i & 1], table);
+      epi.template finish<FAST, 16, 32>(split, mw + 16 * i, nw + 32 * h, v, col[h], row[h][FETCH_AHEAD ? i : i & 1], table);
     }
   }
 }

@@ -17,8 +17,9 @@ constexpr long long MAX_LD = 1 << 21;      // a tile's 256 rows stay inside a bu
 // ---- epilogues ---------------------------------------------------------------------------------------------------
 // finish<FAST, X1, X2>: eight columns [n, n + 8) of row m; the four lanes that hold a group of 32 are X1 and X2 apart.
 // Every lane of the wave calls it (the 8-bit group maximum crosses lanes); rows and columns past the matrix are dropped
-// here.  FAST (stores past the caches: another pass reads them, and 2 % of the launch is saved for the operands' lines): the width is a multiple of eight and every array takes 16-byte accesses (`fast()`); the main loop carries
-// only that form, sixteen times unrolled, and leaves any other result to the join kernel.
+// here.  FAST: the width is a multiple of eight (`fast()`), so no run is cut; stores go past the caches (2 % of a large
+// launch, left to the operands' lines).  The wider tiles carry only that form, up to sixteen times unrolled, and leave
+// any other result to the join kernel.
 //
 // fp32 rows: a lane's eight columns are 32 bytes, and a 16-byte access of every lane would touch half of each sector.  The
 // row swap of lane halves turns them (lane bit 5 against the half of the eight): a lane then holds columns
@@ -36,12 +37,12 @@ __device__ __forceinline__ int turned_column(int n) {                     // of 
 }
 // FAST calls come from whole waves but for lanes past the last row
 template <bool FAST, bool STREAM = true>
-__device__ __forceinline__ void store_run8(void* p, int dt, long long ld, bool vec, int m, int n, int N, float (&y)[8]) {
+__device__ __forceinline__ void store_run8(void* p, int dt, long long ld, int m, int n, int N, float (&y)[8]) {
   if (FAST && dt == DT_FP32) {
     turn8(y);
     const int c = turned_column(n);
-    f32x4* q = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + (size_t)m * ld + c);
-    const f32x4 lo = {y[0], y[1], y[2], y[3]}, hi = {y[4], y[5], y[6], y[7]};
+    f32x4_any* q = reinterpret_cast<f32x4_any*>(reinterpret_cast<float*>(p) + (size_t)m * ld + c);
+    const f32x4_any lo = {y[0], y[1], y[2], y[3]}, hi = {y[4], y[5], y[6], y[7]};
     if constexpr (STREAM) {
       if (c < N) __builtin_nontemporal_store(lo, q);
       if (c + 16 < N) __builtin_nontemporal_store(hi, q + 4);
@@ -53,7 +54,7 @@ __device__ __forceinline__ void store_run8(void* p, int dt, long long ld, bool v
   }
   if (n >= N) return;
   const size_t at = (size_t)m * ld + n;
-  if (FAST || (vec && n + 8 <= N)) store_vec8<FAST>(p, dt, at, y);
+  if (FAST || n + 8 <= N) store_vec8<FAST>(p, dt, at, y);
   else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -78,10 +79,10 @@ template <int X1, int X2> __device__ __forceinline__ unsigned max_of_four(unsign
 template <int ACT>
 struct EpiForward {                          // y = act(acc + bias) * scale + residual, codes of acc + bias
   const float* bias; const float* scale; const void* res; void* y; signed char* codes; unsigned char* bytes;
-  long long ldr, ldy; int M, N, res_dt, y_dt; bool res_vec, y_vec, code_vec;
+  long long ldr, ldy; int M, N, res_dt, y_dt;
   static constexpr int TABLE = 0;            // float2 entries of LDS the epilogue wants
   __device__ __forceinline__ void fill(float2*, int, int) const {}
-  bool fast() const { return (N & 7) == 0 && y_vec && (!res || res_vec) && (!codes || code_vec); }
+  bool fast() const { return (N & 7) == 0; }
   struct Columns { float s[8]; };
   struct Row { Raw8 r; };
   // where the sums of columns n .. n + 7 begin
@@ -101,10 +102,10 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
     if (!res || m >= M) return;
     if (FAST && res_dt == DT_FP32) {
       const int c = turned_column(n);
-      const u32x4v* q = reinterpret_cast<const u32x4v*>(reinterpret_cast<const float*>(res) + (size_t)m * ldr + c);
-      r.r.a = c < N ? q[0] : u32x4v{0, 0, 0, 0};
-      r.r.b = c + 16 < N ? q[4] : u32x4v{0, 0, 0, 0};
-    } else if ((FAST || (res_vec && n + 8 <= N)) && n < N) r.r = load_raw8(res, res_dt, (size_t)m * ldr + n);
+      const float* q = reinterpret_cast<const float*>(res) + (size_t)m * ldr + c;
+      r.r.a = c < N ? (u32x4v)*reinterpret_cast<const u32x4_any*>(q) : u32x4v{0, 0, 0, 0};
+      r.r.b = c + 16 < N ? (u32x4v)*reinterpret_cast<const u32x4_any*>(q + 16) : u32x4v{0, 0, 0, 0};
+    } else if ((FAST || n + 8 <= N) && n < N) r.r = load_raw8(res, res_dt, (size_t)m * ldr + n);
   }
   template <bool FAST, int X1, int X2>
   __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns& c, const Row& r, const float2*) const {
@@ -119,7 +120,7 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
         const unsigned byte = group_byte(top);
         const u32x2 q = pack_codes(v, byte);
         signed char* to = codes + (size_t)m * N + n;
-        if (FAST || (code_vec && n + 8 <= N)) *reinterpret_cast<u32x2*>(to) = q;
+        if (FAST || n + 8 <= N) *reinterpret_cast<u32x2_any*>(to) = q;
         else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -137,7 +138,7 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
     }
     if (res) {
       float a[8];
-      if (FAST || (res_vec && n + 8 <= N)) {
+      if (FAST || n + 8 <= N) {
         cvt_raw8(r.r, res_dt, a);
         if (FAST && res_dt == DT_FP32) turn8(a);
       } else {
@@ -147,7 +148,7 @@ struct EpiForward {                          // y = act(acc + bias) * scale + re
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += a[j];
     }
-    store_run8<FAST>(y, y_dt, ldy, y_vec, m, n, N, v);
+    store_run8<FAST>(y, y_dt, ldy, m, n, N, v);
   }
 };
 
@@ -161,7 +162,7 @@ constexpr int TABLE_STEPS = 8;
 template <int ACT>
 struct EpiInput {
   const signed char* codes; const unsigned char* bytes; void* dx; void* a; long long lddx, lda;
-  int M, N, dx_dt, a_dt; bool dx_vec, a_vec, code_vec;
+  int M, N, dx_dt, a_dt;
   static constexpr int TABLE = ACT == ACT_GELU ? TABLE_STEPS * 256 : 0;
   __device__ __forceinline__ void fill(float2* table, int tid, int threads) const {
     if constexpr (ACT == ACT_GELU)
@@ -171,7 +172,7 @@ struct EpiInput {
         table[i] = f;
       }
   }
-  bool fast() const { return (N & 7) == 0 && dx_vec && (!a || a_vec) && (!codes || code_vec); }
+  bool fast() const { return (N & 7) == 0; }
   struct Columns {};
   struct Row { u32x2 q; unsigned byte; };
   __device__ __forceinline__ void start(int, float (&b)[8]) const {
@@ -185,7 +186,7 @@ struct EpiInput {
     if constexpr (ACT != ACT_NONE) {
       if (m < M && n < N) {
         const signed char* p = codes + (size_t)m * N + n;
-        if (FAST || (code_vec && n + 8 <= N)) r.q = *reinterpret_cast<const u32x2*>(p);
+        if (FAST || n + 8 <= N) r.q = *reinterpret_cast<const u32x2_any*>(p);
         else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -220,14 +221,14 @@ struct EpiInput {
           u[j] = value;
         }
       }
-      if (a) store_run8<FAST>(a, a_dt, lda, a_vec, m, n, N, u);
+      if (a) store_run8<FAST>(a, a_dt, lda, m, n, N, u);
     }
-    store_run8<FAST>(dx, dx_dt, lddx, dx_vec, m, n, N, v);
+    store_run8<FAST>(dx, dx_dt, lddx, m, n, N, v);
   }
 };
 
 struct EpiPlain {                            // the product itself
-  void* out; long long ld; int M, N, dt; bool vec;
+  void* out; long long ld; int M, N, dt;
   static constexpr int TABLE = 0;
   __device__ __forceinline__ void fill(float2*, int, int) const {}
   struct Columns {};
@@ -241,7 +242,7 @@ struct EpiPlain {                            // the product itself
   __device__ __forceinline__ void fetch(int, int, Row&) const {}
   template <bool FAST, int X1, int X2>
   __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row&, const float2*) const {
-    if (m < M) store_run8<FAST>(out, dt, ld, vec, m, n, N, v);
+    if (m < M) store_run8<FAST>(out, dt, ld, m, n, N, v);
   }
 };
 
@@ -260,7 +261,7 @@ struct EpiPart {                             // fp32 partial sums [split][M][Np]
   __device__ __forceinline__ void fetch(int, int, Row&) const {}
   template <bool FAST, int X1, int X2>
   __device__ __forceinline__ void finish(int split, int m, int n, float (&v)[8], const Columns&, const Row&, const float2*) const {
-    if (m < M) store_run8<true, false>(part + (size_t)split * M * Np, DT_FP32, Np, true, m, n, Np, v);      // read back at once
+    if (m < M) store_run8<true, false>(part + (size_t)split * M * Np, DT_FP32, Np, m, n, Np, v);      // read back at once
   }
 };
 
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 // parts); one row, for more blocks, below.
 struct WeightFinish {
   const float* part; const float* col_sum; const float* xs; const float* xt; const float* scale; const unsigned short* W;
-  const float* bias; void* dW; float* db; float* ds; long long ldw, lddw; int N, K, Kp, splits, dt, dw_dt; bool vec;
+  const float* bias; void* dW; float* db; float* ds; long long ldw, lddw; int N, K, Kp, splits, dt, dw_dt;
 };
 template <int ROWS>
 __global__ __launch_bounds__(256) void weight_finish_kernel(WeightFinish a) {
@@ -357,7 +358,7 @@ __global__ __launch_bounds__(256) void weight_finish_kernel(WeightFinish a) {
         g[r][j] *= sc[r];
       }
       const size_t at = (size_t)row[r] * a.lddw + k;
-      if (a.vec && k + 4 <= a.K && a.dw_dt == DT_FP32) *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.dW) + at) = g[r];
+      if (k + 4 <= a.K && a.dw_dt == DT_FP32) *reinterpret_cast<f32x4_any*>(reinterpret_cast<float*>(a.dW) + at) = g[r];
       else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -439,28 +440,22 @@ constexpr float JOIN_FIXED = 5.f, JOIN_PER_BYTE = 1.f / 5.0e6f;
 
 struct Shape { int tile, tiles_m, tiles_n, splits, kt_per_split; };
 
-// `joined`: the second kernel runs whether or not the sum is split
-Shape shape_of(int M, int N, int K, bool a_along_k, bool joined) {
+// `joined`: the second kernel runs whether or not the sum is split; `ragged`: it does but for the smallest tile
+Shape shape_of(int M, int N, int K, bool a_along_k, bool joined, bool ragged) {
   const int nk = (K + TK - 1) / TK;
   Shape best{};
   float least = 0.f;
   for (int t = 0; t < TILES; ++t) {
-#ifdef FORCE
-    if (t != (FORCE == TILE_192 && !a_along_k ? TILE_256 : FORCE)) continue;
-#endif
     if (t == TILE_192 && !a_along_k) continue;
     const TileCost& c = TILE_COST[t];
     const int tm = (M + c.m - 1) / c.m, tn = (N + c.n - 1) / c.n;
     for (int want = 1; want <= 64; want += want < 4 ? 1 : want / 2) {
-#ifdef FORCE
-      if (want > 1) break;
-#endif
       if (want > 1 && nk < 2 * want) break;
       const int per = (nk + want - 1) / want, splits = (nk + per - 1) / per;            // no part is empty
       const double blocks = (double)tm * tn * splits;
       const double rounds = blocks <= c.slots ? 1.0 : (double)((long long)((blocks + c.slots - 1) / c.slots));
       float us = (float)rounds * (c.fixed + per * (blocks * 2 <= c.slots ? c.alone_k : c.per_k));
-      if (splits > 1 || joined) us += JOIN_FIXED + JOIN_PER_BYTE * 8.f * splits * (float)M * (float)N;
+      if (splits > 1 || joined || (ragged && t != TILE_64)) us += JOIN_FIXED + JOIN_PER_BYTE * 8.f * splits * (float)M * (float)N;
       if (best.splits == 0 || us < least) {
         least = us;
         best = Shape{t, tm, tn, splits, per};
@@ -502,12 +497,13 @@ int run_copies(Side& a, Side& b, int dt, char*& ws, hipStream_t st) {
   return COGAIM_LAUNCH_CHECK();
 }
 
-template <class T, bool AKC, bool BKC, class Epi>
+template <class T, bool AKC, bool BKC, bool FAST = true, class Epi>
 int launch_gemm(const Operands& g, int tile, const Epi& e, hipStream_t st) {
   const long long blocks = (long long)g.tiles_m * g.tiles_n * g.splits;
   if (blocks <= 0 || blocks >= (1LL << 31)) return COGAIM_EINVAL;
-#define TRAIN_LAUNCH(TL_) hipLaunchKernelGGL((train_gemm_kernel<T, AKC, BKC, TL_, Epi>), dim3((unsigned)blocks), dim3(TL_::NW * 64), 0, st, g, e)
-  if (tile == TILE_256) TRAIN_LAUNCH(T256);
+#define TRAIN_LAUNCH(TL_) hipLaunchKernelGGL((train_gemm_kernel<T, AKC, BKC, TL_, Epi, FAST>), dim3((unsigned)blocks), dim3(TL_::NW * 64), 0, st, g, e)
+  if constexpr (!FAST) TRAIN_LAUNCH(T64);
+  else if (tile == TILE_256) TRAIN_LAUNCH(T256);
   else if (tile == TILE_192) {
     if constexpr (AKC) TRAIN_LAUNCH(T192);
     else return COGAIM_EINVAL;
@@ -519,11 +515,11 @@ int launch_gemm(const Operands& g, int tile, const Epi& e, hipStream_t st) {
 }
 
 // the epilogue runs in a kernel of its own: parts to add, or a result that 16-byte stores cannot reach
-template <class Epi> bool joins(const Shape& s, const Epi& e) { return s.splits > 1 || !e.fast(); }
+template <class Epi> bool joins(const Shape& s, const Epi& e) { return s.splits > 1 || (!e.fast() && s.tile != TILE_64); }
 
 template <class T, bool AKC, bool BKC, class Epi>
 int product(const Operands& g, const Shape& s, const Epi& e, float* part, hipStream_t st) {
-  if (!joins(s, e)) return launch_gemm<T, AKC, BKC>(g, s.tile, e, st);
+  if (!joins(s, e)) return e.fast() ? launch_gemm<T, AKC, BKC>(g, s.tile, e, st) : launch_gemm<T, AKC, BKC, false>(g, s.tile, e, st);
   const int Np = round8(g.N);
   const int rc = launch_gemm<T, AKC, BKC>(g, s.tile, EpiPart{part, g.M, Np}, st);
   if (rc) return rc;
@@ -544,7 +540,6 @@ Operands operands(const Side& a, const Side& b, bool akc, bool bkc, int M, int N
 }
 bool half_dt(int dt) { return dt == DT_BF16 || dt == DT_FP16; }
 bool any_dt(int dt) { return dt >= 0 && dt <= 2; }
-bool vec_ok(const void* p, long long ld) { return aligned(p, 16) && (ld & 7) == 0; }
 bool matrix_ok(const void* p, long long ld, int cols, int elem) { return p && ld >= cols && ld <= MAX_LD && aligned(p, elem); }
 
 bool forward_ok(const cogaim_linear_fwd_desc* d) {
@@ -572,19 +567,14 @@ bool weight_ok(const cogaim_linear_bwd_weight_desc* d) {
 }
 }  // namespace
 
-#ifdef NOFEW
-#define few_rows(...) false
-#endif
 // the epilogues of a descriptor
 template <int ACT> EpiForward<ACT> forward_epi(const cogaim_linear_fwd_desc* d) {
   return EpiForward<ACT>{d->bias, d->scale, d->residual, d->y, (signed char*)d->codes, (unsigned char*)d->exponents, d->ldr,
-                         d->ldy, d->M, d->N, d->residual_dtype, d->y_dtype, d->residual && vec_ok(d->residual, d->ldr),
-                         vec_ok(d->y, d->ldy), (d->N & 7) == 0 && aligned(d->codes, 8)};
+                         d->ldy, d->M, d->N, d->residual_dtype, d->y_dtype};
 }
 template <int ACT> EpiInput<ACT> input_epi(const cogaim_linear_bwd_input_desc* d) {
   return EpiInput<ACT>{(const signed char*)d->codes, (const unsigned char*)d->exponents, d->dx, d->a, d->lddx, d->lda, d->M,
-                       d->K, d->dx_dtype, d->dtype, vec_ok(d->dx, d->lddx), d->a && vec_ok(d->a, d->lda),
-                       (d->K & 7) == 0 && aligned(d->codes, 8)};
+                       d->K, d->dx_dtype, d->dtype};
 }
 
 extern "C" {
@@ -592,7 +582,7 @@ extern "C" {
 long long cogaim_linear_fwd_workspace_bytes(const cogaim_linear_fwd_desc* d) {
   if (!forward_ok(d)) return COGAIM_EINVAL;
   if (few_rows(d->M, d->N, d->K, true)) return 0;
-  const Shape s = shape_of(d->M, d->N, d->K, true, !forward_epi<ACT_NONE>(d).fast());
+  const Shape s = shape_of(d->M, d->N, d->K, true, false, !forward_epi<ACT_NONE>(d).fast());
   return copy_bytes(side(d->x, d->ldx, d->M, d->K)) + copy_bytes(side(d->w, d->ldw, d->N, d->K)) +
          (joins(s, forward_epi<ACT_NONE>(d)) ? (long long)s.splits * d->M * round8(d->N) * 4 : 0);
 }
@@ -610,7 +600,7 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long lon
     return d->dtype == DT_BF16 ? FEW_RUN(__bf16, DT_BF16) : FEW_RUN(_Float16, DT_FP16);
 #undef FEW_RUN
   }
-  const Shape s = shape_of(d->M, d->N, d->K, true, !forward_epi<ACT_NONE>(d).fast());
+  const Shape s = shape_of(d->M, d->N, d->K, true, false, !forward_epi<ACT_NONE>(d).fast());
   Side a = side(d->x, d->ldx, d->M, d->K), b = side(d->w, d->ldw, d->N, d->K);
   char* ws = (char*)workspace;
   const int rc = run_copies(a, b, d->dtype, ws, st);
@@ -626,7 +616,7 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long lon
 long long cogaim_linear_bwd_input_workspace_bytes(const cogaim_linear_bwd_input_desc* d) {
   if (!input_ok(d)) return COGAIM_EINVAL;
   if (few_rows(d->M, d->K, d->N, false)) return 0;
-  const Shape s = shape_of(d->M, d->K, d->N, true, !input_epi<ACT_NONE>(d).fast());
+  const Shape s = shape_of(d->M, d->K, d->N, true, false, !input_epi<ACT_NONE>(d).fast());
   return copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + copy_bytes(side(d->w, d->ldw, d->N, d->K, d->scale)) +
          (joins(s, input_epi<ACT_NONE>(d)) ? (long long)s.splits * d->M * round8(d->K) * 4 : 0);
 }
@@ -644,7 +634,7 @@ int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspa
     return d->dtype == DT_BF16 ? FEW_RUN(__bf16, DT_BF16) : FEW_RUN(_Float16, DT_FP16);
 #undef FEW_RUN
   }
-  const Shape s = shape_of(d->M, d->K, d->N, true, !input_epi<ACT_NONE>(d).fast());
+  const Shape s = shape_of(d->M, d->K, d->N, true, false, !input_epi<ACT_NONE>(d).fast());
   Side a = side(d->dy, d->lddy, d->M, d->N), b = side(d->w, d->ldw, d->N, d->K, d->scale);
   char* ws = (char*)workspace;
   const int rc = run_copies(a, b, d->dtype, ws, st);
@@ -657,15 +647,15 @@ int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspa
   return d->dtype == DT_BF16 ? IN_RUN(__bf16) : IN_RUN(_Float16);
 }
 
-// something to put on the finished sums, or a result that 16-byte stores cannot reach: the row-wise second kernel runs
+// something to put on the finished sums, or a ragged result: the row-wise second kernel runs
 static bool weight_has_more(const cogaim_linear_bwd_weight_desc* d) {
-  return d->x_scale || d->x_shift || d->scale || (d->K & 7) || !vec_ok(d->dw, d->lddw);
+  return d->x_scale || d->x_shift || d->scale || (d->K & 7);
 }
 static bool weight_needs_finish(const cogaim_linear_bwd_weight_desc* d, const Shape& s) { return s.splits > 1 || weight_has_more(d); }
 
 long long cogaim_linear_bwd_weight_workspace_bytes(const cogaim_linear_bwd_weight_desc* d) {
   if (!weight_ok(d)) return COGAIM_EINVAL;
-  const Shape s = shape_of(d->N, d->K, d->M, false, weight_has_more(d));
+  const Shape s = shape_of(d->N, d->K, d->M, false, weight_has_more(d), false);
   const long long x = d->codes ? round256((long long)d->M * round8(d->K) * 2) : copy_bytes(side(d->x, d->ldx, d->M, d->K));
   const long long part = weight_needs_finish(d, s) ? round256((long long)s.splits * d->N * round8(d->K) * 4) + (long long)s.splits * d->N * 4 : 0;
   return copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + x + part;
@@ -675,7 +665,7 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
   const long long need = cogaim_linear_bwd_weight_workspace_bytes(d);
   if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  const Shape s = shape_of(d->N, d->K, d->M, false, weight_has_more(d));
+  const Shape s = shape_of(d->N, d->K, d->M, false, weight_has_more(d), false);
   char* ws = (char*)workspace;
   Side a = side(d->dy, d->lddy, d->M, d->N), b{};
   if (!d->codes) b = side(d->x, d->ldx, d->M, d->K);
@@ -692,7 +682,7 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
   Operands g = operands(a, b, false, false, d->N, d->K, s);
   if (!weight_needs_finish(d, s)) {
     g.col_sum = d->db;
-    const EpiPlain e{d->dw, d->lddw, d->N, d->K, d->dw_dtype, true};
+    const EpiPlain e{d->dw, d->lddw, d->N, d->K, d->dw_dtype};
     return d->dtype == DT_BF16 ? launch_gemm<__bf16, false, false>(g, s.tile, e, st) : launch_gemm<_Float16, false, false>(g, s.tile, e, st);
   }
   const int kp = round8(d->K);
@@ -703,7 +693,7 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
   rc = d->dtype == DT_BF16 ? launch_gemm<__bf16, false, false>(g, s.tile, e, st) : launch_gemm<_Float16, false, false>(g, s.tile, e, st);
   if (rc) return rc;
   const WeightFinish f{part, sums, d->x_scale, d->x_shift, d->scale, (const unsigned short*)d->w, d->bias, d->dw, d->db, d->ds, d->ldw, d->lddw,
-                       d->N, d->K, kp, s.splits, d->dtype, d->dw_dtype, vec_ok(d->dw, d->lddw)};
+                       d->N, d->K, kp, s.splits, d->dtype, d->dw_dtype};
   if (d->N >= 4 * 512) hipLaunchKernelGGL(weight_finish_kernel<4>, dim3((d->N + 3) / 4), dim3(256), 0, st, f);
   else hipLaunchKernelGGL(weight_finish_kernel<1>, dim3(d->N), dim3(256), 0, st, f);
   return COGAIM_LAUNCH_CHECK();

@@ -188,8 +188,8 @@ def test_layer_norm_non_finite_rows_stay_in_their_row():
 # ---- linear layers -----------------------------------------------------------------------------------------------
 SHAPES = [(1, 1, 1), (1, 8, 8), (5, 64, 64), (3, 577, 588), (65, 129, 72), (130, 256, 768), (64, 200, 8), (257, 1000, 264),
           (31, 24, 4096), (1000, 96, 100), (9, 2048, 1024), (300, 1544, 520), (16, 2052, 1000), (17, 100, 72), (32, 333, 1001),
-          (33, 333, 1001), (2, 7, 30)]
-LARGE = [(2600, 4096, 264), (11000, 1000, 200), (2100, 2048, 4160), (700, 5000, 136)]
+          (33, 333, 1001), (2, 7, 30), (40, 333, 5001)]
+LARGE = [(2600, 4096, 264), (11000, 1000, 200), (2100, 2048, 4160), (700, 5000, 136), (20000, 520, 264), (2600, 264, 4096)]
 
 
 def product_bound(A, B, K):
@@ -355,7 +355,7 @@ def test_linear_backward_weight(M, N, K, dtype, kept, affine, scale, out):
     check_weight(M, N, K, dtype, kept, affine, scale, out)
 
 
-@pytest.mark.parametrize("M,N,K", [(264, 2600, 4096), (200, 11000, 1000), (4160, 2100, 2048), (136, 700, 5000), (20000, 520, 264)])
+@pytest.mark.parametrize("M,N,K", [(264, 2600, 4096), (200, 11000, 1000), (4160, 2100, 2048), (136, 700, 5000), (20000, 520, 264), (11000, 1000, 200)])
 def test_linear_backward_weight_large(M, N, K):
     check_weight(M, N, K, "bf16", False, False, False)
     check_weight(M, N, K, "fp16", True, True, True)
