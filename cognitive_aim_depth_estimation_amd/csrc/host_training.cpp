@@ -13,7 +13,7 @@ using at::Tensor;
 using OptTensor = std::optional<Tensor>;
 using OptType = std::optional<at::ScalarType>;
 
-constexpr int64_t GROUP = 32, MAX_NORM_WIDTH = 16384, MAX_LEADING_DIM = 1 << 21, MAX_ROWS = 0x7fffffff;
+constexpr int64_t GROUP = 32, MAX_NORM_WIDTH = 16384, MAX_LEADING_DIM = 1 << 21, MAX_ROWS = 0x7fffffff - 511, MAX_WIDTH = 1 << 30;
 enum { ACT_NONE, ACT_RELU, ACT_GELU };
 
 #define ENTRIES(X)                                                                                                        \
@@ -103,7 +103,7 @@ struct Rows { Tensor keep; void* p; int64_t ld; int n; };
 Rows rows(const Tensor& t) {
   const int64_t D = t.size(-1);
   auto take = [&](const Tensor& u, int64_t n, int64_t ld) {
-    TORCH_CHECK_VALUE(n <= MAX_ROWS, "more than 2^31 - 1 rows");
+    TORCH_CHECK_VALUE(n <= MAX_ROWS, "more rows than the kernels count");
     return Rows{u, u.data_ptr(), ld, (int)n};
   };
   if (t.is_contiguous()) return take(t, t.numel() / D, D);
@@ -118,7 +118,7 @@ int64_t leading(int64_t ld, const char* name) {
   return ld;
 }
 int narrow(int64_t n, const char* name) {
-  TORCH_CHECK_VALUE(n <= MAX_ROWS, name, " is wider than 2^31 - 1");
+  TORCH_CHECK_VALUE(n <= MAX_WIDTH, name, " is wider than ", MAX_WIDTH);
   return (int)n;
 }
 
@@ -159,7 +159,7 @@ Tensor unpack8(const Tensor& codes, const Tensor& exponents, at::ScalarType dtyp
   const On on(codes.device());
   const Tensor out = fresh(codes, codes.sizes(), t);
   const int64_t M = codes.numel() / D;
-  TORCH_CHECK_VALUE(M <= MAX_ROWS, "more than 2^31 - 1 rows");
+  TORCH_CHECK_VALUE(M <= MAX_ROWS, "more rows than the kernels count");
   if (M)
     check(cogaim_unpack8_(s.codes.data_ptr(), s.exponents.data_ptr(), out.data_ptr(), code(t), D, (int)M, D, D, on.stream), "cogaim_unpack8");
   return out;

@@ -277,7 +277,7 @@ __global__ __launch_bounds__(TL::NW * 64, 2) void train_gemm_kernel(Operands g, 
   if constexpr (TL::STEPS) {
     // Two stages.  A K-tile is eight steps of 8 MFMAs, a quarter of the wave's tile at one k32 half each, ordered so that
     // a step changes one operand; the fragments of a step are read between the MFMAs of the one before it, and the
-    // eight DMA pieces that a wave owes the K-tile after the next go out one per step, in the order in which the stage's
+    // six to eight DMA pieces that a wave owes the K-tile after the next go out one per step, in the order in which the stage's
     // halves fall free: the first half behind the barrier in mid-tile, the second behind the one at its end.
     static_assert(NJ == 4 && ST == 2 && MI % 2 == 0, "written for strips of 64 columns");
     constexpr int MH = MI / 2, PA = decltype(sa)::PIECES, EA = decltype(sa)::EARLY, LATE = PA - EA;

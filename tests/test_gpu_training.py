@@ -595,6 +595,34 @@ def test_transposed_and_broadcast_inputs():
     assert torch.equal(dx, same[0]) and torch.equal(dw, same[1]) and torch.equal(db, same[2])
 
 
+def test_offsets_past_32_bits():
+    """Matrices of more than 2^31 elements: their last rows against the same rows alone."""
+    M, D = 600_000, 4096
+    x = torch.empty(M, D, device="cuda", dtype=torch.bfloat16)
+    x[-70:] = rnd(70, D, dtype=torch.bfloat16)
+    x[:-70] = 1.0
+    last = x[-70:].clone()
+    p, q = T.pack8(x), T.pack8(last)
+    assert torch.equal(p.codes[-70:], q.codes) and torch.equal(p.exponents[-70:], q.exponents)
+    assert torch.equal(T.unpack8(p, torch.bfloat16)[-70:], T.unpack8(q, torch.bfloat16))
+    g, b = 1 + 0.1 * rnd(D), rnd(D)
+    y, mean, rstd, _ = T.layer_norm_forward(x, g, b)
+    y2, mean2, rstd2, _ = T.layer_norm_forward(last, g, b)
+    assert torch.equal(y[-70:], y2) and torch.equal(mean[-70:], mean2) and torch.equal(rstd[-70:], rstd2)
+    dx = T.layer_norm_backward(x, p, None, rstd, g)[0]
+    assert torch.equal(dx[-70:], T.layer_norm_backward(last, q, None, rstd2, g)[0])
+    del y, dx
+    w = rnd(64, D, dtype=torch.bfloat16, scale=D ** -0.5)
+    z, s = T.linear_forward(x, w, activation="gelu", checkpoint=True)              # offsets of the operand
+    dx, a = T.linear_backward_input(z, w, "gelu", p, want_activation=True)           # of the results and of the codes
+    u = last.double() @ w.double().t()
+    within(z[-70:], act(u, "gelu"), 1.13 * product_bound(last, w, D) + 2e-7 + 6 * U32 * u.abs() + half_step(z.dtype) * (1.01 * u.abs() + 1e-6))
+    v = decode(q.codes, q.exponents)
+    G, f = z[-70:].double() @ w.double(), slope(v, "gelu")
+    within(dx[-70:], G * f, 80 * 2 * U32 * (z[-70:].double().abs() @ w.double().abs()) * f.abs() + G.abs() * 4e-7 + 1.01 * half_step(dx.dtype) * (G * f).abs())
+    within(a[-70:], act(v, "gelu"), 2e-7 + 1.01 * half_step(a.dtype) * act(v, "gelu").abs())
+
+
 def step_functions(p, dy):
     x, g, b, w1, b1, w2, b2, s = [v.detach() for v in p]
     v1, v2 = w1.bfloat16(), w2.bfloat16()

@@ -104,6 +104,7 @@ def test_entry_points_refuse():
     assert raw("cogaim_pack8", P + 1, 0, 8, P, P, 1, 8, None) == bad
     assert raw("cogaim_pack8", P, 0, 8, P, None, 1, 8, None) == bad
     assert raw("cogaim_pack8", P, 0, 8, P, P, 0, 8, None) == bad
+    assert raw("cogaim_pack8", P, 0, 1 << 31, P, P, 1, (1 << 30) + 1, None) == bad
     assert raw("cogaim_unpack8", P, P, P, 0, 8, 1, 8, 7, None) == bad
     assert raw("cogaim_unpack8", P, P, P, 0, 7, 1, 8, 8, None) == bad
     assert raw("cogaim_activation_bwd", P, 0, 8, P, P, P, 0, 8, 0, 1, 8, None) == bad
@@ -123,12 +124,14 @@ def test_descriptors_refuse():
         a.update(k)
         return raw("cogaim_linear_fwd_workspace_bytes", C.byref(_lib.LinearFwdDesc(**a)))
     assert fwd() >= 0
-    for k in (dict(x=None), dict(M=0), dict(N=-1), dict(K=0), dict(dtype=2), dict(y_dtype=3), dict(ldx=63), dict(ldw=1 << 22), dict(ldy=31),
+    for k in (dict(x=None), dict(M=0), dict(M=0x7fffffff), dict(N=-1), dict(K=0), dict(dtype=2), dict(y_dtype=3), dict(ldx=63), dict(ldw=1 << 22), dict(ldy=31),
               dict(activation=3), dict(activation=2, scale=P), dict(codes=P), dict(residual=P, ldr=31), dict(residual=P, ldr=32, residual_dtype=5),
               dict(x=P + 1)):
         assert fwd(**k) == -22, k
     assert raw("cogaim_linear_fwd_workspace_bytes", None) == -22
     d = _lib.LinearFwdDesc(x=P, w=P, y=P, ldx=61, ldw=64, ldy=32, M=4, N=32, K=61, dtype=0)
+    assert raw("cogaim_linear_fwd_workspace_bytes", C.byref(d)) == 0    # few rows are read where they lie
+    d.M = 64
     need = raw("cogaim_linear_fwd_workspace_bytes", C.byref(d))
     assert need > 0                                                     # rows that 16-byte loads cannot address are copied
     assert raw("cogaim_linear_fwd", C.byref(d), P, need - 1, None) == -22 and raw("cogaim_linear_fwd", C.byref(d), None, need, None) == -22
