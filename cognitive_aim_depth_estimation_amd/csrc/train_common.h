@@ -94,6 +94,31 @@ __device__ __forceinline__ void store_one(void* p, int dt, size_t off, float y) 
 
 // Sum over the 64 lanes, result in every lane, without the LDS permute path: rotations inside rows of 16 lanes (DPP), then
 // the two row-swap instructions of gfx950.
+// An operand times a vector of scales, rounded to fp16: a LayerScale of 1e-5 would push it into fp16's subnormals (0.02 times
+// that keeps two bits).  So the scales are multiplied by a power of two that brings the largest into [0.5, 1), and the
+// sums by its reciprocal, both exact.  `top`: the largest magnitude's bits; infinities, NaN and all zeros: no change.
+__device__ __forceinline__ void scale_units(unsigned top, float& up, float& down) {
+  const unsigned e = top >> 23;
+  up = down = 1.f;
+  if (top == 0 || e == 255) return;
+  const unsigned c = e < 252 ? e : 252;
+  up = __uint_as_float((253 - c) << 23);
+  down = __uint_as_float((c + 1) << 23);
+}
+__device__ __forceinline__ unsigned wave_top(const float* s, int n, int from, int by) {      // largest magnitude's bits
+  unsigned top = 0;
+#pragma unroll 4
+  for (int i = from; i < n; i += by) {
+    const unsigned b = __float_as_uint(s[i]) & 0x7fffffffu;
+    top = b > top ? b : top;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const unsigned o = (unsigned)__shfl_xor((int)top, d);
+    top = o > top ? o : top;
+  }
+  return top;
+}
 __device__ __forceinline__ float wave_sum_dpp(float v) {
 #define TRAIN_ROR(ctrl_) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl_, 0xf, 0xf, false))
   v += TRAIN_ROR(0x128);   // row_ror:8

@@ -49,6 +49,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void train_few_kernel(Few g, Epi ep
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float up = 1.f, down = 1.f;
+  if (DT == DT_FP16 && g.scale) scale_units(wave_top(g.scale, g.K, lane, 64), up, down);
   auto four = [&](u32x2 w) __attribute__((always_inline)) {
     if (shift == 0) return w;
     const unsigned long long x = ((unsigned long long)w[1] << 32) | w[0];
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void train_few_kernel(Few g, Epi ep
     if (g.scale) {
       float s[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = g.scale[k + j < limit ? k + j : limit - 1];
+      for (int j = 0; j < 8; ++j) s[j] = g.scale[k + j < limit ? k + j : limit - 1] * up;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         float v[8];
@@ -134,6 +136,12 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void train_few_kernel(Few g, Epi ep
       }
     }
     multiply(af, bf, raw, k, g.K);
+  }
+  if (DT == DT_FP16 && g.scale) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) acc[i][j] *= down;
   }
   // element e of a lane is column 16 j + 4 q + e (forward), 4 (4 q + e) + j (input gradient) of row 16 i + fr
 #pragma unroll

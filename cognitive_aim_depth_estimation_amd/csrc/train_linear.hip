@@ -165,6 +165,7 @@ template <int ACT>
 struct EpiInput {
   const signed char* codes; const unsigned char* bytes; void* dx; void* a; long long lddx, lda;
   int M, N, dx_dt, a_dt;
+  const float* unit;                           // what the sums are multiplied by (see scale_units), or null
   static constexpr int TABLE = ACT == ACT_GELU ? TABLE_STEPS * 256 : 0;
   __device__ __forceinline__ void fill(float2* table, int tid, int threads) const {
     if constexpr (ACT == ACT_GELU)
@@ -201,6 +202,11 @@ struct EpiInput {
   template <bool FAST, int X1, int X2>
   __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row& r, const float2* table) const {
     if (m >= M) return;                          // lanes of one row leave together
+    if (unit) {
+      const float f = *unit;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= f;
+    }
     if constexpr (ACT != ACT_NONE) {
       float u[8];
       const bool listed = ACT == ACT_GELU && FAST && (n >= N || r.byte - TABLE_FIRST < (unsigned)TABLE_STEPS);
@@ -387,14 +393,26 @@ __global__ __launch_bounds__(256) void weight_finish_kernel(WeightFinish a) {
 }
 
 // Copies of operands whose rows the DMA's 16-byte loads cannot address (odd widths, strides or bases), padded with zeros to
-// a multiple of eight columns; with `scale`, row r times scale[r] (rounded once to 16 bits: the matrix cores take it so).
+// a multiple of eight columns; with `scale`, row r times scale[r] (rounded once to 16 bits: the matrix cores take it so), in
+// fp16 times scale[r] * up, and *unit = down.
 // Both operands of a product in one launch: blocks [0, blocks0) copy the first.
-struct CopyOne { const unsigned short* src; unsigned short* dst; const float* scale; long long ld; int rows, cols, padded; };
+struct CopyOne { const unsigned short* src; unsigned short* dst; const float* scale; float* unit; long long ld; int rows, cols, padded; };
 struct CopyTwo { CopyOne one[2]; unsigned blocks0; int dt; };
 __global__ __launch_bounds__(256) void copy_rows_kernel(CopyTwo a) {
   const bool second = blockIdx.x >= a.blocks0;
   const CopyOne& c = a.one[second];
   const unsigned block = second ? blockIdx.x - a.blocks0 : blockIdx.x, blocks = second ? gridDim.x - a.blocks0 : a.blocks0;
+  float up = 1.f;
+  if (c.unit) {                                                           // uniform over the block
+    __shared__ unsigned tops[4];
+    const unsigned mine = wave_top(c.scale, c.rows, threadIdx.x, 256);
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    const unsigned t0 = tops[0] > tops[1] ? tops[0] : tops[1], t1 = tops[2] > tops[3] ? tops[2] : tops[3];
+    float down;
+    scale_units(t0 > t1 ? t0 : t1, up, down);
+    if (block == 0 && threadIdx.x == 0) *c.unit = down;
+  }
   const unsigned runs = (unsigned)c.padded / 8;
   const unsigned long long total = (unsigned long long)c.rows * runs;
   for (unsigned long long i = block * 256ULL + threadIdx.x; i < total; i += 256ULL * blocks) {
@@ -408,7 +426,7 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(CopyTwo a) {
       for (int j = 0; j < 4; ++j) w[j] = (k0 + 2 * j < c.cols ? (unsigned)src[2 * j] : 0u) | (k0 + 2 * j + 1 < c.cols ? (unsigned)src[2 * j + 1] << 16 : 0u);
     }
     if (c.scale) {
-      const float s = c.scale[r];
+      const float s = c.scale[r] * up;
       float v[8];
       cvt_raw8(Raw8{w, w}, a.dt, v);
 #pragma unroll
@@ -471,9 +489,9 @@ long long round256(long long v) { return (v + 255) / 256 * 256; }
 int round8(int v) { return (v + 7) & ~7; }
 
 // an operand as the main loop takes it: `copy` when 16-byte loads cannot address it
-struct Side { const void* p; long long ld; int rows, cols; bool copy; const float* scale; };
+struct Side { const void* p; long long ld; int rows, cols; bool copy; const float* scale; float* unit; };
 Side side(const void* p, long long ld, int rows, int cols, const float* scale = nullptr) {
-  Side s{p, ld, rows, cols, scale || (cols & 7) || (ld & 7) || !aligned(p, 16), scale};
+  Side s{p, ld, rows, cols, scale || (cols & 7) || (ld & 7) || !aligned(p, 16), scale, nullptr};
   return s;
 }
 long long copy_bytes(const Side& s) { return s.copy ? round256((long long)s.rows * round8(s.cols) * 2) : 0; }
@@ -487,7 +505,7 @@ int run_copies(Side& a, Side& b, int dt, char*& ws, hipStream_t st) {
   for (Side* s : {&a, &b}) {
     if (!s->copy) continue;
     const int c8 = round8(s->cols);
-    c.one[n] = CopyOne{(const unsigned short*)s->p, (unsigned short*)ws, s->scale, s->ld, s->rows, s->cols, c8};
+    c.one[n] = CopyOne{(const unsigned short*)s->p, (unsigned short*)ws, s->scale, s->unit, s->ld, s->rows, s->cols, c8};
     const unsigned long long want = ((unsigned long long)s->rows * (c8 / 8) + 255) / 256;
     blocks[n++] = (unsigned)(want > 256 * 16 ? 256 * 16 : want);
     s->p = ws; s->ld = c8; s->cols = c8;
@@ -574,9 +592,9 @@ template <int ACT> EpiForward<ACT> forward_epi(const cogaim_linear_fwd_desc* d) 
   return EpiForward<ACT>{d->bias, d->scale, d->residual, d->y, (signed char*)d->codes, (unsigned char*)d->exponents, d->ldr,
                          d->ldy, d->M, d->N, d->residual_dtype, d->y_dtype};
 }
-template <int ACT> EpiInput<ACT> input_epi(const cogaim_linear_bwd_input_desc* d) {
+template <int ACT> EpiInput<ACT> input_epi(const cogaim_linear_bwd_input_desc* d, const float* unit = nullptr) {
   return EpiInput<ACT>{(const signed char*)d->codes, (const unsigned char*)d->exponents, d->dx, d->a, d->lddx, d->lda, d->M,
-                       d->K, d->dx_dtype, d->dtype};
+                       d->K, d->dx_dtype, d->dtype, unit};
 }
 
 extern "C" {
@@ -615,11 +633,13 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long lon
   return d->dtype == DT_BF16 ? FWD_RUN(__bf16) : FWD_RUN(_Float16);
 }
 
+static bool input_unit(const cogaim_linear_bwd_input_desc* d) { return d->scale && d->dtype == DT_FP16; }
+
 long long cogaim_linear_bwd_input_workspace_bytes(const cogaim_linear_bwd_input_desc* d) {
   if (!input_ok(d)) return COGAIM_EINVAL;
   if (few_rows(d->M, d->K, d->N, false)) return 0;
   const Shape s = shape_of(d->M, d->K, d->N, true, false, !input_epi<ACT_NONE>(d).fast());
-  return copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + copy_bytes(side(d->w, d->ldw, d->N, d->K, d->scale)) +
+  return (input_unit(d) ? 256 : 0) + copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + copy_bytes(side(d->w, d->ldw, d->N, d->K, d->scale)) +
          (joins(s, input_epi<ACT_NONE>(d)) ? (long long)s.splits * d->M * round8(d->K) * 4 : 0);
 }
 
@@ -639,13 +659,18 @@ int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspa
   const Shape s = shape_of(d->M, d->K, d->N, true, false, !input_epi<ACT_NONE>(d).fast());
   Side a = side(d->dy, d->lddy, d->M, d->N), b = side(d->w, d->ldw, d->N, d->K, d->scale);
   char* ws = (char*)workspace;
+  if (input_unit(d)) {
+    b.unit = (float*)ws;
+    ws += 256;
+  }
+  const float* const unit = b.unit;
   const int rc = run_copies(a, b, d->dtype, ws, st);
   if (rc) return rc;
   const Operands g = operands(a, b, true, false, d->M, d->K, s);
 #define IN_RUN(T_)                                                                                                     \
-  (d->activation == ACT_RELU ? product<T_, true, false>(g, s, input_epi<ACT_RELU>(d), (float*)ws, st)                         \
-   : d->activation == ACT_GELU ? product<T_, true, false>(g, s, input_epi<ACT_GELU>(d), (float*)ws, st)                       \
-                               : product<T_, true, false>(g, s, input_epi<ACT_NONE>(d), (float*)ws, st))
+  (d->activation == ACT_RELU ? product<T_, true, false>(g, s, input_epi<ACT_RELU>(d, unit), (float*)ws, st)                         \
+   : d->activation == ACT_GELU ? product<T_, true, false>(g, s, input_epi<ACT_GELU>(d, unit), (float*)ws, st)                       \
+                               : product<T_, true, false>(g, s, input_epi<ACT_NONE>(d, unit), (float*)ws, st))
   return d->dtype == DT_BF16 ? IN_RUN(__bf16) : IN_RUN(_Float16);
 }
 
@@ -677,7 +702,7 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
     // the 8-bit rows as 16-bit values in front of the product (a power-of-two step makes them exact in bf16)
     const int k8 = round8(d->K);
     rc = cogaim_unpack8(d->codes, d->exponents, ws, d->dtype, k8, d->M, d->K, k8, stream);
-    b = Side{ws, k8, d->M, k8, false, nullptr};
+    b = Side{ws, k8, d->M, k8, false, nullptr, nullptr};
     ws += round256((long long)d->M * k8 * 2);
     if (rc) return rc;
   }

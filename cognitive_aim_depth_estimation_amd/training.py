@@ -131,7 +131,8 @@ def linear_backward_input(dy: Tensor, weight: Tensor, activation: str = "none", 
     """``(dx, a)`` for ``dy [..., N]`` and ``weight [N, K]`` of one 16-bit type:  ``dx = ((dy * scale) weight) * act'(u)``,
     ``u [..., K]`` the pre-activation, kept in 8 bits (``saved``), of the activation that produced the layer's input; with
     ``want_activation``, ``a = act(u)`` in 16 bits: that input again, for ``linear_backward_weight``.  With ``scale``,
-    ``weight * scale`` (``dy * scale`` up to 32 rows) is rounded to 16 bits."""
+    ``weight * scale`` (``dy * scale`` up to 32 rows) is rounded to 16 bits, in fp16 relative to the largest scale: a
+    LayerScale of 1e-5 loses nothing to subnormals."""
     codes, exponents = (None, None) if saved is None else _checkpoint(saved, "saved")
     return (_host or _ops()).linear_backward_input(dy, weight, activation, codes, exponents, scale, out_dtype, want_activation)
 

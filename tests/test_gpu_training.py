@@ -274,6 +274,37 @@ def test_linear_backward_input(M, N, K, dtype, activation, scale, out):
     check_input(M, N, K, dtype, activation, scale, out)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 64, 40), (20, 333, 72), (150, 520, 264), (70, 33, 41), (300, 4096, 128)])
+@pytest.mark.parametrize("size", [1e-5, 1.0, 3e4, 1e-30])
+def test_linear_backward_input_fp16_scales(M, N, K, size):
+    """fp16 with scales far from one.  Scale times an operand is rounded with the largest scale brought into [0.5, 1): by half
+    a step of the product, or half of fp16's least number in units of at most twice the largest scale."""
+    t = torch.float16
+    dy, w = rnd(M, N, dtype=t, scale=0.1), rnd(N, K, dtype=t, scale=N ** -0.5)
+    s = size * (0.5 + torch.rand(N, device="cuda"))
+    dx, _ = T.linear_backward_input(dy, w, scale=s, out_dtype=torch.float32)
+    ws, top = w.double() * s.double()[:, None], float(s.max())
+    want, wide = dy.double() @ ws, dy.double().abs() @ ws.abs()
+    bound = (N + 8) * 2 * U32 * wide + 1.01 * half_step(t) * wide
+    bound = bound + 2.0 ** -24 * top * (dy.double().abs().sum(1, keepdim=True) + w.double().abs().sum(0)) + least(torch.float32)
+    within(dx, want, bound + U32 * want.abs(), "dx")
+
+
+@pytest.mark.parametrize("scales", ["zeros", "inf", "nan"])
+@pytest.mark.parametrize("M", [3, 80])
+def test_linear_backward_input_fp16_special_scales(M, scales):
+    N, K = 64, 72
+    dy, w = rnd(M, N, dtype=torch.float16), rnd(N, K, dtype=torch.float16)
+    s = torch.zeros(N, device="cuda")
+    if scales != "zeros":
+        s[5] = float(scales)
+    dx, _ = T.linear_backward_input(dy, w, scale=s, out_dtype=torch.float32)
+    want = dy.double() @ (w.double() * s.double()[:, None])
+    assert torch.equal(torch.isfinite(dx), torch.isfinite(want))
+    if scales == "zeros":
+        assert int(dx.count_nonzero()) == 0
+
+
 @pytest.mark.parametrize("M,K,N", LARGE)
 def test_linear_backward_input_large(M, K, N):
     check_input(M, N, K, "bf16", "gelu", False, "bf16")
@@ -621,6 +652,16 @@ def test_offsets_past_32_bits():
     G, f = z[-70:].double() @ w.double(), slope(v, "gelu")
     within(dx[-70:], G * f, 80 * 2 * U32 * (z[-70:].double().abs() @ w.double().abs()) * f.abs() + G.abs() * 4e-7 + 1.01 * half_step(dx.dtype) * (G * f).abs())
     within(a[-70:], act(v, "gelu"), 2e-7 + 1.01 * half_step(a.dtype) * act(v, "gelu").abs())
+    del dx, a
+    # the weight's gradient walks down the rows: only the last 70 have a gradient, so it is theirs alone
+    dy = torch.zeros(M, 64, device="cuda", dtype=torch.bfloat16)
+    dy[-70:] = z[-70:]
+    want, wide = dy[-70:].double().t() @ last.double(), dy[-70:].double().abs().t() @ last.double().abs()
+    dw, db, _ = T.linear_backward_weight(dy, x)
+    within(dw, want, 80 * 2 * U32 * wide)
+    within(db, dy[-70:].double().sum(0), 80 * 2 * U32 * dy[-70:].double().abs().sum(0))
+    dw = T.linear_backward_weight(dy, p)[0]
+    within(dw, dy[-70:].double().t() @ v, 80 * 2 * U32 * (dy[-70:].double().abs().t() @ v.abs()))
 
 
 def step_functions(p, dy):
