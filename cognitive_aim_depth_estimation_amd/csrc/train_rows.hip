@@ -4,14 +4,19 @@
 #include "train_common.h"
 #include "../../include/cogaim.h"
 
+#include <type_traits>
+
 namespace {
 using namespace train;
 
 // A row lives in the registers of TPR threads, NCH runs of V consecutive columns each (runs t, t + TPR, ...; 32 / V
 // neighbouring threads hold a group of 32).  Rows may begin at any element: runs are moved with accesses of whatever
 // alignment the row has (gfx950 takes them).
-// EVEN: the width is a multiple of the run, and no run crosses a row's end; otherwise that one is moved element by
-// element, which costs a branch around every access (and the batching of loads across it: 33 -> 24 us at 21920 x 1024).
+// EVEN: the width is a multiple of the run, and no run crosses a row's end.  Otherwise one does, by at most V - 1 elements:
+// with V rows or more behind this one, these lie in the matrix too, so the run is loaded whole and the columns past the end
+// are zeroed where they are used; only the last V rows' runs are loaded element by element.  (With a branch around every
+// load they are no longer in flight together: fp32 43840 x 767 to bf16 and 8 bits 66 us, now 40, where 768 columns take 36;
+// backward from 8 bits 52, now 41, against 35.)
 template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
   v = wave_sum_dpp(v);
   if constexpr (TPR > 64) {
@@ -79,24 +84,44 @@ template <int V, bool EVEN> __device__ __forceinline__ Run<DT_FP32, V> load_any(
   for (int j = 0; j < V; ++j) o.w[j] = j < V / 2 ? r.w[j] : 0u;
   return o;
 }
+// the first n < V elements of a run: of eight in pieces of four, two and one, of four one by one (the backward kernel has no
+// registers for more: 43840 x 767 from fp32 74 against 72 us)
+template <int V, class E> __device__ __forceinline__ void store_end(E* q, const E (&y)[V], int n) {
+  if constexpr (V == 4) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) if (j < n) q[j] = y[j];
+    return;
+  }
+  E v[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = y[j];
+#pragma unroll
+  for (int p = V / 2; p; p /= 2)
+    if (n & p) {
+      __builtin_memcpy(q, v, p * sizeof(E));
+      q += p;
+#pragma unroll
+      for (int j = 0; j + p < V; ++j) v[j] = v[j + p];
+    }
+}
 template <int V, bool EVEN> __device__ __forceinline__ void store_any(void* p, int dt, long long row, int c, int D, const float (&y)[V]) {
   if (dt == DT_FP32) {
     float* q = reinterpret_cast<float*>(p) + row + c;
     if (EVEN || c + V <= D) __builtin_memcpy(q, y, 4 * V);
-    else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) if (c + j < D) q[j] = y[j];
-    }
+    else store_end<V>(q, y, D - c);
   } else {
     unsigned short* q = reinterpret_cast<unsigned short*>(p) + row + c;
     unsigned short h[V];
     pack_half<V>(y, dt, h);
     if (EVEN || c + V <= D) __builtin_memcpy(q, h, 2 * V);
-    else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) if (c + j < D) q[j] = h[j];
-    }
+    else store_end<V>(q, h, D - c);
   }
+}
+// whether runs of row `row` may reach into the rows behind it (the same for the wave)
+template <int V> __device__ __forceinline__ bool runs_whole(long long row, int M) { return __builtin_amdgcn_readfirstlane((int)(row + V <= M)); }
+template <int V> __device__ __forceinline__ void end_row(float (&v)[V], int c, int D) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = c + j < D ? v[j] : 0.f;
 }
 template <int V> struct Codes { unsigned w[V / 4]; };
 template <int V, bool EVEN> __device__ __forceinline__ Codes<V> load_codes(const signed char* row, int c, int D) {
@@ -119,6 +144,19 @@ template <int V> __device__ __forceinline__ void decode_run(const Codes<V>& q, f
 template <int V, bool EVEN> __device__ __forceinline__ void load_f32(const float* p, int c, int D, float (&v)[V]) {
   cvt_run<DT_FP32, V>(load_run<DT_FP32, V, EVEN>(p, 0, c, D), v);
 }
+// a run of an fp32 vector of D >= V elements without a branch around the load: the one that crosses the end is read from
+// D - V, and moved into place by settle() where it is used
+template <int V, bool EVEN> __device__ __forceinline__ Run<DT_FP32, V> load_vec(const float* p, int c, int D) {
+  return load_run<DT_FP32, V, true>(p, 0, EVEN || c + V <= D ? c : D - V, D);
+}
+template <int V, bool EVEN> __device__ __forceinline__ void settle(Run<DT_FP32, V>& r, int c, int D) {
+  const int by = c + V - D;
+  if (EVEN || by <= 0) return;
+#pragma unroll
+  for (int p = V / 2; p; p /= 2)
+#pragma unroll
+    for (int j = 0; j < V; ++j) r.w[j] = by & p ? (j + p < V ? r.w[j + p < V ? j + p : j] : 0u) : r.w[j];
+}
 // codes and exponent byte of a thread's run; all threads of a group call this together, with zeros past the row's end
 template <int V, bool EVEN> __device__ __forceinline__ void save_run(const float (&v)[V], signed char* codes, unsigned char* bytes, long long row, int D, int c) {
   unsigned m = top_bits<V>(v);
@@ -133,8 +171,9 @@ template <int V, bool EVEN> __device__ __forceinline__ void save_run(const float
   signed char* to = codes + row * D + c;
   if (EVEN || c + V <= D) __builtin_memcpy(to, q.w, V);
   else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) if (c + j < D) to[j] = (signed char)(q.w[j >> 2] >> (8 * (j & 3)));
+    signed char e[V];
+    __builtin_memcpy(e, q.w, V);
+    store_end<V>(to, e, D - c);
   }
   if ((c & (GROUP - 1)) == 0) bytes[row * groups_of(D) + c / GROUP] = (unsigned char)byte;
 }
@@ -154,27 +193,34 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_fwd_kernel(LnF
   const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
   if (RPB > 1 && row >= a.M) return;                        // whole waves: a row per wave
   // runs past the row's end are read from its beginning and zeroed: no branch, so all loads are in flight together
+  const bool whole = EVEN || runs_whole<V>(row, a.M);
   Run<XDT, V> raw[NCH];
   Run<DT_FP32, V> g[NCH], b[NCH];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     const int c = (t + TPR * i) * V;
-    raw[i] = load_run<XDT, V, EVEN>(a.x, row * a.ldx, c < a.D ? c : 0, a.D);
+    if (whole) raw[i] = load_run<XDT, V, true>(a.x, row * a.ldx, c < a.D ? c : 0, a.D);
+    else raw[i] = load_run<XDT, V, false>(a.x, row * a.ldx, c < a.D ? c : 0, a.D);
   }
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     const int c = (t + TPR * i) * V;
-    g[i] = load_run<DT_FP32, V, EVEN>(a.gamma, 0, c < a.D ? c : 0, a.D);
-    b[i] = load_run<DT_FP32, V, EVEN>(a.beta, 0, c < a.D ? c : 0, a.D);
+    if (EVEN || a.D >= V) {
+      g[i] = load_vec<V, EVEN>(a.gamma, c < a.D ? c : 0, a.D);
+      b[i] = load_vec<V, EVEN>(a.beta, c < a.D ? c : 0, a.D);
+    } else {
+      g[i] = load_run<DT_FP32, V, false>(a.gamma, 0, c < a.D ? c : 0, a.D);
+      b[i] = load_run<DT_FP32, V, false>(a.beta, 0, c < a.D ? c : 0, a.D);
+    }
   }
   float v[NCH][V];
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     cvt_run<XDT, V>(raw[i], v[i]);
-    const bool in = (t + TPR * i) * V < a.D;
+    const int c = (t + TPR * i) * V;
 #pragma unroll
-    for (int j = 0; j < V; ++j) { v[i][j] = in ? v[i][j] : 0.f; sum += v[i][j]; }
+    for (int j = 0; j < V; ++j) { v[i][j] = (EVEN ? c : c + j) < a.D ? v[i][j] : 0.f; sum += v[i][j]; }
   }
   const float mean = row_sum<TPR>(sum, red) / (float)a.D;
   float sq = 0.f;
@@ -196,6 +242,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_fwd_kernel(LnF
     for (int j = 0; j < V; ++j) v[i][j] *= rstd;
     if (a.codes) save_run<V, EVEN>(v[i], a.codes, a.bytes, row, a.D, c);
     if (c < a.D) {
+      if (EVEN || a.D >= V) {
+        settle<V, EVEN>(g[i], c, a.D);
+        settle<V, EVEN>(b[i], c, a.D);
+      }
       float y[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) y[j] = __builtin_fmaf(v[i][j], __uint_as_float(g[i].w[j]), __uint_as_float(b[i].w[j]));
@@ -218,7 +268,7 @@ struct LnBwd {
 
 constexpr int SRC_CODES = 3;               // the rows come from their 8-bit copy
 template <int DYT, int SRC, int V, int TPR, int NCH, bool EVEN>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnBwd a) {
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR, TPR == 64 && NCH <= 3 ? 3 : 1) void ln_train_bwd_kernel(LnBwd a) {
   constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
   constexpr int XDT = SRC == SRC_CODES ? DT_BF16 : SRC;
   __shared__ float red[32];
@@ -231,19 +281,24 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnB
     for (int j = 0; j < V; ++j) { dg[i][j] = 0.f; db[i][j] = 0.f; }
   const long long groups = groups_of(a.D);
   struct Loads { Run<DYT, V> dy[NCH]; Run<XDT, V> x[NCH]; Codes<V> codes[NCH]; unsigned byte[NCH]; Run<DT_FP32, V> add[NCH]; float rstd, mean; };
-  auto load = [&](long long row, Loads& l) __attribute__((always_inline)) {
+  auto load_as = [&](auto whole, long long row, Loads& l) __attribute__((always_inline)) {
+    constexpr bool W = decltype(whole)::value;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int c = (t + TPR * i) * V < a.D ? (t + TPR * i) * V : 0;     // no branch around the loads
-      {
-        l.dy[i] = load_run<DYT, V, EVEN>(a.dy, row * a.lddy, c, a.D);
-        if constexpr (SRC == SRC_CODES) {
-          l.codes[i] = load_codes<V, EVEN>(a.codes + row * a.D, c, a.D);
-          l.byte[i] = a.bytes[row * groups + c / GROUP];
-        } else l.x[i] = load_run<XDT, V, EVEN>(a.x, row * a.ldx, c, a.D);
-        if (a.add) l.add[i] = load_any<V, EVEN>(a.add, a.add_dt, row * a.ldadd, c, a.D);
-      }
+      l.dy[i] = load_run<DYT, V, W>(a.dy, row * a.lddy, c, a.D);
+      if constexpr (SRC == SRC_CODES) {
+        l.codes[i] = load_codes<V, W>(a.codes + row * a.D, c, a.D);
+        l.byte[i] = a.bytes[row * groups + c / GROUP];
+      } else l.x[i] = load_run<XDT, V, W>(a.x, row * a.ldx, c, a.D);
+      if (a.add) l.add[i] = load_any<V, W>(a.add, a.add_dt, row * a.ldadd, c, a.D);
     }
+  };
+  auto load = [&](long long row, Loads& l) __attribute__((always_inline)) {
+    // 1024 threads have no registers for both forms (2000 x 12001: 178 against 160 us)
+    if constexpr (EVEN) load_as(std::true_type{}, row, l);
+    else if (TPR < 1024 && runs_whole<V>(row, a.M)) load_as(std::true_type{}, row, l);
+    else load_as(std::false_type{}, row, l);
     l.rstd = a.rstd[row];
     l.mean = SRC == SRC_CODES ? 0.f : a.mean[row];
   };
@@ -276,6 +331,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_bwd_kernel(LnB
           cvt_run<XDT, V>(now.x[i], h[i]);
 #pragma unroll
           for (int j = 0; j < V; ++j) h[i][j] = (h[i][j] - mean) * rstd;
+        }
+        if constexpr (!EVEN && TPR < 1024) {
+          end_row<V>(dy, c, a.D);
+          end_row<V>(h[i], c, a.D);
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -384,8 +443,12 @@ __global__ __launch_bounds__(256) void pack8_kernel(const void* __restrict__ x, 
   for (Walk w((unsigned)groups_of(D) * (GROUP / V)); w.row < (unsigned long long)M; w.step()) {     // a group's threads leave together
     const int c = (int)w.run * V;
     float v[V];
-    if (c < D) cvt_run<DT, V>(load_run<DT, V, EVEN>(x, (long long)w.row * ldx, c, D), v);
-    else {
+    if (c < D) {
+      if (EVEN || w.row + V <= (unsigned long long)M) {
+        cvt_run<DT, V>(load_run<DT, V, true>(x, (long long)w.row * ldx, c, D), v);
+        if constexpr (!EVEN) end_row<V>(v, c, D);
+      } else cvt_run<DT, V>(load_run<DT, V, false>(x, (long long)w.row * ldx, c, D), v);
+    } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] = 0.f;
     }
@@ -406,7 +469,7 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const signed char* __restr
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = 0.f;
     if (c < D) {
-      const Codes<V> q = load_codes<V, EVEN>(codes + row * D, c, D);
+      const Codes<V> q = EVEN || row + V <= M ? load_codes<V, true>(codes + row * D, c, D) : load_codes<V, false>(codes + row * D, c, D);
       float u[V];
       decode_run<V>(q, group_step(bytes[row * groups + c / GROUP]), u);
 #pragma unroll
@@ -429,8 +492,15 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const void* __restrict__ d
   for (Walk w((unsigned)(D + V - 1) / V); w.row < (unsigned long long)M; w.step()) {
     const long long row = (long long)w.row;
     const int c = (int)w.run * V;
-    const Run<DT, V> r = load_run<DT, V, EVEN>(dy, row * lddy, c, D);
-    const Codes<V> q = load_codes<V, EVEN>(codes + row * D, c, D);
+    Run<DT, V> r;
+    Codes<V> q;
+    if (EVEN || row + V <= M) {
+      r = load_run<DT, V, true>(dy, row * lddy, c, D);
+      q = load_codes<V, true>(codes + row * D, c, D);
+    } else {
+      r = load_run<DT, V, false>(dy, row * lddy, c, D);
+      q = load_codes<V, false>(codes + row * D, c, D);
+    }
     float u[V], g[V];
     decode_run<V>(q, group_step(bytes[row * groups + c / GROUP]), u);
     cvt_run<DT, V>(r, g);
