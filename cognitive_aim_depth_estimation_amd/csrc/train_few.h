@@ -116,8 +116,17 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void train_few_kernel(Few g, Epi ep
     const int k = 32 * whole + 8 * fq, left = g.K - k;        // of this lane's eight, `left` exist (none if negative)
     u32x4v af[MT], bf[NF];
     u32x2 raw[8];
+    // the last eight of a row in one load, moved down over those that are not this lane's (a row of fewer: one by one)
     auto some = [&](const unsigned short* p) __attribute__((always_inline)) {
       u32x4v w;
+      if (g.K >= 8) {
+        const int by = left < 0 ? 8 : left < 8 ? 8 - left : 0;
+        __builtin_memcpy(&w, left < 8 ? p + (left - 8) : p, 16);
+        if (by & 4) w = u32x4v{w[2], w[3], 0u, 0u};
+        if (by & 2) w = u32x4v{w[1], w[2], w[3], 0u};
+        if (by & 1) w = u32x4v{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16};
+        return by < 8 ? w : u32x4v{0u, 0u, 0u, 0u};
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = (2 * j < left ? (unsigned)p[2 * j] : 0u) | (2 * j + 1 < left ? (unsigned)p[2 * j + 1] << 16 : 0u);
       return w;
@@ -130,9 +139,12 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void train_few_kernel(Few g, Epi ep
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        raw[e] = u32x2{0, 0};
-        if (e < left) __builtin_memcpy(&raw[e], pb[0] + (size_t)(32 * whole + e) * g.ldb, 8);
+        __builtin_memcpy(&raw[e], pb[0] + ((long long)(32 * whole) + (e < left ? e : left - 1)) * g.ldb, 8);      // k + left = K
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
         raw[e] = four(raw[e]);
+        if (e >= left) raw[e] = u32x2{0, 0};
       }
     }
     multiply(af, bf, raw, k, g.K);

@@ -626,6 +626,43 @@ def test_transposed_and_broadcast_inputs():
     assert torch.equal(dx, same[0]) and torch.equal(dw, same[1]) and torch.equal(db, same[2])
 
 
+@pytest.mark.parametrize("D", [1, 3, 5, 33, 577, 767, 1022, 2047, 4095, 8191, 12001])
+@pytest.mark.parametrize("gap", [0, 3])
+def test_a_row_ignores_what_lies_behind_it(D, gap):
+    """NaN in every second row and between the rows: the others' results are those of the same rows alone."""
+    M = 41
+    def among(t):
+        wide = torch.full((2 * M, D + gap), float("nan"), device="cuda", dtype=t.dtype)
+        wide[::2, :D] = t
+        return wide[:, :D]
+    x, dy = rnd(M, D), rnd(M, D, dtype=torch.bfloat16)
+    g, b = 1 + 0.1 * rnd(D), rnd(D)
+    for t in (x, dy):
+        p, q = T.pack8(among(t)), T.pack8(t)
+        assert torch.equal(p.codes[::2], q.codes) and torch.equal(p.exponents[::2], q.exponents)
+        assert bool((p.exponents[1::2] == 255).all())
+        for o in (torch.bfloat16, torch.float32):
+            assert torch.equal(T.unpack8(p, o)[::2], T.unpack8(q, o)) and bool(T.unpack8(p, o)[1::2].isnan().all())
+        assert torch.equal(T.activation_backward(among(dy), p, "gelu")[::2], T.activation_backward(dy, q, "gelu"))
+        y, mean, rstd, s = T.layer_norm_forward(among(t), g, b, out_dtype=torch.bfloat16, checkpoint=True)
+        y2, mean2, rstd2, s2 = T.layer_norm_forward(t, g, b, out_dtype=torch.bfloat16, checkpoint=True)
+        assert torch.equal(y[::2], y2) and torch.equal(mean[::2], mean2) and torch.equal(rstd[::2], rstd2)
+        assert torch.equal(s.codes[::2], s2.codes) and torch.equal(s.exponents[::2], s2.exponents)
+        assert torch.equal(T.layer_norm_backward(among(dy), among(t), mean, rstd, g, add=among(x))[0][::2],
+                           T.layer_norm_backward(dy, t, mean2, rstd2, g, add=x)[0])
+        assert torch.equal(T.layer_norm_backward(among(dy), s, None, rstd, g)[0][::2], T.layer_norm_backward(dy, s2, None, rstd2, g)[0])
+        # a gradient that is zero in the other rows leaves the sums to these ones
+        near = torch.zeros(2 * M, D, device="cuda", dtype=torch.bfloat16)
+        near[::2] = dy
+        full = torch.zeros(2 * M, D, device="cuda", dtype=t.dtype)
+        full[::2] = t
+        _, m3, r3, s3 = T.layer_norm_forward(full, g, b, checkpoint=True)
+        h = (t.double() - mean2.double()[:, None]) * rstd2.double()[:, None]
+        dg, db = T.layer_norm_backward(near, full, m3, r3, g)[1:]
+        within(db, dy.double().sum(0), 4 * M * U32 * dy.double().abs().sum(0))
+        within(dg, (dy.double() * h).sum(0), 4 * M * U32 * (dy.double() * h).abs().sum(0) + 8 * U32 * (dy.double().abs() * (h.abs() + mean2.double().abs()[:, None] * rstd2.double()[:, None])).sum(0))
+
+
 def test_offsets_past_32_bits():
     """Matrices of more than 2^31 elements: their last rows against the same rows alone."""
     M, D = 600_000, 4096
