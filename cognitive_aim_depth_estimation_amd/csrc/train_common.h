@@ -188,9 +188,10 @@ __device__ __forceinline__ void decode4(unsigned c, float step, float* v) {
   for (int i = 0; i < 4; ++i) v[i] = (float)(signed char)(c >> (8 * i)) * step;
 }
 __device__ __forceinline__ void decode8(u32x2 c, float step, float (&v)[8]) { decode4(c[0], step, v); decode4(c[1], step, v + 4); }
-// 127 steps of a group whose magnitudes reach the top of fp16 can exceed its largest finite value by less than one
-// step: such a value is held at the largest finite one (the group's own values were finite)
-__device__ __forceinline__ float hold_fp16(float y) { return y > 65504.f ? 65504.f : y < -65504.f ? -65504.f : y; }
+// A finite fp16 number of 65024 or more becomes 64 steps of 1024: 65536, past fp16's largest finite value, at which it is
+// held.  Nothing larger comes of fp16 numbers (a code is a multiple of its step); rows of bf16 or fp32 that leave fp16's
+// range become infinities, as in any conversion.
+__device__ __forceinline__ float hold_fp16(float y) { return fabsf(y) == 65536.f ? __builtin_copysignf(65504.f, y) : y; }
 
 // ---- activations -----------------------------------------------------------------------------------------------------
 // Phi(-a), the normal distribution's lower tail, for a in [0, 5.5]: log2 Phi(-a) is close to a parabola, and a

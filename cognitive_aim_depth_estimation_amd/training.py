@@ -83,7 +83,8 @@ def pack8(x: Tensor) -> Checkpoint8:
 
 
 def unpack8(saved: Checkpoint8, dtype: torch.dtype = torch.float32) -> Tensor:
-    """The values of an 8-bit copy: exact in fp32 and bf16, rounded once (and held at +-65504) in fp16."""
+    """The values of an 8-bit copy: exact in fp32 and bf16, rounded once in fp16, where +-65536, which the largest finite
+    numbers become in 8 bits, is held at +-65504 and anything larger is an infinity."""
     codes, exponents = _checkpoint(saved, "saved")
     return (_host or _ops()).unpack8(codes, exponents, dtype)
 

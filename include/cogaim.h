@@ -316,8 +316,9 @@ int cogaim_heatmap_postprocess(const float* attn, float* out, int B, int N, int 
  *    32 columns of a row share the step 2^(exponent - 127), the smallest from 2^-126 up for which the group's largest
  *    magnitude rounds to at most 127 steps; a code is x / step rounded to nearest, ties to even.  Exponent 255 marks a
  *    group that held an infinity or a NaN: all of it stands for NaN.  Steps are powers of two, so a value is exact in
- *    bf16; in fp16 it is rounded once.  Where a code's rounding would pass the largest finite value (63.5 steps of 2^122;
- *    65504 in fp16) it is held below it.
+ *    bf16; in fp16 it is rounded once.  Where a code's rounding would pass the largest finite value (63.5 steps of 2^122)
+ *    it is held below it; in fp16, a value of 65536 (64 steps of 1024: what a finite fp16 number of 65024 or more becomes)
+ *    is held at 65504, and a larger one is an infinity.
  */
 
 /* hf:348,353,441 nn.LayerNorm with what its backward pass needs: y = (x - mean) rstd * gamma + beta, mean and
