@@ -226,7 +226,7 @@ struct EpiInput {
           if constexpr (ACT == ACT_GELU) gelu_both(u[j], value, slope);
           else { value = relu_of(u[j]); slope = relu_slope(u[j]); }
           v[j] *= slope;
-          u[j] = value;
+          u[j] = a_dt == DT_FP16 ? hold_fp16(value) : value;      // finite where the forward's was
         }
       }
       if (a) store_run8<FAST>(a, a_dt, lda, m, n, N, u);

@@ -359,7 +359,7 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* desc, void* workspace, long 
 
 /* Gradient of a linear layer's input, and of the activation that produced that input:
  *   dx = ((dy * scale) W) * act'(u),  u [M,K] the pre-activation of the layer below in 8 bits;  a = act(u) unless NULL
- * (the layer's own input again, for its weight's gradient).  activation 0: no u.  With scale, W * scale (up to 32 rows:
+ * (the layer's own input again, for its weight's gradient; in fp16, 65536 held at 65504 as above).  activation 0: no u.  With scale, W * scale (up to 32 rows:
  * dy * scale) is rounded to `dtype` for the matrix cores; in fp16 relative to the largest scale, so that small scales lose
  * nothing to subnormals. */
 typedef struct {

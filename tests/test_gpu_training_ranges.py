@@ -39,3 +39,19 @@ def test_unpack8_to_fp16_overflows(dtype):
     v = decode(saved.codes, saved.exponents)
     assert bool((v.abs() > 65536).any()) and bool((v.abs() == 65536).any())
     assert torch.equal(T.unpack8(saved, torch.float16), in_fp16(v))
+
+
+@pytest.mark.parametrize("M", [3, 80])
+@pytest.mark.parametrize("name", ["relu", "gelu"])
+def test_activation_again_at_the_top_of_fp16(M, name):
+    """The layer's input, made again from its 8-bit copy, is finite where it was in the forward."""
+    N, K = 40, 72
+    u = torch.full((M, K), 65500.0, device="cuda")
+    u[1] = -65500.0
+    u[2, 32:] = 1e6
+    dy, w = rnd(M, N, dtype=torch.float16), rnd(N, K, dtype=torch.float16)
+    saved = T.pack8(u)
+    _, a = T.linear_backward_input(dy, w, name, saved, want_activation=True)
+    want = in_fp16(act(decode(saved.codes, saved.exponents), name))
+    assert torch.equal(torch.isinf(a), u > 1e5) and bool((a[0] == 65504).all())
+    assert torch.equal(a[0], want[0]) and torch.equal(a[2], want[2]) and float(a[1].abs().max()) < 1e-6
