@@ -193,6 +193,18 @@ __device__ __forceinline__ void decode8(u32x2 c, float step, float (&v)[8]) { de
 // range become infinities, as in any conversion.
 __device__ __forceinline__ float hold_fp16(float y) { return fabsf(y) == 65536.f ? __builtin_copysignf(65504.f, y) : y; }
 
+// ---- 8-bit rows in an fp16 product ---------------------------------------------------------------------------------------
+// fp16 holds a code exactly from steps of 2^-24 to steps of 2^9, fewer than rows come with.  So each group of 32 columns is
+// brought to where its largest step over all rows is 2^9 (`tops`: that step's byte), by a power of two that the finished sums
+// of those columns are divided by again: exact for steps down to 2^-33 of the column's largest, below that rounded to
+// half of fp16's least number, under 2^-41 of the column's largest magnitude.
+constexpr int UNIT_BYTE = 136;                                           // 127 steps of 2^9 = 65024
+__device__ __forceinline__ unsigned unit_byte(unsigned byte, unsigned top) {      // a step in those units; 0 (no step) under 2^-126
+  const int b = (int)byte - (int)top + UNIT_BYTE;
+  return byte == 255u ? 255u : (unsigned)(b > 0 ? b : 0);
+}
+__device__ __forceinline__ float from_unit(float sum, int top) { return __builtin_ldexpf(sum, top - UNIT_BYTE); }
+
 // ---- activations -----------------------------------------------------------------------------------------------------
 // Phi(-a), the normal distribution's lower tail, for a in [0, 5.5]: log2 Phi(-a) is close to a parabola, and a
 // degree-6 polynomial (weighted minimax fit in Chebyshev form, weight Phi(-a) max(1, a)) followed by one exp2 is within
@@ -223,5 +235,9 @@ __device__ __forceinline__ void gelu_both(float x, float& value, float& slope) {
   slope = __builtin_fmaf(x * 0.3989422804f, bell, 0.5f + __builtin_copysignf(0.5f - q, x));
 }
 __device__ __forceinline__ float relu_slope(float x) { return x > 0.f ? 1.f : x != x ? x : 0.f; }
+
+// codes [M, D] -> fp16 [M, width], both ends as above; tops [groups], behind it room for the rows' parts (train_rows.hip)
+long long tops_bytes(int M, int D);
+int unpack8_units(const void* codes, const void* exponents, unsigned char* tops, void* out, int M, int D, int width, hipStream_t st);
 
 }  // namespace train

@@ -235,22 +235,27 @@ struct EpiInput {
   }
 };
 
-struct EpiPlain {                            // the product itself
-  void* out; long long ld; int M, N, dt;
+struct EpiPlain {                            // the product itself, brought back from its columns' units (tops, or null)
+  void* out; long long ld; int M, N, dt; const unsigned char* tops;
   static constexpr int TABLE = 0;
   __device__ __forceinline__ void fill(float2*, int, int) const {}
-  struct Columns {};
+  struct Columns { int top; };
   struct Row {};
   __device__ __forceinline__ void start(int, float (&b)[8]) const {
 #pragma unroll
     for (int j = 0; j < 8; ++j) b[j] = 0.f;
   }
-  __device__ __forceinline__ void columns(int, Columns&) const {}
+  __device__ __forceinline__ void columns(int n, Columns& c) const { c.top = tops && n < N ? tops[n / GROUP] : UNIT_BYTE; }
   template <bool FAST>
   __device__ __forceinline__ void fetch(int, int, Row&) const {}
   template <bool FAST, int X1, int X2>
-  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns&, const Row&, const float2*) const {
-    if (m < M) store_run8<FAST>(out, dt, ld, m, n, N, v);
+  __device__ __forceinline__ void finish(int, int m, int n, float (&v)[8], const Columns& c, const Row&, const float2*) const {
+    if (m >= M) return;
+    if (tops) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = from_unit(v[j], c.top);
+    }
+    store_run8<FAST>(out, dt, ld, m, n, N, v);
   }
 };
 
@@ -297,13 +302,14 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
   epi.template finish<false, 1, 2>(0, m, n, v, col, r, nullptr);
 }
 
-// ROWS rows n of the weight's gradient to a block (their loads in flight together):  G = sum of the parts, with
+// ROWS rows n of the weight's gradient to a block (their loads in flight together):  G = sum of the parts, out of its
+// columns' units (tops, or null), with
 // x = xh * xs + xt put back  (sum_m dy (xh xs + xt) = (dy^T xh) xs + (sum_m dy) xt);  dW = s G, db = s sum dy,
 // ds = sum_k W G + b sum dy.  Four rows where they still make 512 blocks (12 against 17 us at 4096 x 1024 in two
 // parts); one row, for more blocks, below.
 struct WeightFinish {
   const float* part; const float* col_sum; const float* xs; const float* xt; const float* scale; const unsigned short* W;
-  const float* bias; void* dW; float* db; float* ds; long long ldw, lddw; int N, K, Kp, splits, dt, dw_dt;
+  const float* bias; void* dW; float* db; float* ds; const unsigned char* tops; long long ldw, lddw; int N, K, Kp, splits, dt, dw_dt;
 };
 template <int ROWS>
 __global__ __launch_bounds__(256) void weight_finish_kernel(WeightFinish a) {
@@ -349,6 +355,7 @@ __global__ __launch_bounds__(256) void weight_finish_kernel(WeightFinish a) {
         for (int j = 0; j < 4; ++j) g[r][j] += p[j];
       }
     float xs[4], xt[4];
+    const int top = a.tops ? a.tops[k / GROUP] : UNIT_BYTE;              // four columns of one group
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int at = k + j < a.K ? k + j : a.K - 1;
@@ -360,6 +367,7 @@ __global__ __launch_bounds__(256) void weight_finish_kernel(WeightFinish a) {
       if (n0 + r >= a.N) break;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        if (a.tops) g[r][j] = from_unit(g[r][j], top);
         if (a.xs) g[r][j] *= xs[j];
         if (a.xt) g[r][j] = __builtin_fmaf(total[r], xt[j], g[r][j]);
         if (a.ds && k + j < a.K) dot[r] = __builtin_fmaf(w[r][j], g[r][j], dot[r]);
@@ -680,12 +688,14 @@ static bool weight_has_more(const cogaim_linear_bwd_weight_desc* d) {
 }
 static bool weight_needs_finish(const cogaim_linear_bwd_weight_desc* d, const Shape& s) { return s.splits > 1 || weight_has_more(d); }
 
+static bool weight_in_units(const cogaim_linear_bwd_weight_desc* d) { return d->codes && d->dtype == DT_FP16; }
+
 long long cogaim_linear_bwd_weight_workspace_bytes(const cogaim_linear_bwd_weight_desc* d) {
   if (!weight_ok(d)) return COGAIM_EINVAL;
   const Shape s = shape_of(d->N, d->K, d->M, false, weight_has_more(d), false);
   const long long x = d->codes ? round256((long long)d->M * round8(d->K) * 2) : copy_bytes(side(d->x, d->ldx, d->M, d->K));
   const long long part = weight_needs_finish(d, s) ? round256((long long)s.splits * d->N * round8(d->K) * 4) + (long long)s.splits * d->N * 4 : 0;
-  return copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + x + part;
+  return copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + x + part + (weight_in_units(d) ? round256(tops_bytes(d->M, d->K)) : 0);
 }
 
 int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* workspace, long long workspace_bytes, void* stream) {
@@ -698,10 +708,16 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
   if (!d->codes) b = side(d->x, d->ldx, d->M, d->K);
   int rc = run_copies(a, b, d->dtype, ws, st);
   if (rc) return rc;
+  unsigned char* tops = nullptr;
   if (d->codes) {
-    // the 8-bit rows as 16-bit values in front of the product (a power-of-two step makes them exact in bf16)
+    // the 8-bit rows as 16-bit values in front of the product (a power-of-two step makes them exact in bf16, and in fp16
+    // in units of their columns)
     const int k8 = round8(d->K);
-    rc = cogaim_unpack8(d->codes, d->exponents, ws, d->dtype, k8, d->M, d->K, k8, stream);
+    if (weight_in_units(d)) {
+      tops = (unsigned char*)ws;
+      ws += round256(tops_bytes(d->M, d->K));
+      rc = unpack8_units(d->codes, d->exponents, tops, ws, d->M, d->K, k8, st);
+    } else rc = cogaim_unpack8(d->codes, d->exponents, ws, d->dtype, k8, d->M, d->K, k8, stream);
     b = Side{ws, k8, d->M, k8, false, nullptr, nullptr};
     ws += round256((long long)d->M * k8 * 2);
     if (rc) return rc;
@@ -709,7 +725,7 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
   Operands g = operands(a, b, false, false, d->N, d->K, s);
   if (!weight_needs_finish(d, s)) {
     g.col_sum = d->db;
-    const EpiPlain e{d->dw, d->lddw, d->N, d->K, d->dw_dtype};
+    const EpiPlain e{d->dw, d->lddw, d->N, d->K, d->dw_dtype, tops};
     return d->dtype == DT_BF16 ? launch_gemm<__bf16, false, false>(g, s.tile, e, st) : launch_gemm<_Float16, false, false>(g, s.tile, e, st);
   }
   const int kp = round8(d->K);
@@ -719,7 +735,7 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
   const EpiPart e{part, d->N, kp};
   rc = d->dtype == DT_BF16 ? launch_gemm<__bf16, false, false>(g, s.tile, e, st) : launch_gemm<_Float16, false, false>(g, s.tile, e, st);
   if (rc) return rc;
-  const WeightFinish f{part, sums, d->x_scale, d->x_shift, d->scale, (const unsigned short*)d->w, d->bias, d->dw, d->db, d->ds, d->ldw, d->lddw,
+  const WeightFinish f{part, sums, d->x_scale, d->x_shift, d->scale, (const unsigned short*)d->w, d->bias, d->dw, d->db, d->ds, tops, d->ldw, d->lddw,
                        d->N, d->K, kp, s.splits, d->dtype, d->dw_dtype};
   if (d->N >= 4 * 512) hipLaunchKernelGGL(weight_finish_kernel<4>, dim3((d->N + 3) / 4), dim3(256), 0, st, f);
   else hipLaunchKernelGGL(weight_finish_kernel<1>, dim3(d->N), dim3(256), 0, st, f);

@@ -456,11 +456,53 @@ __global__ __launch_bounds__(256) void pack8_kernel(const void* __restrict__ x, 
   }
 }
 
-// codes [M, D] -> out [M, width >= D] (columns past D are written as zero)
+// Largest exponent byte of each column group over a part of the rows, 255 (not finite) left out: tops[part][group].  A block
+// takes four groups, a thread every 1024th row; the last four groups of a row are read together, not past its end.
+__global__ __launch_bounds__(1024) void column_tops_kernel(const unsigned char* __restrict__ bytes, unsigned char* __restrict__ tops, int M, int G, int rows) {
+  __shared__ unsigned char s[16][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g0 = G < 4 ? 0 : (int)(4 * blockIdx.x) < G - 4 ? (int)(4 * blockIdx.x) : G - 4, n = G < 4 ? G : 4;
+  const long long first = (long long)blockIdx.y * rows, last = first + rows < M ? first + rows : M;
+  unsigned top[4] = {0, 0, 0, 0};
+#pragma unroll 8
+  for (long long r = first + threadIdx.x; r < last; r += 1024) {
+    const unsigned char* p = bytes + r * G + g0;
+    unsigned w = 0;
+    if (n == 4) __builtin_memcpy(&w, p, 4);
+    else {
+      w = p[0];
+      if (n > 1) w |= (unsigned)p[1] << 8;
+      if (n > 2) w |= (unsigned)p[2] << 16;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned b = w >> (8 * j) & 255u;
+      top[j] = umax(top[j], b == 255u ? 0u : b);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top[j] = umax(top[j], (unsigned)__shfl_xor((int)top[j], d));
+    if (lane == 0) s[wave][j] = (unsigned char)top[j];
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < n) {
+    unsigned t = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) t = umax(t, s[w][threadIdx.x]);
+    tops[(size_t)blockIdx.y * G + g0 + threadIdx.x] = (unsigned char)t;
+  }
+}
+// rows of a part, at most 1024 parts (more than one: a second launch over the parts)
+int tops_rows(int M) { return M <= 16384 * 1024 ? 16384 : (int)((M + 1023LL) / 1024); }
+int tops_parts(int M) { return (int)((M + tops_rows(M) - 1LL) / tops_rows(M)); }
+
+// codes [M, D] -> out [M, width >= D] (columns past D are written as zero); tops, or null: in units (fp16)
 template <int DT, int V, bool EVEN>
 __global__ __launch_bounds__(256) void unpack8_kernel(const signed char* __restrict__ codes,
                                                       const unsigned char* __restrict__ bytes, void* __restrict__ out,
-                                                      long long ldo, int M, int D, int width) {
+                                                      long long ldo, int M, int D, int width, const unsigned char* __restrict__ tops) {
   const long long groups = groups_of(D);
   for (Walk w((unsigned)(width + V - 1) / V); w.row < (unsigned long long)M; w.step()) {
     const long long row = (long long)w.row;
@@ -471,7 +513,9 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const signed char* __restr
     if (c < D) {
       const Codes<V> q = EVEN || row + V <= M ? load_codes<V, true>(codes + row * D, c, D) : load_codes<V, false>(codes + row * D, c, D);
       float u[V];
-      decode_run<V>(q, group_step(bytes[row * groups + c / GROUP]), u);
+      unsigned byte = bytes[row * groups + c / GROUP];
+      if (DT == DT_FP16 && tops) byte = unit_byte(byte, tops[c / GROUP]);
+      decode_run<V>(q, group_step(byte), u);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         if (DT == DT_FP16) u[j] = hold_fp16(u[j]);
@@ -581,6 +625,20 @@ template <int DYT> void run_ln_bwd_from(const LnBwd& a, int x_dt, int blocks, hi
     else hipLaunchKernelGGL((KERNEL_<DT_, V_, false>), __VA_ARGS__);                                                            \
   } while (0)
 
+namespace train {
+long long tops_bytes(int M, int D) { return ((tops_parts(M) > 1 ? tops_parts(M) : 0) + 1LL) * groups_of(D); }
+
+int unpack8_units(const void* codes, const void* exponents, unsigned char* tops, void* out, int M, int D, int width, hipStream_t st) {
+  const int G = (int)groups_of(D), parts = tops_parts(M);
+  unsigned char* const first = parts > 1 ? tops + G : tops;
+  hipLaunchKernelGGL(column_tops_kernel, dim3((G + 3) / 4, parts), dim3(1024), 0, st, (const unsigned char*)exponents, first, M, G, tops_rows(M));
+  if (parts > 1) hipLaunchKernelGGL(column_tops_kernel, dim3((G + 3) / 4), dim3(1024), 0, st, (const unsigned char*)first, tops, parts, G, parts);
+  BY_EVEN(DT_FP16, 8, (D | width), unpack8_kernel, dim3(blocks_for((unsigned long long)M * (width / 8LL + 1))), dim3(256), 0, st, (const signed char*)codes,
+          (const unsigned char*)exponents, out, (long long)width, M, D, width, (const unsigned char*)tops);
+  return COGAIM_LAUNCH_CHECK();
+}
+}  // namespace train
+
 extern "C" {
 
 int cogaim_layernorm_train_fwd(const void* x, int x_dtype, long long ldx, const float* gamma, const float* beta, void* y,
@@ -640,7 +698,7 @@ int cogaim_unpack8(const void* codes, const void* exponents, void* out, int out_
       !aligned(out, dt_size(out_dtype)))
     return COGAIM_EINVAL;
   BY_TYPE(out_dtype, (D | width), unpack8_kernel, dim3(blocks_for((unsigned long long)M * (width / (out_dtype == DT_FP32 ? 4LL : 8LL) + 1))), dim3(256), 0, (hipStream_t)stream,
-          (const signed char*)codes, (const unsigned char*)exponents, out, ldo, M, D, width);
+          (const signed char*)codes, (const unsigned char*)exponents, out, ldo, M, D, width, (const unsigned char*)nullptr);
   return COGAIM_LAUNCH_CHECK();
 }
 

@@ -143,7 +143,8 @@ def linear_backward_weight(dy: Tensor, x: Union[Tensor, Checkpoint8], weight: Op
                            x_shift: Optional[Tensor] = None,
                            out_dtype: torch.dtype = torch.float32) -> Tuple[Tensor, Tensor, Optional[Tensor]]:
     """``(dW, db, dscale)`` for ``dy [..., N]`` in 16 bits and the layer's input ``x [..., K]``, in dy's type or in 8 bits;
-    an 8-bit copy stands for ``x_scale * copy + x_shift`` (a norm's weight and bias over its kept rows).  Without
+    an 8-bit copy stands for ``x_scale * copy + x_shift`` (a norm's weight and bias over its kept rows) and enters the
+    product exactly whatever dy's type (with fp16, steps under 2^-33 of their column group's largest are rounded).  Without
     ``scale``, ``dW = dy^T x`` and ``db`` sums dy's rows (dscale None).  With ``scale`` (and the forward's ``weight`` and
     ``bias``), for ``y = scale * (x weight^T + bias)``: dW and db are those times scale, ``dscale`` sums ``dy * (x weight^T + bias)``.
     db and dscale are fp32, dW is of type ``out_dtype``."""

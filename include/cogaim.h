@@ -370,7 +370,8 @@ long long cogaim_linear_bwd_input_workspace_bytes(const cogaim_linear_bwd_input_
 int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* desc, void* workspace, long long workspace_bytes, void* stream);
 
 /* Gradients of a linear layer's parameters.  x [M,K] is given in 16 bits, or in 8 bits with x = xh * x_scale + x_shift
- * (fp32 [K], NULL: 1 and 0; a LayerNorm's weight and bias over its kept rows).  dW [N,K] = scale * dy^T x, db [N] =
+ * (fp32 [K], NULL: 1 and 0; a LayerNorm's weight and bias over its kept rows).  Codes enter the product exactly:
+ * any value in bf16, in fp16 those within 2^33 of a column group's largest step over the rows, whatever that is.  dW [N,K] = scale * dy^T x, db [N] =
  * scale * sum over rows of dy, and, with scale (fp32 [N]), ds [N] = sum over rows of dy (x W^T + bias), for which w and
  * bias (NULL: none) are read; without scale ds is NULL. */
 typedef struct {

@@ -55,3 +55,41 @@ def test_activation_again_at_the_top_of_fp16(M, name):
     want = in_fp16(act(decode(saved.codes, saved.exponents), name))
     assert torch.equal(torch.isinf(a), u > 1e5) and bool((a[0] == 65504).all())
     assert torch.equal(a[0], want[0]) and torch.equal(a[2], want[2]) and float(a[1].abs().max()) < 1e-6
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 8, 32), (5, 24, 40), (70, 33, 161), (700, 136, 288), (5000, 64, 1000), (3000, 520, 4096)])
+@pytest.mark.parametrize("affine,scaled", [(False, False), (True, False), (False, True)])
+def test_linear_backward_weight_fp16_any_magnitude(M, N, K, affine, scaled):
+    """8-bit rows whose column groups lie anywhere between 1e-30 and 1e30 and vary by 2^30 from row to row: their codes enter
+    an fp16 product exactly, so the result is off only by the order of its fp32 sums.  (A column's steps more than 2^33 below
+    its largest are rounded: by half of fp16's least number where the largest step is 2^9.)"""
+    t = torch.float16
+    groups = -(-K // 32)
+    size = torch.tensor([1.0, 1e-30, 1e-12, 3e-8, 1e-5, 300.0, 1e6, 1e30, 0.0], device="cuda").repeat(groups)[:groups].repeat_interleave(32)[:K]
+    x = rnd(M, K) * size * torch.exp2(-torch.randint(0, 31, (M, 1), device="cuda").float())
+    saved = T.pack8(x)
+    v, dy = decode(saved.codes, saved.exponents), rnd(M, N, dtype=t, scale=0.1)
+    more, d = {}, dy.double()
+    xs = xt = None
+    if affine:
+        xs, xt = 1 + 0.2 * rnd(K), 0.1 * rnd(K)
+    if scaled:
+        more = {"weight": rnd(N, K, dtype=t), "scale": 0.5 + torch.rand(N, device="cuda")}
+    dW, db, _ = T.linear_backward_weight(dy, saved, x_scale=xs, x_shift=xt, **more)
+    want, bound = d.t() @ v, (M + 8) * 2 * U32 * (d.abs().t() @ v.abs())
+    bound = bound + d.abs().sum(0)[:, None] * steps(saved.exponents, K).amax(0) * 2.0 ** -34
+    if affine:
+        total = d.sum(0)
+        tb = (M + 8) * 2 * U32 * d.abs().sum(0)
+        shift = xt.double()
+        bound = bound * xs.double().abs() + tb[:, None] * shift.abs() + 4 * U32 * ((want * xs.double()).abs() + total.abs()[:, None] * shift.abs())
+        want = want * xs.double() + total[:, None] * shift
+    if scaled:
+        s = more["scale"].double()[:, None]
+        want, bound = want * s, bound * s + U32 * (want * s).abs()
+    within(dW, want, bound + U32 * want.abs() + least(torch.float32), "dW")
+    within(db, d.sum(0) * (more["scale"].double() if scaled else 1), (M + 8) * 4 * U32 * d.abs().sum(0), "db")
+    x[M // 2, K - 1] = float("nan")
+    dW = T.linear_backward_weight(dy, T.pack8(x), x_scale=xs, x_shift=xt, **more)[0]
+    bad = torch.isnan(dW)
+    assert bool(bad[:, (K - 1) // 32 * 32:].all()) and not bool(bad[:, :(K - 1) // 32 * 32].any())
