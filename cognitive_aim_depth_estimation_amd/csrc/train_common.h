@@ -55,6 +55,8 @@ __device__ __forceinline__ unsigned bits16(float y, int dt) {
   return __builtin_bit_cast(unsigned short, (_Float16)y);
 }
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+// number of 16-bit parts that hold an fp32 value: three of bf16 (24 bits), two of fp16 (22 bits, down to its least number)
+constexpr int parts_of(int dt) { return dt == DT_BF16 ? 3 : 2; }
 template <int V> __device__ __forceinline__ void pack_half(const float (&y)[V], int dt, void* to) {       // V 16-bit values in registers
   typedef float fv __attribute__((ext_vector_type(V)));
   typedef __bf16 bv __attribute__((ext_vector_type(V)));
@@ -64,6 +66,19 @@ template <int V> __device__ __forceinline__ void pack_half(const float (&y)[V], 
   for (int i = 0; i < V; ++i) v[i] = y[i];
   if (dt == DT_BF16) { const bv h = __builtin_convertvector(v, bv); __builtin_memcpy(to, &h, 2 * V); }
   else { const hv h = __builtin_convertvector(v, hv); __builtin_memcpy(to, &h, 2 * V); }
+}
+// eight values rounded to 16 bits, and what the rounding left of them (nothing of one that is not finite)
+__device__ __forceinline__ void take_part(float (&v)[8], int dt, void* to) {
+  pack_half<8>(v, dt, to);
+  u32x4v w;
+  __builtin_memcpy(&w, to, 16);
+  float h[8];
+  cvt_raw8(Raw8{w, w}, dt, h);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float left = v[j] - h[j];
+    v[j] = fabsf(left) < __builtin_inff() ? left : 0.f;
+  }
 }
 template <bool STREAM = false>
 __device__ __forceinline__ void store_vec8(void* p, int dt, size_t off, const float (&y)[8]) {

@@ -13,6 +13,7 @@ constexpr int FEW_ROWS = 32, FEW_WAVES = 8;
 struct Few {
   const void* A; const void* B; const float* scale;        // scale: of A's columns (input gradient), or null
   long long lda, ldb; int M, N, K;                          // result [M, N], sum over K
+  int parts;                                                // 16-bit parts that A * scale is taken in
 };
 
 // ALONG: B is [N][K] (forward), a lane's fragment is one load; otherwise B is [K][N] (input gradient): a lane loads four
@@ -59,19 +60,6 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void train_few_kernel(Few g, Epi ep
   };
   // one step from loaded operands: k its first element for this lane, `limit` the sum's end
   auto multiply = [&](u32x4v (&af)[MT], u32x4v (&bf)[NF], const u32x2* raw, int k, int limit) __attribute__((always_inline)) {
-    if (g.scale) {
-      float s[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = g.scale[k + j < limit ? k + j : limit - 1] * up;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        float v[8];
-        cvt_raw8(Raw8{af[i], af[i]}, DT, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = k + j < limit ? v[j] * s[j] : 0.f;
-        pack_half<8>(v, DT, &af[i]);
-      }
-    }
     if constexpr (!ALONG) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -79,10 +67,28 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void train_few_kernel(Few g, Epi ep
         for (int d = 0; d < 4; ++d)
           bf[j][d] = __builtin_amdgcn_perm(raw[2 * d + 1][j >> 1], raw[2 * d][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
     }
+    float v[MT][8];
+    if (g.scale) {
+      float s[8];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+      for (int j = 0; j < 8; ++j) s[j] = g.scale[k + j < limit ? k + j : limit - 1] * up;
 #pragma unroll
-      for (int j = 0; j < NF; ++j) acc[i][j] = H::mfma16(__builtin_bit_cast(v8, bf[j]), __builtin_bit_cast(v8, af[i]), acc[i][j]);
+      for (int i = 0; i < MT; ++i) {
+        cvt_raw8(Raw8{af[i], af[i]}, DT, v[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = k + j < limit ? v[i][j] * s[j] : 0.f;
+        take_part(v[i], DT, &af[i]);
+      }
+    }
+    for (int p = 0;;) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = H::mfma16(__builtin_bit_cast(v8, bf[j]), __builtin_bit_cast(v8, af[i]), acc[i][j]);
+      if (++p >= g.parts) break;                              // uniform over the launch
+#pragma unroll
+      for (int i = 0; i < MT; ++i) take_part(v[i], DT, &af[i]);
+    }
   };
 
   for (int c0 = wave; c0 < whole; c0 += FEW_WAVES * STEPS) {

@@ -401,10 +401,12 @@ __global__ __launch_bounds__(256) void weight_finish_kernel(WeightFinish a) {
 }
 
 // Copies of operands whose rows the DMA's 16-byte loads cannot address (odd widths, strides or bases), padded with zeros to
-// a multiple of eight columns; with `scale`, row r times scale[r] (rounded once to 16 bits: the matrix cores take it so), in
-// fp16 times scale[r] * up, and *unit = down.
+// a multiple of eight columns; with `scale`, row r times scale[r] (in fp16 times scale[r] * up, and *unit = down).  The
+// matrix cores take 16 bits.  For a 16-bit result the product is rounded once, by as much as the result itself will be: independent
+// roundings of the terms, no larger together than one of their sum.  An fp32 result keeps its precision: the copy then holds
+// `parts` matrices, each the 16-bit rounding of what the ones before it left, and the product is taken with each.
 // Both operands of a product in one launch: blocks [0, blocks0) copy the first.
-struct CopyOne { const unsigned short* src; unsigned short* dst; const float* scale; float* unit; long long ld; int rows, cols, padded; };
+struct CopyOne { const unsigned short* src; unsigned short* dst; const float* scale; float* unit; long long ld; int rows, cols, padded, parts; };
 struct CopyTwo { CopyOne one[2]; unsigned blocks0; int dt; };
 __global__ __launch_bounds__(256) void copy_rows_kernel(CopyTwo a) {
   const bool second = blockIdx.x >= a.blocks0;
@@ -439,7 +441,12 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(CopyTwo a) {
       cvt_raw8(Raw8{w, w}, a.dt, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = k0 + j < c.cols ? v[j] * s : 0.f;   // the padding stays zero whatever the scale
-      pack_half<8>(v, a.dt, &w);
+      take_part(v, a.dt, &w);
+      for (int p = 1; p < c.parts; ++p) {
+        u32x4v low;
+        take_part(v, a.dt, &low);
+        *reinterpret_cast<u32x4v*>(c.dst + ((unsigned long long)p * c.rows + r) * c.padded + k0) = low;
+      }
     }
     *reinterpret_cast<u32x4v*>(c.dst + r * c.padded + k0) = w;
   }
@@ -497,12 +504,12 @@ long long round256(long long v) { return (v + 255) / 256 * 256; }
 int round8(int v) { return (v + 7) & ~7; }
 
 // an operand as the main loop takes it: `copy` when 16-byte loads cannot address it
-struct Side { const void* p; long long ld; int rows, cols; bool copy; const float* scale; float* unit; };
-Side side(const void* p, long long ld, int rows, int cols, const float* scale = nullptr) {
-  Side s{p, ld, rows, cols, scale || (cols & 7) || (ld & 7) || !aligned(p, 16), scale, nullptr};
+struct Side { const void* p; long long ld; int rows, cols; bool copy; const float* scale; float* unit; int parts; };
+Side side(const void* p, long long ld, int rows, int cols, const float* scale = nullptr, int parts = 1) {
+  Side s{p, ld, rows, cols, scale || (cols & 7) || (ld & 7) || !aligned(p, 16), scale, nullptr, parts};
   return s;
 }
-long long copy_bytes(const Side& s) { return s.copy ? round256((long long)s.rows * round8(s.cols) * 2) : 0; }
+long long copy_bytes(const Side& s) { return s.copy ? round256((long long)s.rows * round8(s.cols) * 2 * s.parts) : 0; }
 
 // copies those of the two operands that need it, moves `ws` behind them
 int run_copies(Side& a, Side& b, int dt, char*& ws, hipStream_t st) {
@@ -513,11 +520,12 @@ int run_copies(Side& a, Side& b, int dt, char*& ws, hipStream_t st) {
   for (Side* s : {&a, &b}) {
     if (!s->copy) continue;
     const int c8 = round8(s->cols);
-    c.one[n] = CopyOne{(const unsigned short*)s->p, (unsigned short*)ws, s->scale, s->unit, s->ld, s->rows, s->cols, c8};
+    const long long bytes = copy_bytes(*s);
+    c.one[n] = CopyOne{(const unsigned short*)s->p, (unsigned short*)ws, s->scale, s->unit, s->ld, s->rows, s->cols, c8, s->parts};
     const unsigned long long want = ((unsigned long long)s->rows * (c8 / 8) + 255) / 256;
     blocks[n++] = (unsigned)(want > 256 * 16 ? 256 * 16 : want);
     s->p = ws; s->ld = c8; s->cols = c8;
-    ws += round256((long long)s->rows * c8 * 2);
+    ws += bytes;
   }
   if (n == 0) return COGAIM_OK;
   c.blocks0 = blocks[0];
@@ -545,15 +553,20 @@ int launch_gemm(const Operands& g, int tile, const Epi& e, hipStream_t st) {
 // the epilogue runs in a kernel of its own: parts to add, or a result that 16-byte stores cannot reach
 template <class Epi> bool joins(const Shape& s, const Epi& e) { return s.splits > 1 || (!e.fast() && s.tile != TILE_64); }
 
+// with several parts of B (matrices behind one another) the join adds their products, too
 template <class T, bool AKC, bool BKC, class Epi>
-int product(const Operands& g, const Shape& s, const Epi& e, float* part, hipStream_t st) {
-  if (!joins(s, e)) return e.fast() ? launch_gemm<T, AKC, BKC>(g, s.tile, e, st) : launch_gemm<T, AKC, BKC, false>(g, s.tile, e, st);
+int product(const Operands& g, const Shape& s, const Epi& e, float* part, hipStream_t st, int parts = 1) {
+  if (parts == 1 && !joins(s, e)) return e.fast() ? launch_gemm<T, AKC, BKC>(g, s.tile, e, st) : launch_gemm<T, AKC, BKC, false>(g, s.tile, e, st);
   const int Np = round8(g.N);
-  const int rc = launch_gemm<T, AKC, BKC>(g, s.tile, EpiPart{part, g.M, Np}, st);
-  if (rc) return rc;
+  for (int p = 0; p < parts; ++p) {
+    Operands one = g;
+    one.B = reinterpret_cast<const unsigned short*>(g.B) + (size_t)p * g.ldb * (BKC ? g.rows_b : g.KB);
+    const int rc = launch_gemm<T, AKC, BKC>(one, s.tile, EpiPart{part + (size_t)p * s.splits * g.M * Np, g.M, Np}, st);
+    if (rc) return rc;
+  }
   const long long threads = (long long)g.M * groups_of(g.N) * 4;
   if ((threads + 255) / 256 >= (1LL << 31)) return COGAIM_EINVAL;
-  hipLaunchKernelGGL((join_kernel<Epi>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, part, s.splits, g.M, g.N, Np, e);
+  hipLaunchKernelGGL((join_kernel<Epi>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, part, s.splits * parts, g.M, g.N, Np, e);
   return COGAIM_LAUNCH_CHECK();
 }
 
@@ -620,7 +633,7 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long lon
   if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   if (few_rows(d->M, d->N, d->K, true)) {
-    const Few f{d->x, d->w, nullptr, d->ldx, d->ldw, d->M, d->N, d->K};
+    const Few f{d->x, d->w, nullptr, d->ldx, d->ldw, d->M, d->N, d->K, 1};
 #define FEW_RUN(T_, DT_)                                                                      \
   (d->activation == ACT_RELU ? launch_few<T_, DT_, true>(f, forward_epi<ACT_RELU>(d), st)      \
    : d->activation == ACT_GELU ? launch_few<T_, DT_, true>(f, forward_epi<ACT_GELU>(d), st)    \
@@ -642,13 +655,18 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* d, void* workspace, long lon
 }
 
 static bool input_unit(const cogaim_linear_bwd_input_desc* d) { return d->scale && d->dtype == DT_FP16; }
+static int input_parts(const cogaim_linear_bwd_input_desc* d) { return d->scale && d->dx_dtype == DT_FP32 ? parts_of(d->dtype) : 1; }
+static Shape input_shape(const cogaim_linear_bwd_input_desc* d) {
+  return shape_of(d->M, d->K, d->N, true, input_parts(d) > 1, !input_epi<ACT_NONE>(d).fast());
+}
 
 long long cogaim_linear_bwd_input_workspace_bytes(const cogaim_linear_bwd_input_desc* d) {
   if (!input_ok(d)) return COGAIM_EINVAL;
   if (few_rows(d->M, d->K, d->N, false)) return 0;
-  const Shape s = shape_of(d->M, d->K, d->N, true, false, !input_epi<ACT_NONE>(d).fast());
-  return (input_unit(d) ? 256 : 0) + copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + copy_bytes(side(d->w, d->ldw, d->N, d->K, d->scale)) +
-         (joins(s, input_epi<ACT_NONE>(d)) ? (long long)s.splits * d->M * round8(d->K) * 4 : 0);
+  const Shape s = input_shape(d);
+  const int parts = input_parts(d);
+  return (input_unit(d) ? 256 : 0) + copy_bytes(side(d->dy, d->lddy, d->M, d->N)) + copy_bytes(side(d->w, d->ldw, d->N, d->K, d->scale, parts)) +
+         (parts > 1 || joins(s, input_epi<ACT_NONE>(d)) ? (long long)parts * s.splits * d->M * round8(d->K) * 4 : 0);
 }
 
 int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspace, long long workspace_bytes, void* stream) {
@@ -656,7 +674,7 @@ int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspa
   if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))) return COGAIM_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   if (few_rows(d->M, d->K, d->N, false)) {
-    const Few f{d->dy, d->w, d->scale, d->lddy, d->ldw, d->M, d->K, d->N};
+    const Few f{d->dy, d->w, d->scale, d->lddy, d->ldw, d->M, d->K, d->N, input_parts(d)};
 #define FEW_RUN(T_, DT_)                                                                      \
   (d->activation == ACT_RELU ? launch_few<T_, DT_, false>(f, input_epi<ACT_RELU>(d), st)       \
    : d->activation == ACT_GELU ? launch_few<T_, DT_, false>(f, input_epi<ACT_GELU>(d), st)     \
@@ -664,8 +682,9 @@ int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspa
     return d->dtype == DT_BF16 ? FEW_RUN(__bf16, DT_BF16) : FEW_RUN(_Float16, DT_FP16);
 #undef FEW_RUN
   }
-  const Shape s = shape_of(d->M, d->K, d->N, true, false, !input_epi<ACT_NONE>(d).fast());
-  Side a = side(d->dy, d->lddy, d->M, d->N), b = side(d->w, d->ldw, d->N, d->K, d->scale);
+  const Shape s = input_shape(d);
+  const int parts = input_parts(d);
+  Side a = side(d->dy, d->lddy, d->M, d->N), b = side(d->w, d->ldw, d->N, d->K, d->scale, parts);
   char* ws = (char*)workspace;
   if (input_unit(d)) {
     b.unit = (float*)ws;
@@ -676,9 +695,9 @@ int cogaim_linear_bwd_input(const cogaim_linear_bwd_input_desc* d, void* workspa
   if (rc) return rc;
   const Operands g = operands(a, b, true, false, d->M, d->K, s);
 #define IN_RUN(T_)                                                                                                     \
-  (d->activation == ACT_RELU ? product<T_, true, false>(g, s, input_epi<ACT_RELU>(d, unit), (float*)ws, st)                         \
-   : d->activation == ACT_GELU ? product<T_, true, false>(g, s, input_epi<ACT_GELU>(d, unit), (float*)ws, st)                       \
-                               : product<T_, true, false>(g, s, input_epi<ACT_NONE>(d, unit), (float*)ws, st))
+  (d->activation == ACT_RELU ? product<T_, true, false>(g, s, input_epi<ACT_RELU>(d, unit), (float*)ws, st, parts)                         \
+   : d->activation == ACT_GELU ? product<T_, true, false>(g, s, input_epi<ACT_GELU>(d, unit), (float*)ws, st, parts)                       \
+                               : product<T_, true, false>(g, s, input_epi<ACT_NONE>(d, unit), (float*)ws, st, parts))
   return d->dtype == DT_BF16 ? IN_RUN(__bf16) : IN_RUN(_Float16);
 }
 
@@ -718,7 +737,7 @@ int cogaim_linear_bwd_weight(const cogaim_linear_bwd_weight_desc* d, void* works
       ws += round256(tops_bytes(d->M, d->K));
       rc = unpack8_units(d->codes, d->exponents, tops, ws, d->M, d->K, k8, st);
     } else rc = cogaim_unpack8(d->codes, d->exponents, ws, d->dtype, k8, d->M, d->K, k8, stream);
-    b = Side{ws, k8, d->M, k8, false, nullptr, nullptr};
+    b = Side{ws, k8, d->M, k8, false, nullptr, nullptr, 1};
     ws += round256((long long)d->M * k8 * 2);
     if (rc) return rc;
   }

@@ -131,9 +131,10 @@ def linear_backward_input(dy: Tensor, weight: Tensor, activation: str = "none", 
                           want_activation: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
     """``(dx, a)`` for ``dy [..., N]`` and ``weight [N, K]`` of one 16-bit type:  ``dx = ((dy * scale) weight) * act'(u)``,
     ``u [..., K]`` the pre-activation, kept in 8 bits (``saved``), of the activation that produced the layer's input; with
-    ``want_activation``, ``a = act(u)`` in 16 bits: that input again, for ``linear_backward_weight``.  With ``scale``,
-    ``weight * scale`` (``dy * scale`` up to 32 rows) is rounded to 16 bits, in fp16 relative to the largest scale: a
-    LayerScale of 1e-5 loses nothing to subnormals."""
+    ``want_activation``, ``a = act(u)`` in 16 bits: that input again, for ``linear_backward_weight``.  With ``scale``, the
+    matrix cores take ``weight * scale`` (``dy * scale`` up to 32 rows): rounded to 16 bits for a 16-bit dx, in parts that keep
+    fp32's precision for an fp32 one; in fp16 relative to the largest scale, so that a LayerScale of 1e-5 does not push
+    the operand into subnormals (a small dx in fp16 still does: ask for fp32 or bf16, or scale the loss)."""
     codes, exponents = (None, None) if saved is None else _checkpoint(saved, "saved")
     return (_host or _ops()).linear_backward_input(dy, weight, activation, codes, exponents, scale, out_dtype, want_activation)
 

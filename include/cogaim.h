@@ -359,9 +359,9 @@ int cogaim_linear_fwd(const cogaim_linear_fwd_desc* desc, void* workspace, long 
 
 /* Gradient of a linear layer's input, and of the activation that produced that input:
  *   dx = ((dy * scale) W) * act'(u),  u [M,K] the pre-activation of the layer below in 8 bits;  a = act(u) unless NULL
- * (the layer's own input again, for its weight's gradient; in fp16, 65536 held at 65504 as above).  activation 0: no u.  With scale, W * scale (up to 32 rows:
- * dy * scale) is rounded to `dtype` for the matrix cores; in fp16 relative to the largest scale, so that small scales lose
- * nothing to subnormals. */
+ * (the layer's own input again, for its weight's gradient; in fp16, 65536 held at 65504 as above).  activation 0: no u.  With scale, the matrix cores take W * scale (up
+ * to 32 rows: dy * scale) rounded to `dtype`, in fp16 relative to the largest scale, so that small scales do not push the
+ * operand into subnormals; for an fp32 dx in as many parts of `dtype` as hold it (three of bf16, two of fp16). */
 typedef struct {
   const void* dy; const void* w; const float* scale; const void* codes; const void* exponents; void* dx; void* a;
   long long lddy, ldw, lddx, lda; int M, N, K, dtype, dx_dtype, activation;

@@ -93,3 +93,25 @@ def test_linear_backward_weight_fp16_any_magnitude(M, N, K, affine, scaled):
     dW = T.linear_backward_weight(dy, T.pack8(x), x_scale=xs, x_shift=xt, **more)[0]
     bad = torch.isnan(dW)
     assert bool(bad[:, (K - 1) // 32 * 32:].all()) and not bool(bad[:, :(K - 1) // 32 * 32].any())
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 64, 40), (20, 333, 72), (32, 1001, 333), (33, 1001, 333), (150, 520, 264), (70, 33, 41), (300, 4096, 128), (2600, 264, 1024)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("size", [1e-5, 1.0])
+def test_linear_backward_input_scale_in_fp32(M, N, K, dtype, size):
+    """An fp32 result keeps fp32's precision through the scale: the scaled operand is taken in 16-bit parts.  Three of bf16
+    hold 24 bits.  Two of fp16 hold 22, and are off by half of fp16's least number, in units of at most twice the largest
+    scale, where the second part is that small."""
+    t = DT[dtype]
+    dy, w = rnd(M, N, dtype=t, scale=0.1), rnd(N, K, dtype=t, scale=N ** -0.5)
+    s = size * (0.5 + torch.rand(N, device="cuda"))
+    dx, _ = T.linear_backward_input(dy, w, scale=s, out_dtype=torch.float32)
+    want, wide = dy.double() @ (w.double() * s.double()[:, None]), (dy.double().abs() * s.double()) @ w.double().abs()
+    bound = (3 * (N + 8) + 8) * 2 * U32 * wide
+    if dtype == "fp16":
+        bound = bound + 2.0 ** -22 * wide + 2.0 ** -24 * float(s.max()) * (dy.double().abs().sum(1, keepdim=True) + w.double().abs().sum(0))
+    # the worst case of a long sum's order would hide a rounding of 2^-9: independent roundings of that size would give the
+    # 2-norm 2^-9 / sqrt(3) of the terms' root sum of squares, fp32 sums a thousandth of it
+    within(dx, want, bound, "dx")
+    terms = ((dy.double() * s.double()).square() @ w.double().square()).sqrt()
+    assert float(((dx.double() - want) / terms).square().mean().sqrt()) <= (2.0 ** -17 if dtype == "bf16" else 2.0 ** -14)
