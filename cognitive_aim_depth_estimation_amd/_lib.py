@@ -64,6 +64,7 @@ SIGNATURES = {
     "cogaim_layernorm_train_fwd": [P, I, LL, P, P, P, I, LL, P, P, P, P, I, I, F, P],
     "cogaim_layernorm_bwd_workspace_bytes": [I, I],
     "cogaim_layernorm_bwd": [P, I, LL, P, I, LL, P, P, P, P, P, P, I, LL, P, I, LL, P, P, I, I, P, LL, P],
+    "cogaim_scale_unit": [P, P, P, I, P],
     "cogaim_pack8": [P, I, LL, P, P, I, I, P],
     "cogaim_unpack8": [P, P, P, I, LL, I, I, I, P],
     "cogaim_activation_bwd": [P, I, LL, P, P, P, I, LL, I, I, I, P],

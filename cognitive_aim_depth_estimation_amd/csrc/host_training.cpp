@@ -20,7 +20,7 @@ enum { ACT_NONE, ACT_RELU, ACT_GELU };
   X(cogaim_pack8) X(cogaim_unpack8) X(cogaim_activation_bwd) X(cogaim_layernorm_train_fwd) X(cogaim_layernorm_bwd)        \
   X(cogaim_layernorm_bwd_workspace_bytes) X(cogaim_linear_fwd) X(cogaim_linear_fwd_workspace_bytes)                       \
   X(cogaim_linear_bwd_input) X(cogaim_linear_bwd_input_workspace_bytes) X(cogaim_linear_bwd_weight)                       \
-  X(cogaim_linear_bwd_weight_workspace_bytes)
+  X(cogaim_linear_bwd_weight_workspace_bytes) X(cogaim_scale_unit)
 #define DECLARE(n) decltype(&::n) n##_;
 ENTRIES(DECLARE)
 PyObject* error_class = nullptr;
@@ -249,6 +249,16 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& dy, const O
   return {dx, dw, db};
 }
 
+// scale times a power of two that brings small scales towards 1, and the 1-element tensor that undoes it
+std::tuple<Tensor, Tensor> scale_unit(const Tensor& scale) {
+  TORCH_CHECK_VALUE(scale.dim() == 1 && scale.size(0) >= 1, "scale must be a vector");
+  const OptTensor s = vec(scale, "scale", narrow(scale.size(0), "scale"), scale.device());
+  const On on(scale.device());
+  const Tensor scaled = fresh(scale, scale.sizes(), at::kFloat), unit = fresh(scale, {1}, at::kFloat);
+  check(cogaim_scale_unit_((const float*)s->data_ptr(), (float*)scaled.data_ptr(), (float*)unit.data_ptr(), (int)scale.size(0), on.stream), "cogaim_scale_unit");
+  return {scaled, unit};
+}
+
 // ---- linear layers -----------------------------------------------------------------------------------------------
 template <class Desc>
 void run(const Desc& d, long long (*size)(const Desc*), int (*launch)(const Desc*, void*, long long, void*), const char* name, const Tensor& like, void* stream) {
@@ -399,6 +409,7 @@ PYBIND11_MODULE(_host, m) {
   m.def("activation_backward", &activation_backward);
   m.def("layer_norm_forward", &layer_norm_forward);
   m.def("layer_norm_backward", &layer_norm_backward);
+  m.def("scale_unit", &scale_unit);
   m.def("linear_forward", &linear_forward);
   m.def("linear_backward_input", &linear_backward_input);
   m.def("linear_backward_weight", &linear_backward_weight);

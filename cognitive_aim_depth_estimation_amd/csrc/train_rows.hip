@@ -418,6 +418,21 @@ __global__ __launch_bounds__(1024) void ln_train_reduce_kernel(const float* __re
   }
 }
 
+// A LayerScale vector times the power of two that brings its largest magnitude into [2^-5, 2^-4), where it is smaller, and
+// what undoes it.  One block; a vector has a few thousand elements.
+__global__ __launch_bounds__(256) void scale_unit_kernel(const float* __restrict__ scale, float* __restrict__ scaled, float* __restrict__ unit, int N) {
+  __shared__ unsigned tops[4];
+  const unsigned mine = wave_top(scale, N, threadIdx.x, 256);
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  const unsigned e = umax(umax(tops[0], tops[1]), umax(tops[2], tops[3])) >> 23;           // 2^(e - 127) or more
+  constexpr unsigned E = 122;                                                              // 2^-5
+  const bool small = e != 0 && e < E;                                                      // not zeros alone (subnormals stay as they are)
+  const float up = small ? __uint_as_float((127 + E - e) << 23) : 1.f;
+  for (int i = threadIdx.x; i < N; i += 256) scaled[i] = scale[i] * up;
+  if (threadIdx.x == 0) *unit = small ? __uint_as_float((127 + e - E) << 23) : 1.f;
+}
+
 // Walks the runs of a matrix, thread by thread with the grid's stride, without a division per step.
 struct Walk {
   unsigned long long i, row; unsigned run, per_row, drow, drun;
@@ -681,6 +696,12 @@ int cogaim_layernorm_bwd(const void* dy, int dy_dtype, long long lddy, const voi
   else run_ln_bwd_from<DT_FP32>(a, x_dtype, nblk, (hipStream_t)stream);
   if (nblk > 1) hipLaunchKernelGGL(ln_train_reduce_kernel, dim3((2 * D + 31) / 32), dim3(1024), 0, (hipStream_t)stream,
                      (const float*)workspace, dgamma, dbeta, nblk, D);
+  return COGAIM_LAUNCH_CHECK();
+}
+
+int cogaim_scale_unit(const float* scale, float* scaled, float* unit, int N, void* stream) {
+  if (!scale || !scaled || !unit || N <= 0) return COGAIM_EINVAL;
+  hipLaunchKernelGGL(scale_unit_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, scale, scaled, unit, N);
   return COGAIM_LAUNCH_CHECK();
 }
 

@@ -239,16 +239,22 @@ class _MlpHalf(torch.autograd.Function):
         need = ctx.needs_input_grad
         d16 = dy.to(ctx.compute)
         second = need[5] or need[6] or need[7]
-        du, a = linear_backward_input(d16, v2, "gelu", pre, scale=scale, want_activation=second)
+        # fp16: du and dh carry the power of two that keeps a small LayerScale out of the subnormals; `unit` undoes it on the
+        # vectors that dW1, dx and the sums are multiplied by
+        carried, unit = (scale, None) if scale is None or ctx.compute != torch.float16 else (_host or _ops()).scale_unit(scale)
+        du, a = linear_backward_input(d16, v2, "gelu", pre, scale=carried, want_activation=second)
         dw2 = db2 = ds = dw1 = db1 = dx = dg = db = None
         if second:
             more = {"weight": v2, "bias": b2, "scale": scale} if scale is not None else {}
             dw2, db2, ds = linear_backward_weight(d16, a, out_dtype=ctx.w_dtypes[1], **more)
         if need[3] or need[4]:
-            dw1, db1, _ = linear_backward_weight(du, rows, x_scale=g, x_shift=b, out_dtype=ctx.w_dtypes[0])
+            xs, xt = (g, b) if unit is None else (g * unit, b * unit)
+            dw1, db1, _ = linear_backward_weight(du, rows, x_scale=xs, x_shift=xt, out_dtype=ctx.w_dtypes[0])
         if need[0] or need[1] or need[2]:
             dh = linear_backward_input(du, v1)[0]
-            dx, dg, db = layer_norm_backward(dh, rows, None, rstd, g, add=dy, out_dtype=ctx.x_dtype)
+            dx, dg, db = layer_norm_backward(dh, rows, None, rstd if unit is None else rstd * unit, g, add=dy, out_dtype=ctx.x_dtype)
+        if unit is not None:
+            db1, dg, db = (t if t is None else t.mul_(unit) for t in (db1, dg, db))
         got = (dx, dg, db, dw1, db1, dw2, db2, ds)
         return tuple(t if n else None for t, n in zip(got, need)) + (None, None)
 
@@ -258,7 +264,9 @@ def mlp_half(x: Tensor, norm_weight: Tensor, norm_bias: Tensor, w1: Tensor, b1: 
     """The MLP half of an encoder layer (hf:372-378):  ``x + scale * (gelu(LN(x) w1^T + b1) w2^T + b2)``, differentiable in
     all its tensors.  For the backward pass it keeps the normalised rows and the hidden pre-activation in 8 bits and one
     fp32 number a row: D + H + (D + H) / 32 + 4 bytes for a row of D columns and H hidden ones, against 4 D + 2 D + 4 H for
-    x, LN(x), the pre-activation and its GELU as the products read them.  ``w1``, ``w2`` may be fp32 parameters."""
+    x, LN(x), the pre-activation and its GELU as the products read them.  ``w1``, ``w2`` may be fp32 parameters.  With fp16
+    products, the gradients between the layers carry a power of two that keeps a LayerScale of 1e-5 out of fp16's
+    subnormals; dy itself is rounded to fp16, so scale the loss where it is small."""
     if compute_dtype not in _HALF:
         raise TypeError(f"compute_dtype must be bf16 or fp16, not {compute_dtype}")
     for name, w in (("w1", w1), ("w2", w2)):

@@ -337,6 +337,12 @@ int cogaim_layernorm_bwd(const void* dy, int dy_dtype, long long lddy, const voi
                          long long lddx, float* dgamma, float* dbeta, int M, int D, void* workspace,
                          long long workspace_bytes, void* stream);
 
+/* scaled = scale * 2^p (fp32 [N]), p >= 0 bringing the largest magnitude into [2^-5, 2^-4) where it is below that (p = 0
+ * otherwise, for zeros, infinities and NaN), *unit = 2^-p.  A chain of fp16 gradients that begins with `scaled` keeps a small
+ * LayerScale out of fp16's subnormals, and leaves a factor of 16 above the gradient it began with; its ends are brought back
+ * by `unit`. */
+int cogaim_scale_unit(const float* scale, float* scaled, float* unit, int N, void* stream);
+
 /* x [M, D] to 8 bits, and back into out [M, width >= D] (columns past D are written as zero). */
 int cogaim_pack8(const void* x, int x_dtype, long long ldx, void* codes, void* exponents, int M, int D, void* stream);
 int cogaim_unpack8(const void* codes, const void* exponents, void* out, int out_dtype, long long ldo, int M, int D, int width,

@@ -115,3 +115,83 @@ def test_linear_backward_input_scale_in_fp32(M, N, K, dtype, size):
     within(dx, want, bound, "dx")
     terms = ((dy.double() * s.double()).square() @ w.double().square()).sqrt()
     assert float(((dx.double() - want) / terms).square().mean().sqrt()) <= (2.0 ** -17 if dtype == "bf16" else 2.0 ** -14)
+
+
+def mlp_tensors(M, D, H, x_dtype, layer_scale):
+    p = [rnd(M, D) * 1.5 + 0.2, 1 + 0.2 * rnd(D), 0.1 * rnd(D), rnd(H, D, scale=D ** -0.5), 0.1 * rnd(H), rnd(D, H, scale=H ** -0.5),
+         0.1 * rnd(D), layer_scale * (0.5 + 0.5 * torch.rand(D, device="cuda"))]
+    p[0] = p[0].to(x_dtype)
+    return [t.requires_grad_() for t in p]
+
+
+def mlp_plain(x, g, b, w1, b1, w2, b2, s, eps=1e-6):
+    h = torch.nn.functional.layer_norm(x, (x.shape[-1],), g, b, eps)
+    u = h @ w1.t() + b1
+    return s * ((u * torch.special.ndtr(u)) @ w2.t() + b2)
+
+
+@pytest.mark.parametrize("M,D,H,dtype,layer_scale,size", [
+    (300, 768, 520, "fp16", 1.0, 1.0), (300, 768, 520, "bf16", 1.0, 1.0), (37, 64, 256, "bf16", 1.0, 1.0), (90, 100, 130, "fp16", 0.7, 1.0),
+    (300, 256, 520, "fp16", 1e-5, 0.1), (300, 256, 520, "fp16", 1e-5, 1e-3), (20, 96, 160, "fp16", 1e-5, 1e-3), (300, 256, 520, "bf16", 1e-5, 1e-3),
+    (300, 256, 520, "fp16", 1e-4, 2e3), (300, 256, 520, "fp16", 0.02, 1e4)])
+def test_mlp_half_gradient_by_gradient(M, D, H, dtype, layer_scale, size):
+    """Each gradient of an MLP half against float64 autograd under a bound of its own, at LayerScales down to those a model
+    starts with.  With e = 0.0136, an 8-bit copy's error relative to its group's rms at the worst step, and r the half step
+    of the 16-bit type, the sources are:
+      b2      no copy: dy is exact in the type here, so only the fp32 sum
+      w2, s   a = gelu(u) from its copy: gelu' weighted over N(0, 1) against gelu's own rms is 1.03, two roundings
+      b1, b   du through gelu'(u): |gelu''| <= 0.8 against an rms slope of 0.67, so 1.2 e; W2 s, du, dh: four roundings
+      w1, g   the same and the rows' copy, e;   x's MLP part likewise
+    in the 2-norm, doubled for the fewest terms."""
+    t = DT[dtype]
+    p = mlp_tensors(M, D, H, torch.float32, layer_scale)
+    dy = rnd(M, D, scale=size).to(t).float()
+    grads = torch.autograd.grad(T.mlp_half(*p, compute_dtype=t), p, dy)
+    q = [v.detach().double().requires_grad_() for v in p]
+    want = torch.autograd.grad(mlp_plain(*q), q, dy.double())
+    e, r = 0.0136, half_step(t)
+    bound = {"w2": 1.03 * e + 2 * r, "s": 1.03 * e + 2 * r, "b1": 1.2 * e + 4 * r, "b": 1.2 * e + 4 * r, "w1": 2.2 * e + 4 * r, "g": 2.2 * e + 4 * r}
+    for name, a, v in zip("x g b w1 b1 w2 b2 s".split(), grads, want):
+        assert bool(torch.isfinite(a).all()), name
+        if name == "b2":
+            within(a, v, (M + 8) * 2 * U32 * dy.double().abs().sum(0) * p[7].double() + U32 * v.abs(), name)
+        elif name == "x":
+            # x's gradient is dy + the MLP's part: that part alone, where the sum's fp32 rounding leaves enough of it to see
+            if layer_scale >= 0.5:
+                off = float((a.double() - dy.double() - v).norm() / v.norm())
+                assert off <= 2 * (2.2 * e + 4 * r), (name, off)
+        else:
+            off = float((a.double() - v).norm() / v.norm())
+            assert off <= 2 * bound[name], (name, off, 2 * bound[name])
+
+
+@pytest.mark.parametrize("top,p", [(1.0, 0), (2.0 ** -4, 0), (0.0624, 0), (2.0 ** -5, 0), (0.031, 1), (1e-5, 12), (2.0 ** -126, 121), (0.0, 0), (float("inf"), 0), (float("nan"), 0)])
+@pytest.mark.parametrize("N", [1, 64, 1000, 20000])
+def test_scale_unit(N, top, p):
+    scale = torch.full((N,), 0.25 * top, device="cuda")
+    scale[N // 2] = -top
+    scaled, unit = T._ops().scale_unit(scale)
+    assert torch.equal(unit.cpu(), torch.tensor([2.0 ** -p])) and torch.equal(scaled.nan_to_num(7.0), (scale * 2.0 ** p).nan_to_num(7.0))
+
+
+def test_mlp_half_fp16_in_a_graph():
+    """The carried power of two is found on the device: a captured backward pass follows the LayerScale of each replay."""
+    p = mlp_tensors(50, 96, 160, torch.float32, 1e-5)
+    dy = rnd(50, 96)
+    step = lambda: torch.autograd.grad(T.mlp_half(*p, compute_dtype=torch.float16), p, dy)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for size in (1e-5, 1.0, 1e-3):
+        with torch.no_grad():
+            p[7].copy_(size * (0.5 + 0.5 * torch.rand(96, device="cuda")))
+            p[0].mul_(0.9)
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), size
