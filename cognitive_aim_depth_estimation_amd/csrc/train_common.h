@@ -8,6 +8,9 @@ namespace train {
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4v __attribute__((ext_vector_type(4)));
 
+// A launch counts its work-items along x in 32 bits; kernels whose grid grows with the rows take no more in one launch.
+constexpr long long MAX_ITEMS = 0xffffffffLL;
+
 enum { DT_BF16 = 0, DT_FP16 = 1, DT_FP32 = 2 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2 };
 constexpr int GROUP = 32;                       // columns of a row that share one 8-bit step

@@ -278,11 +278,12 @@ struct EpiPart {                             // fp32 partial sums [split][M][Np]
   }
 };
 
-// adds the parts of eight columns in split order and applies the epilogue; four neighbouring threads hold a group
+// adds the parts of eight columns in split order and applies the epilogue; four neighbouring threads hold a group.  `first`:
+// the first of the launch's threads among all of them.
 template <class Epi>
-__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int M, int N, int Np, Epi epi) {
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int M, int N, int Np, long long first, Epi epi) {
   const int per_row = (int)groups_of(N) * 4;
-  const long long i = blockIdx.x * 256LL + threadIdx.x;
+  const long long i = first + blockIdx.x * 256LL + threadIdx.x;
   const long long row = i / per_row;
   const int n = (int)(i - row * per_row) * 8;
   const int m = row < M ? (int)row : M;                       // past the end: dropped by the epilogue
@@ -473,6 +474,8 @@ const TileCost TILE_COST[TILES] = {{256, 256, 256, 1.50f, 4.5f, 1.20f}, {192, 25
 // read back once at 5 TB/s.
 constexpr float JOIN_FIXED = 5.f, JOIN_PER_BYTE = 1.f / 5.0e6f;
 
+int tile_threads(int tile) { return tile == TILE_128 || tile == TILE_64 ? 256 : 512; }
+
 struct Shape { int tile, tiles_m, tiles_n, splits, kt_per_split; };
 
 // `joined`: the second kernel runs whether or not the sum is split; `ragged`: it does but for the smallest tile
@@ -488,6 +491,7 @@ Shape shape_of(int M, int N, int K, bool a_along_k, bool joined, bool ragged) {
       if (want > 1 && nk < 2 * want) break;
       const int per = (nk + want - 1) / want, splits = (nk + per - 1) / per;            // no part is empty
       const double blocks = (double)tm * tn * splits;
+      if (blocks * tile_threads(t) > (double)MAX_ITEMS) continue;           // (256 rows of a narrow result to a tile: any M)
       const double rounds = blocks <= c.slots ? 1.0 : (double)((long long)((blocks + c.slots - 1) / c.slots));
       float us = (float)rounds * (c.fixed + per * (blocks * 2 <= c.slots ? c.alone_k : c.per_k));
       if (splits > 1 || joined || (ragged && t != TILE_64)) us += JOIN_FIXED + JOIN_PER_BYTE * 8.f * splits * (float)M * (float)N;
@@ -536,7 +540,7 @@ int run_copies(Side& a, Side& b, int dt, char*& ws, hipStream_t st) {
 template <class T, bool AKC, bool BKC, bool FAST = true, class Epi>
 int launch_gemm(const Operands& g, int tile, const Epi& e, hipStream_t st) {
   const long long blocks = (long long)g.tiles_m * g.tiles_n * g.splits;
-  if (blocks <= 0 || blocks >= (1LL << 31)) return COGAIM_EINVAL;
+  if (blocks <= 0 || blocks * tile_threads(FAST ? tile : TILE_64) > MAX_ITEMS) return COGAIM_EINVAL;
 #define TRAIN_LAUNCH(TL_) hipLaunchKernelGGL((train_gemm_kernel<T, AKC, BKC, TL_, Epi, FAST>), dim3((unsigned)blocks), dim3(TL_::NW * 64), 0, st, g, e)
   if constexpr (!FAST) TRAIN_LAUNCH(T64);
   else if (tile == TILE_256) TRAIN_LAUNCH(T256);
@@ -564,9 +568,11 @@ int product(const Operands& g, const Shape& s, const Epi& e, float* part, hipStr
     const int rc = launch_gemm<T, AKC, BKC>(one, s.tile, EpiPart{part + (size_t)p * s.splits * g.M * Np, g.M, Np}, st);
     if (rc) return rc;
   }
-  const long long threads = (long long)g.M * groups_of(g.N) * 4;
-  if ((threads + 255) / 256 >= (1LL << 31)) return COGAIM_EINVAL;
-  hipLaunchKernelGGL((join_kernel<Epi>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, part, s.splits * parts, g.M, g.N, Np, e);
+  const long long threads = (long long)g.M * groups_of(g.N) * 4, most = MAX_ITEMS & ~255LL;
+  for (long long first = 0; first < threads; first += most) {
+    const long long n = threads - first < most ? threads - first : most;
+    hipLaunchKernelGGL((join_kernel<Epi>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, s.splits * parts, g.M, g.N, Np, first, e);
+  }
   return COGAIM_LAUNCH_CHECK();
 }
 

@@ -588,7 +588,21 @@ int ln_bwd_blocks(int M, int D) {
   const long long want = ((long long)M + rpb - 1) / rpb;
   return (int)(want < most ? want : most);
 }
+// rows of the forward kernel that one launch takes: 64 threads to 1024 threads each
+int ln_fwd_rows(int D) { return (int)(MAX_ITEMS / (D <= 1024 ? 64 : D <= 4096 ? 256 : 1024)) & ~255; }
 template <int XDT> void run_ln_fwd(const LnFwd& a, hipStream_t st) {
+  const int most = ln_fwd_rows(a.D);
+  if (a.M > most) {                             // the rows in turn
+    const size_t x = dt_size(XDT), y = dt_size(a.y_dt), g = groups_of(a.D);
+    for (long long m = 0; m < a.M; m += most) {
+      LnFwd p = a;
+      p.M = (int)(a.M - m < most ? a.M - m : most);
+      p.x = (const char*)a.x + m * a.ldx * x; p.y = (char*)a.y + m * a.ldy * y; p.mean += m; p.rstd += m;
+      if (a.codes) { p.codes += m * a.D; p.bytes += m * g; }
+      run_ln_fwd<XDT>(p, st);
+    }
+    return;
+  }
 #define LN_LAUNCH(V_, TPR_, NCH_, RPB_, TH_)                                                                              \
   do {                                                                                                                    \
     const dim3 grid((unsigned)(((long long)a.M + RPB_ - 1) / RPB_));                                                      \

@@ -195,3 +195,37 @@ def test_mlp_half_fp16_in_a_graph():
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), size
+
+
+@pytest.mark.parametrize("M,D", [((1 << 26) + 77, 3), ((1 << 22) + 9, 4100)])
+def test_layer_norm_forward_past_one_launch(M, D):
+    """More rows than a launch has work-items for (64 a row, 1024 in the second case): the first ones, those where the second
+    launch takes over and the last ones against the same rows alone."""
+    x = torch.empty(M, D, device="cuda", dtype=torch.bfloat16)
+    at = (1 << 26 if D == 3 else 1 << 22) - 256                    # the first row of the second launch, at or just ahead of this
+    parts = [slice(0, 70), slice(at - 70, at + 260), slice(M - 70, M)]
+    w, b = 1 + 0.1 * rnd(D), rnd(D)
+    for p in parts:
+        x[p] = rnd(len(range(*p.indices(M))), D, dtype=torch.bfloat16)
+    y, mean, rstd, saved = T.layer_norm_forward(x, w, b, checkpoint=True)
+    for p in parts:
+        y2, mean2, rstd2, saved2 = T.layer_norm_forward(x[p].clone(), w, b, checkpoint=True)
+        assert torch.equal(y[p], y2) and torch.equal(mean[p], mean2) and torch.equal(rstd[p], rstd2)
+        assert torch.equal(saved.codes[p], saved2.codes) and torch.equal(saved.exponents[p], saved2.exponents)
+
+
+def test_linear_past_one_launch():
+    """2^30 rows of a ragged result: more work-items than a launch has in the tiles of 64 rows and in the join kernel."""
+    M, N, K = (1 << 30) + 5, 9, 8
+    w = rnd(N, K, dtype=torch.bfloat16)
+    x = torch.empty(M, K, device="cuda", dtype=torch.bfloat16)
+    parts = [slice(0, 300), slice((1 << 30) - 300, M)]
+    for p in parts:
+        x[p] = rnd(len(range(*p.indices(M))), K, dtype=torch.bfloat16)
+    y, _ = T.linear_forward(x, w)
+    for p in parts:
+        u = x[p].double() @ w.double().t()
+        bound = (K + 8) * 2 * U32 * (x[p].double().abs() @ w.double().abs().t())
+        within(y[p], u, bound + half_step(y.dtype) * (u.abs() + bound) + least(y.dtype))
+    del x, y
+    torch.cuda.empty_cache()
