@@ -68,6 +68,7 @@ SIGNATURES = {
     "cogaim_pack8": [P, I, LL, P, P, I, I, P],
     "cogaim_unpack8": [P, P, P, I, LL, I, I, I, P],
     "cogaim_activation_bwd": [P, I, LL, P, P, P, I, LL, I, I, I, P],
+    "cogaim_activation_bwd_from": [P, I, LL, P, I, LL, P, I, LL, I, I, I, P],
     "cogaim_linear_fwd_workspace_bytes": [P],
     "cogaim_linear_fwd": [P, P, LL, P],
     "cogaim_linear_bwd_input_workspace_bytes": [P],
@@ -95,7 +96,7 @@ class LinearFwdDesc(C.Structure):
     """cogaim_linear_fwd_desc of include/cogaim.h."""
     _fields_ = ([(n, P) for n in ("x", "w", "bias", "scale", "residual", "y", "codes", "exponents")]
                 + [(n, LL) for n in ("ldx", "ldw", "ldr", "ldy")]
-                + [(n, I) for n in ("M", "N", "K", "dtype", "residual_dtype", "y_dtype", "activation", "reserved")])
+                + [(n, I) for n in ("M", "N", "K", "dtype", "residual_dtype", "y_dtype", "activation", "extended")] + [("pre", P)])
 
 
 class LinearBwdInputDesc(C.Structure):

@@ -20,7 +20,8 @@ enum { ACT_NONE, ACT_RELU, ACT_GELU };
   X(cogaim_pack8) X(cogaim_unpack8) X(cogaim_activation_bwd) X(cogaim_layernorm_train_fwd) X(cogaim_layernorm_bwd)        \
   X(cogaim_layernorm_bwd_workspace_bytes) X(cogaim_linear_fwd) X(cogaim_linear_fwd_workspace_bytes)                       \
   X(cogaim_linear_bwd_input) X(cogaim_linear_bwd_input_workspace_bytes) X(cogaim_linear_bwd_weight)                       \
-  X(cogaim_linear_bwd_weight_workspace_bytes) X(cogaim_scale_unit)
+  X(cogaim_linear_bwd_weight_workspace_bytes) X(cogaim_scale_unit)       \
+  X(cogaim_activation_bwd_from)
 #define DECLARE(n) decltype(&::n) n##_;
 ENTRIES(DECLARE)
 PyObject* error_class = nullptr;
@@ -165,12 +166,24 @@ Tensor unpack8(const Tensor& codes, const Tensor& exponents, at::ScalarType dtyp
   return out;
 }
 
-Tensor activation_backward(const Tensor& dy, const Tensor& codes, const Tensor& exponents, const std::string& name, OptType dtype) {
+Tensor activation_backward(const Tensor& dy, const OptTensor& u, const OptTensor& codes, const OptTensor& exponents, const std::string& name, OptType dtype) {
   floats(dy, "dy");
   const int act = activation(name);
   TORCH_CHECK_VALUE(act != ACT_NONE, "activation must be 'relu' or 'gelu'");
   const at::ScalarType t = out_type(dtype, dy.scalar_type());
-  const Saved s = saved8(codes, exponents, "saved", dy.sizes(), dy.device());
+  if (u) {
+    floats(*u, "saved");
+    same_shape(*u, "saved", dy.sizes(), dy.device());
+    const int D = narrow(dy.size(-1), "dy");
+    const On on(dy.device());
+    const Tensor out = fresh(dy, dy.sizes(), t);
+    const Rows v = rows(dy), uv = rows(*u);
+    if (v.n)
+      check(cogaim_activation_bwd_from_(v.p, code(dy.scalar_type()), v.ld, uv.p, code(u->scalar_type()), uv.ld, out.data_ptr(), code(t), D, act, v.n, D,
+                                        on.stream), "cogaim_activation_bwd_from");
+    return out;
+  }
+  const Saved s = saved8(*codes, *exponents, "saved", dy.sizes(), dy.device());
   const int D = narrow(dy.size(-1), "dy");
   const On on(dy.device());
   const Tensor out = fresh(dy, dy.sizes(), t);
@@ -273,8 +286,9 @@ void matrix(const Tensor& w) {
   TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) >= 1, "weight must be a matrix");
 }
 
-std::tuple<Tensor, OptTensor, OptTensor> linear_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, const std::string& name,
-                                                        const OptTensor& scale, const OptTensor& residual, OptType dtype, bool checkpoint) {
+std::tuple<Tensor, OptTensor, OptTensor, OptTensor> linear_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, const std::string& name,
+                                                                   const OptTensor& scale, const OptTensor& residual, OptType dtype, bool checkpoint,
+                                                                   bool pre_activation) {
   halves(x, "x");
   matrix(weight);
   const int act = activation(name);
@@ -283,6 +297,7 @@ std::tuple<Tensor, OptTensor, OptTensor> linear_forward(const Tensor& x, const T
   TORCH_CHECK_VALUE(x.size(-1) == K && weight.scalar_type() == x.scalar_type() && weight.device() == dev, "x ", x.sizes(), " ", x.scalar_type(), " on ",
                     dev, " does not go with weight ", weight.sizes(), " ", weight.scalar_type(), " on ", weight.device());
   TORCH_CHECK_VALUE(!scale || act == ACT_NONE, "scale goes with activation 'none'");
+  TORCH_CHECK_VALUE(!checkpoint || !pre_activation, "checkpoint and pre_activation are two ways to keep one thing");
   const OptTensor b = vec(bias, "bias", N, dev), s = vec(scale, "scale", N, dev);
   const at::ScalarType t = out_type(dtype, x.scalar_type());
   const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
@@ -293,11 +308,12 @@ std::tuple<Tensor, OptTensor, OptTensor> linear_forward(const Tensor& x, const T
   }
   const On on(dev);
   const Tensor y = fresh(x, shape, t);
-  OptTensor codes, exponents;
+  OptTensor codes, exponents, pre;
   if (checkpoint) {
     const Saved k = fresh8(x, lead, N);
     codes = k.codes; exponents = k.exponents;
   }
+  if (pre_activation) pre = fresh(x, shape, x.scalar_type());
   const Rows xv = rows(x);
   if (xv.n) {
     const Rows wv = rows(weight), rv = residual ? rows(*residual) : Rows{Tensor(), nullptr, 0, 0};
@@ -306,10 +322,10 @@ std::tuple<Tensor, OptTensor, OptTensor> linear_forward(const Tensor& x, const T
     d.codes = ptr(codes); d.exponents = ptr(exponents);
     d.ldx = leading(xv.ld, "x"); d.ldw = leading(wv.ld, "weight"); d.ldr = leading(rv.ld, "residual"); d.ldy = leading(N, "y");
     d.M = xv.n; d.N = N; d.K = K; d.dtype = code(x.scalar_type()); d.residual_dtype = residual ? code(residual->scalar_type()) : 0;
-    d.y_dtype = code(t); d.activation = act;
+    d.y_dtype = code(t); d.activation = act; d.extended = 1; d.pre = ptr(pre);
     run(d, cogaim_linear_fwd_workspace_bytes_, cogaim_linear_fwd_, "cogaim_linear_fwd", x, on.stream);
   }
-  return {y, codes, exponents};
+  return {y, codes, exponents, pre};
 }
 
 std::tuple<Tensor, OptTensor> linear_backward_input(const Tensor& dy, const Tensor& weight, const std::string& name, const OptTensor& codes,

@@ -574,6 +574,36 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const void* __restrict__ d
   }
 }
 
+// the same with u itself, of a type known at run time
+template <int DT, int V, bool EVEN>
+__global__ __launch_bounds__(256) void act_bwd_from_kernel(const void* __restrict__ dy, long long lddy, const void* __restrict__ u, int u_dt, long long ldu,
+                                                           void* __restrict__ du, int du_dt, long long lddu, int act, int M, int D) {
+  for (Walk w((unsigned)(D + V - 1) / V); w.row < (unsigned long long)M; w.step()) {
+    const long long row = (long long)w.row;
+    const int c = (int)w.run * V;
+    Run<DT, V> r;
+    Run<DT_FP32, V> q;
+    if (EVEN || row + V <= M) {
+      r = load_run<DT, V, true>(dy, row * lddy, c, D);
+      q = load_any<V, true>(u, u_dt, row * ldu, c, D);
+    } else {
+      r = load_run<DT, V, false>(dy, row * lddy, c, D);
+      q = load_any<V, false>(u, u_dt, row * ldu, c, D);
+    }
+    float v[V], g[V];
+    cvt_words<V>(q.w, u_dt, v);
+    cvt_run<DT, V>(r, g);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float value, slope;
+      if (act == ACT_GELU) gelu_both(v[j], value, slope);
+      else slope = relu_slope(v[j]);
+      g[j] *= slope;
+    }
+    store_any<V, EVEN>(du, du_dt, row * lddu, c, D, g);
+  }
+}
+
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 bool dt_ok(int dt) { return dt >= 0 && dt <= 2; }
 unsigned blocks_for(unsigned long long threads) {
@@ -745,6 +775,17 @@ int cogaim_activation_bwd(const void* dy, int dy_dtype, long long lddy, const vo
     return COGAIM_EINVAL;
   BY_TYPE(dy_dtype, D, act_bwd_kernel, dim3(blocks_for((unsigned long long)M * (D / (dy_dtype == DT_FP32 ? 4LL : 8LL) + 1))), dim3(256), 0, (hipStream_t)stream, dy, lddy,
           (const signed char*)codes, (const unsigned char*)exponents, du, du_dtype, lddu, activation, M, D);
+  return COGAIM_LAUNCH_CHECK();
+}
+
+int cogaim_activation_bwd_from(const void* dy, int dy_dtype, long long lddy, const void* u, int u_dtype, long long ldu, void* du,
+                               int du_dtype, long long lddu, int activation, int M, int D, void* stream) {
+  if (M <= 0 || D <= 0 || D > MAX_D || !dt_ok(dy_dtype) || !dt_ok(u_dtype) || !dt_ok(du_dtype) || lddy < D || ldu < D || lddu < D || !dy || !u || !du ||
+      (activation != ACT_RELU && activation != ACT_GELU) || !aligned(dy, dt_size(dy_dtype)) || !aligned(u, dt_size(u_dtype)) ||
+      !aligned(du, dt_size(du_dtype)))
+    return COGAIM_EINVAL;
+  BY_TYPE(dy_dtype, D, act_bwd_from_kernel, dim3(blocks_for((unsigned long long)M * (D / (dy_dtype == DT_FP32 ? 4LL : 8LL) + 1))), dim3(256), 0, (hipStream_t)stream,
+          dy, lddy, u, u_dtype, ldu, du, du_dtype, lddu, activation, M, D);
   return COGAIM_LAUNCH_CHECK();
 }
 

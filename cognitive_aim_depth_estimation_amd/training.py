@@ -89,10 +89,13 @@ def unpack8(saved: Checkpoint8, dtype: torch.dtype = torch.float32) -> Tensor:
     return (_host or _ops()).unpack8(codes, exponents, dtype)
 
 
-def activation_backward(dy: Tensor, saved: Checkpoint8, activation: str, out_dtype: Optional[torch.dtype] = None) -> Tensor:
-    """``dy * act'(u)`` with ``u`` kept in 8 bits; activation "relu" or "gelu"."""
-    codes, exponents = _checkpoint(saved, "saved")
-    return (_host or _ops()).activation_backward(dy, codes, exponents, activation, out_dtype)
+def activation_backward(dy: Tensor, saved: Union[Tensor, Checkpoint8], activation: str, out_dtype: Optional[torch.dtype] = None) -> Tensor:
+    """``dy * act'(u)`` with ``u`` itself or its 8-bit copy; activation "relu" or "gelu".  In 8 bits a u of under half its
+    group's step is zero, and ReLU's gradient stops there: about 1 % of the positive ones of normally distributed rows."""
+    u, codes, exponents = (None, *saved) if isinstance(saved, Checkpoint8) else (saved, None, None)
+    if u is None and codes is None:
+        raise TypeError("saved must be a tensor or a Checkpoint8")
+    return (_host or _ops()).activation_backward(dy, u, codes, exponents, activation, out_dtype)
 
 
 # ---- layer norm --------------------------------------------------------------------------------------------------
@@ -118,12 +121,13 @@ def layer_norm_backward(dy: Tensor, saved: Union[Tensor, Checkpoint8], mean: Opt
 # ---- linear layers -----------------------------------------------------------------------------------------------
 def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: str = "none",
                    scale: Optional[Tensor] = None, residual: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None,
-                   checkpoint: bool = False) -> Tuple[Tensor, Optional[Checkpoint8]]:
+                   checkpoint: bool = False, pre_activation: bool = False) -> Tuple[Tensor, Union[None, Checkpoint8, Tensor]]:
     """``(y, saved)`` for ``x [..., K]`` and ``weight [N, K]`` of one 16-bit type:  with ``u = x weight^T + bias``,
     ``y = act(u) + residual``, or ``y = scale * u + residual`` (scale: LayerScale, only without an activation).  ``y`` is of
-    type ``out_dtype`` (default: x's); with ``checkpoint``, ``saved`` is u in 8 bits, packed in the product's epilogue."""
-    y, codes, exponents = (_host or _ops()).linear_forward(x, weight, bias, activation, scale, residual, out_dtype, checkpoint)
-    return y, Checkpoint8(codes, exponents) if checkpoint else None
+    type ``out_dtype`` (default: x's); with ``checkpoint``, ``saved`` is u in 8 bits, with ``pre_activation`` u in x's type, both
+    from the product's epilogue."""
+    y, codes, exponents, pre = (_host or _ops()).linear_forward(x, weight, bias, activation, scale, residual, out_dtype, checkpoint, pre_activation)
+    return y, Checkpoint8(codes, exponents) if checkpoint else pre
 
 
 def linear_backward_input(dy: Tensor, weight: Tensor, activation: str = "none", saved: Optional[Checkpoint8] = None,
@@ -186,8 +190,11 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, scale, residual, activation, out_dtype, checkpoint):
         w = weight if weight.dtype == x.dtype else weight.to(x.dtype)
-        y, pre = linear_forward(x, w, bias, activation, scale, residual, out_dtype, checkpoint=activation != "none")
+        active = activation != "none"
+        y, pre = linear_forward(x, w, bias, activation, scale, residual, out_dtype, active and checkpoint, active and not checkpoint)
         kept = pack8(x) if checkpoint else None
+        if not checkpoint:
+            pre = (pre, None)
         ctx.activation, ctx.kept8, ctx.x_dtype, ctx.w_dtype = activation, checkpoint, x.dtype, weight.dtype
         ctx.res_dtype = None if residual is None else residual.dtype
         ctx.has = (bias is not None, scale is not None)
@@ -200,7 +207,7 @@ class _Linear(torch.autograd.Function):
         w, bias, scale, pc, pe, xa, xb = ctx.saved_tensors
         need = ctx.needs_input_grad
         if ctx.activation != "none":
-            du = activation_backward(dy, Checkpoint8(pc, pe), ctx.activation, ctx.x_dtype)
+            du = activation_backward(dy, Checkpoint8(pc, pe) if ctx.kept8 else pc, ctx.activation, ctx.x_dtype)
         else:
             du = dy.to(ctx.x_dtype)
         dx = linear_backward_input(du, w, scale=scale)[0] if need[0] else None
@@ -216,7 +223,8 @@ class _Linear(torch.autograd.Function):
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: str = "none", scale: Optional[Tensor] = None,
            residual: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None, checkpoint: bool = False) -> Tensor:
     """Differentiable ``linear_forward``.  ``weight`` may be an fp32 parameter: it is rounded to x's type for the products
-    and its gradient is fp32.  A pre-activation is always kept in 8 bits; ``checkpoint`` keeps x in 8 bits as well."""
+    and its gradient is fp32.  The backward pass reads x and, with an activation, the pre-activation, kept in x's type or,
+    with ``checkpoint``, in 8 bits (where ReLU's gradient stops at values under half a step: ``activation_backward``)."""
     return _Linear.apply(x, weight, bias, scale, residual, activation, out_dtype, checkpoint)
 
 

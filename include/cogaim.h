@@ -348,17 +348,24 @@ int cogaim_pack8(const void* x, int x_dtype, long long ldx, void* codes, void* e
 int cogaim_unpack8(const void* codes, const void* exponents, void* out, int out_dtype, long long ldo, int M, int D, int width,
                    void* stream);
 
-/* du = dy * act'(u), u from its 8-bit copy; activation 1 ReLU, 2 erf GELU. */
+/* du = dy * act'(u), u from its 8-bit copy; activation 1 ReLU, 2 erf GELU.  A u of under half its group's step is zero in
+ * that copy, and ReLU's gradient stops there (about 1 % of the positive ones of normally distributed rows). */
 int cogaim_activation_bwd(const void* dy, int dy_dtype, long long lddy, const void* codes, const void* exponents, void* du,
                           int du_dtype, long long lddu, int activation, int M, int D, void* stream);
+
+/* The same with u [M, D] itself, of its own type. */
+int cogaim_activation_bwd_from(const void* dy, int dy_dtype, long long lddy, const void* u, int u_dtype, long long ldu, void* du,
+                               int du_dtype, long long lddu, int activation, int M, int D, void* stream);
 
 /* nn.Linear with all that may follow it (hf:199-213, 246-252, 277-278, 286-297, 370-378):
  *   u = x W^T + bias,  y = act(u) + residual  or  y = u * scale + residual,  and u in 8 bits unless codes is NULL.
  * x [M,K], w [N,K] of `dtype` (0 or 1), bias, scale fp32 [N] (NULL: none), residual and y [M,N] of their own types (y may
- * be the residual).  activation 0 none, 1 ReLU, 2 erf GELU; scale (LayerScale) only without one. */
+ * be the residual).  activation 0 none, 1 ReLU, 2 erf GELU; scale (LayerScale) only without one.  extended 1: the fields
+ * behind it are there; pre (NULL: none) takes u in `dtype` too, [M,N] contiguous. */
 typedef struct {
   const void* x; const void* w; const float* bias; const float* scale; const void* residual; void* y; void* codes; void* exponents;
-  long long ldx, ldw, ldr, ldy; int M, N, K, dtype, residual_dtype, y_dtype, activation, reserved;
+  long long ldx, ldw, ldr, ldy; int M, N, K, dtype, residual_dtype, y_dtype, activation, extended;
+  void* pre;
 } cogaim_linear_fwd_desc;
 long long cogaim_linear_fwd_workspace_bytes(const cogaim_linear_fwd_desc* desc);
 int cogaim_linear_fwd(const cogaim_linear_fwd_desc* desc, void* workspace, long long workspace_bytes, void* stream);

@@ -229,3 +229,87 @@ def test_linear_past_one_launch():
         within(y[p], u, bound + half_step(y.dtype) * (u.abs() + bound) + least(y.dtype))
     del x, y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 40, 24), (5, 333, 40), (70, 33, 41), (300, 520, 72), (2600, 1000, 40)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_linear_relu_border_is_exact(M, N, K, dtype, residual):
+    """Without checkpoint, ReLU's gradient passes wherever the pre-activation is positive, however small it is beside its
+    neighbours.  Operands are multiples of 1/8, so the pre-activation has no rounding that could move its sign."""
+    t = DT[dtype]
+    x = (torch.randint(-3, 4, (M, K), device="cuda").float()).to(t).requires_grad_()
+    w = (torch.randint(-3, 4, (N, K), device="cuda").float() / 8).to(t).requires_grad_()
+    b = (torch.randint(-3, 4, (N,), device="cuda").float() / 8).requires_grad_()
+    with torch.no_grad():
+        x[:, 0] = 0
+        w[::7], b[::7] = 0, 2.0 ** -7          # small positive values in groups of large ones
+        w[3::7, 0], b[3::7] = 3, 0
+    res = rnd(M, N).requires_grad_() if residual else None
+    y = T.linear(x, w, b, "relu", residual=res)
+    dy = rnd(M, N, dtype=y.dtype)
+    args = (x, w, b) + ((res,) if residual else ())
+    got = torch.autograd.grad(y, args, dy)
+    X, W, B = x.detach().double(), w.detach().double(), b.detach().double()
+    u = X @ W.t() + B
+    du = dy.double() * (u > 0)
+    want = du @ W, du.t() @ X, du.sum(0)
+    chain = [(N + 8) * 2 * U32 * (du.abs() @ W.abs()), (M + 8) * 2 * U32 * (du.abs().t() @ X.abs()), (M + 8) * 2 * U32 * du.abs().sum(0)]
+    for i, name in enumerate(("dx", "dw", "db")):
+        h = half_step(got[i].dtype)
+        within(got[i], want[i], chain[i] + h * (want[i].abs() + chain[i]) + least(got[i].dtype), name)
+    if residual:
+        assert torch.equal(got[3], dy.to(res.dtype))
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 40, 24), (70, 33, 41), (300, 520, 72)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_linear_gelu_keeps_its_precision(M, N, K, dtype):
+    """Without checkpoint the pre-activation is kept in x's type: the slope is off by |gelu''| <= 0.8 times half a step of u."""
+    t = DT[dtype]
+    x, w, b = rnd(M, K, dtype=t).requires_grad_(), rnd(N, K, dtype=t, scale=K ** -0.5).requires_grad_(), rnd(N).requires_grad_()
+    y = T.linear(x, w, b, "gelu", out_dtype=torch.float32)
+    dy = rnd(M, N)
+    db = torch.autograd.grad(y, b, dy)[0]
+    u = x.detach().double() @ w.detach().double().t() + b.detach().double()
+    f, h = slope(u, "gelu"), half_step(t)
+    du, d = dy.double() * f, dy.double().abs()
+    off = d * (0.8 * (h * u.abs() + least(t) + (K + 8) * 2 * U32 * (x.detach().double().abs() @ w.detach().double().abs().t() + b.detach().double().abs())) + 4e-7)
+    within(db, du.sum(0), (off * (1 + h) + h * du.abs() + least(t)).sum(0) + (M + 8) * 2 * U32 * du.abs().sum(0), "db")
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 64, 64), (3, 577, 588), (130, 256, 768), (257, 1000, 264), (16, 2052, 1000), (40, 333, 5001), (2600, 4096, 264), (20000, 520, 264)])
+@pytest.mark.parametrize("dtype,activation,residual,out", [("bf16", "gelu", None, "bf16"), ("fp16", "relu", "fp32", "fp32"), ("fp16", "none", None, "fp16")])
+def test_linear_forward_pre_activation(M, N, K, dtype, activation, residual, out):
+    t = DT[dtype]
+    x, w, b = rnd(M, K, dtype=t), rnd(N, K, dtype=t, scale=K ** -0.5), rnd(N)
+    r = rnd(M, N, dtype=DT[residual]) if residual else None
+    y, pre = T.linear_forward(x, w, b, activation, residual=r, out_dtype=DT[out], pre_activation=True)
+    assert pre.dtype == t and torch.equal(y, T.linear_forward(x, w, b, activation, residual=r, out_dtype=DT[out])[0])
+    u = x.double() @ w.double().t() + b.double()
+    bound = (K + 8) * 2 * U32 * (x.double().abs() @ w.double().abs().t()) + 2 * U32 * u.abs()
+    within(pre, u, bound + half_step(t) * (u.abs() + bound) + least(t))
+    if activation == "none" and not residual:
+        assert torch.equal(pre, y)
+
+
+@pytest.mark.parametrize("M,D", [(1, 1), (7, 33), (40, 1024), (300, 577), (5, 4104)])
+@pytest.mark.parametrize("u_dtype,dy_dtype,du_dtype", [("bf16", "bf16", "bf16"), ("fp16", "fp32", "fp16"), ("fp32", "bf16", "fp32"), ("fp32", "fp16", "bf16")])
+@pytest.mark.parametrize("name", ["relu", "gelu"])
+def test_activation_backward_of_a_tensor(M, D, u_dtype, dy_dtype, du_dtype, name):
+    wide = 2 * rnd(M, D + 3, dtype=DT[u_dtype])
+    for u in (wide[:, :D], wide[:, 1:D + 1].contiguous()):
+        dy = rnd(M, D, dtype=DT[dy_dtype])
+        got = T.activation_backward(dy, u, name, DT[du_dtype])
+        want = dy.double() * slope(u.double(), name)
+        bound = dy.double().abs() * 3e-7 + 4 * U32 * want.abs()
+        within(got, want, bound + half_step(DT[du_dtype]) * (want.abs() + bound) + least(DT[du_dtype]))
+    dead = torch.full((M, D), float("nan"), device="cuda", dtype=DT[u_dtype])
+    assert bool(torch.isnan(T.activation_backward(dy, dead, name)).all())
+
+
+def test_activation_backward_of_no_rows():
+    e = torch.empty(0, 5, device="cuda", dtype=torch.bfloat16)
+    assert T.activation_backward(e, e, "relu").shape == (0, 5)
+    y, pre = T.linear_forward(e, rnd(24, 5, dtype=torch.bfloat16), pre_activation=True)
+    assert y.shape == pre.shape == (0, 24)
