@@ -313,3 +313,24 @@ def test_activation_backward_of_no_rows():
     assert T.activation_backward(e, e, "relu").shape == (0, 5)
     y, pre = T.linear_forward(e, rnd(24, 5, dtype=torch.bfloat16), pre_activation=True)
     assert y.shape == pre.shape == (0, 24)
+
+
+@pytest.mark.parametrize("M", [3, 200])
+def test_gelu_tails(M):
+    """GELU in fp32 results: no further from the truth than the fp32 erf form where that is accurate (2.7e-8 rms over
+    [-2, 2], here plus the roundings of u), and gone where the normal tail is."""
+    N = 64
+    x = torch.linspace(-2, 2, M * 64, device="cuda").view(M, 64).to(torch.bfloat16)
+    w = torch.eye(N, 64, device="cuda", dtype=torch.bfloat16)
+    y = T.linear_forward(x, w, activation="gelu", out_dtype=torch.float32)[0].double()
+    off = y - act(x.double(), "gelu")
+    assert float(off.square().mean().sqrt()) <= 3e-8 and float(off.abs().max()) <= 1.5e-7
+    far = -torch.linspace(6, 60, M * 64, device="cuda").view(M, 64).to(torch.bfloat16)
+    y = T.linear_forward(far, w, activation="gelu", out_dtype=torch.float32)[0].double()
+    want = act(far.double(), "gelu")
+    assert bool(((y - want).abs() <= 0.05 * want.abs() + 1e-10).all()) and float(y[far < -10].abs().max()) <= 1e-20
+    saved = T.pack8(far.float())
+    dx, a = T.linear_backward_input(torch.ones(M, 64, device="cuda", dtype=torch.bfloat16), w, "gelu", saved, out_dtype=torch.float32, want_activation=True)
+    v = decode(saved.codes, saved.exponents)
+    within(a, act(v, "gelu"), 0.05 * act(v, "gelu").abs() + 1e-10)
+    within(dx, slope(v, "gelu"), 1e-7 + 0 * v)
