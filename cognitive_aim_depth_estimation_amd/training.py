@@ -225,6 +225,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     """Differentiable ``linear_forward``.  ``weight`` may be an fp32 parameter: it is rounded to x's type for the products
     and its gradient is fp32.  The backward pass reads x and, with an activation, the pre-activation, kept in x's type or,
     with ``checkpoint``, in 8 bits (where ReLU's gradient stops at values under half a step: ``activation_backward``)."""
+    if weight.dtype not in _FLOATS:
+        raise TypeError(f"weight must be bf16, fp16 or fp32, not {weight.dtype}")
     return _Linear.apply(x, weight, bias, scale, residual, activation, out_dtype, checkpoint)
 
 

@@ -26,6 +26,7 @@ def raw(name, *args):
     (lambda: T.activation_backward(t(2, 3), t(2, 3), "none"), ValueError, "relu"),
     (lambda: T.activation_backward(t(2, 3), None, "relu"), TypeError, "Checkpoint8"),
     (lambda: T.linear_forward(t(2, 3), t(4, 3), checkpoint=True, pre_activation=True), ValueError, "two ways"),
+    (lambda: T.linear(t(2, 3), t(4, 3, dtype=torch.float64)), TypeError, "weight must be"),
     (lambda: T._ops().scale_unit(t(4, dtype=torch.float32)), RuntimeError, "no CPU path"),
     (lambda: T._ops().scale_unit(t(4)), ValueError, "float32"),
     (lambda: T._ops().scale_unit(t(0, dtype=torch.float32)), ValueError, "vector"),
