@@ -334,3 +334,18 @@ def test_gelu_tails(M):
     v = decode(saved.codes, saved.exponents)
     within(a, act(v, "gelu"), 0.05 * act(v, "gelu").abs() + 1e-10)
     within(dx, slope(v, "gelu"), 1e-7 + 0 * v)
+
+
+@pytest.mark.parametrize("M,N,K", [(2600, 264, 4096), (300, 136, 264)])
+def test_gelu_gradient_does_not_depend_on_the_rows_around(M, N, K):
+    """The main loop's blocks look GELU and its slope up where all of a wave's groups have a listed step and compute it
+    otherwise: a row of another magnitude among sixteen changes the way the others are done, and none of their bits."""
+    dy, w = rnd(M, N, dtype=torch.bfloat16), rnd(N, K, dtype=torch.bfloat16, scale=N ** -0.5)
+    u = 1.5 * rnd(M, K)
+    mixed = u.clone()
+    mixed[5::16] *= 1e-6
+    rest = torch.arange(M, device="cuda") % 16 != 5
+    one = T.linear_backward_input(dy, w, "gelu", T.pack8(u), out_dtype=torch.float32, want_activation=True)
+    two = T.linear_backward_input(dy, w, "gelu", T.pack8(mixed), out_dtype=torch.float32, want_activation=True)
+    for a, b in zip(one, two):
+        assert torch.equal(a[rest], b[rest]) and not torch.equal(a, b)
