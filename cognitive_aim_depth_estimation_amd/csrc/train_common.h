@@ -110,8 +110,6 @@ __device__ __forceinline__ void store_one(void* p, int dt, size_t off, float y) 
   else reinterpret_cast<unsigned short*>(p)[off] = (unsigned short)bits16(y, dt);
 }
 
-// Sum over the 64 lanes, result in every lane, without the LDS permute path: rotations inside rows of 16 lanes (DPP), then
-// the two row-swap instructions of gfx950.
 // An operand times a vector of scales, rounded to fp16: a LayerScale of 1e-5 would push it into fp16's subnormals (0.02 times
 // that keeps two bits).  So the scales are multiplied by a power of two that brings the largest into [0.5, 1), and the
 // sums by its reciprocal, both exact.  `top`: the largest magnitude's bits; infinities, NaN and all zeros: no change.
@@ -137,6 +135,8 @@ __device__ __forceinline__ unsigned wave_top(const float* s, int n, int from, in
   }
   return top;
 }
+// Sum over the 64 lanes, result in every lane, without the LDS permute path: rotations inside rows of 16 lanes (DPP), then
+// the two row-swap instructions of gfx950.
 __device__ __forceinline__ float wave_sum_dpp(float v) {
 #define TRAIN_ROR(ctrl_) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl_, 0xf, 0xf, false))
   v += TRAIN_ROR(0x128);   // row_ror:8

@@ -612,7 +612,8 @@ unsigned blocks_for(unsigned long long threads) {
 }
 constexpr int LN_MAX_D = 16384;
 constexpr int MAX_D = 1 << 30;             // column arithmetic in 32 bits
-// blocks of the backward kernel: 16 waves a CU keep enough rows in flight; each leaves a partial row of 2 D floats
+// blocks of the backward kernel: up to 4096 columns the 768 of four waves that are resident (12 waves a CU); wider rows take
+// sixteen waves a block, in whole rounds of 256 units.  Each block leaves a partial row of 2 D floats.
 int ln_bwd_blocks(int M, int D) {
   const int rpb = D <= 1024 ? 4 : 1, most = D <= 8192 ? 768 : 512;
   const long long want = ((long long)M + rpb - 1) / rpb;
@@ -716,7 +717,7 @@ int cogaim_layernorm_train_fwd(const void* x, int x_dtype, long long ldx, const 
 
 long long cogaim_layernorm_bwd_workspace_bytes(int M, int D) {
   if (M <= 0 || D <= 0 || D > LN_MAX_D) return COGAIM_EINVAL;
-  return (long long)1024 * 2 * D * 4 < (long long)M * 2 * D * 4 ? (long long)1024 * 2 * D * 4 : (long long)M * 2 * D * 4;
+  return (long long)ln_bwd_blocks(M, D) * 2 * D * 4;                    // partial rows
 }
 
 int cogaim_layernorm_bwd(const void* dy, int dy_dtype, long long lddy, const void* x, int x_dtype, long long ldx,

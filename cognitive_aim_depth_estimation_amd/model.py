@@ -1320,9 +1320,9 @@ class CognitiveAimModel(nn.Module):
             return [tuple(t) for t in temp_projection]
         return [tuple(temp_projection)] * K
 
-    # training-only helpers of the reference that callers may probe for
+    # training-only helper of the reference that callers may probe for
     def compute_curiosity_loss(self, *a, **k):
-        raise NotImplementedError("training is out of scope for this build")
+        raise NotImplementedError("the reference's training losses are not built (encoder_mlp and training.py are what fine-tuning has)")
 
     def get_exploration_stats(self):
         """Statistics of the positive entries of the exploration ring buffer (reference src/model.py:775-793, :1456-1460).

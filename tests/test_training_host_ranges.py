@@ -51,3 +51,9 @@ def test_pre_activation_descriptor():
     size = lambda **k: raw("cogaim_linear_fwd_workspace_bytes", C.byref(_lib.LinearFwdDesc(**d, **k)))  # noqa: E731
     assert size(extended=1, pre=P) >= 0 and size(extended=1, pre=P + 1) == -22
     assert size(extended=0, pre=P + 1) >= 0            # a shorter descriptor has no such field
+
+
+def test_layer_norm_backward_workspace_is_its_partial_rows():
+    size = lambda M, D: raw("cogaim_layernorm_bwd_workspace_bytes", M, D)  # noqa: E731
+    assert size(1, 8) == 2 * 8 * 4 and size(4, 768) == 2 * 768 * 4 and size(5, 768) == 2 * 2 * 768 * 4
+    assert size(10 ** 6, 768) == 768 * 2 * 768 * 4 and size(10 ** 6, 16384) == 512 * 2 * 16384 * 4 and size(100, 4096) == 100 * 2 * 4096 * 4
