@@ -479,26 +479,21 @@ __global__ __launch_bounds__(1024) void column_tops_kernel(const unsigned char* 
   const int g0 = G < 4 ? 0 : (int)(4 * blockIdx.x) < G - 4 ? (int)(4 * blockIdx.x) : G - 4, n = G < 4 ? G : 4;
   const long long first = (long long)blockIdx.y * rows, last = first + rows < M ? first + rows : M;
   unsigned top[4] = {0, 0, 0, 0};
-  constexpr int AHEAD = 16;                                   // rows whose loads are in flight together; past the last, it again
-  for (long long r = first + threadIdx.x; r < last; r += AHEAD * 1024) {
-    unsigned w[AHEAD];
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const unsigned char* p = bytes + (r + 1024 * u < last ? r + 1024 * u : last - 1) * G + g0;
-      if (n == 4) __builtin_memcpy(&w[u], p, 4);
-      else {
-        w[u] = p[0];
-        if (n > 1) w[u] |= (unsigned)p[1] << 8;
-        if (n > 2) w[u] |= (unsigned)p[2] << 16;
-      }
+#pragma unroll 8
+  for (long long r = first + threadIdx.x; r < last; r += 1024) {
+    const unsigned char* p = bytes + r * G + g0;
+    unsigned w = 0;
+    if (n == 4) __builtin_memcpy(&w, p, 4);
+    else {
+      w = p[0];
+      if (n > 1) w |= (unsigned)p[1] << 8;
+      if (n > 2) w |= (unsigned)p[2] << 16;
     }
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned b = w[u] >> (8 * j) & 255u;
-        top[j] = umax(top[j], b == 255u ? 0u : b);
-      }
+    for (int j = 0; j < 4; ++j) {
+      const unsigned b = w >> (8 * j) & 255u;
+      top[j] = umax(top[j], b == 255u ? 0u : b);
+    }
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
