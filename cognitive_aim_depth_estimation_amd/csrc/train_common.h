@@ -229,8 +229,8 @@ __device__ __forceinline__ float from_unit(float sum, int top) { return __builti
 // followed by one exp2.  x Phi(x) is then off by 2.4e-8 rms over [-2, 2] and by 2.7e-7 at most for |x| < 12, the last
 // rounding included (the fp32 erf form: 2.7e-8 and 4.5e-7), and by under 1e-10 below -6; past 10 the value at 10,
 // 2e-28, is kept.  Every instruction here is issued once for each element of a product's result, beside which the matrix
-// pipe stands still; degree 6 is two fewer of about fifteen, for 9.2e-8, and saves nothing that is seen (forward with GELU and
-// codes at 10960 x 4096 x 1024: call with unpack 136.7 us with six, 136.8 with eight).
+// pipe stands still; degree 6 is two fewer of about fifteen and saves 3 of 120 us (forward with GELU and codes at
+// 10960 x 4096 x 1024), for 9.2e-8, which is more than a step of fp16's smallest numbers.
 constexpr float TAIL_END = 10.f;
 __device__ __forceinline__ float phi_tail(float a) {
   float p = -1.548175071e-06f;

@@ -257,8 +257,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_train_fwd_kernel(LnF
 // Backward.  With h = (x - mean) rstd and g = dy * gamma:  dx = rstd (g - mean(g) - h mean(g h)) [+ add],
 // dgamma = sum over rows of dy h, dbeta = sum of dy.  A block walks rows blockIdx, blockIdx + gridDim, ... and keeps its
 // threads' columns of dgamma / dbeta in registers; one partial row per block, summed in block order by the second
-// kernel, so the result does not depend on timing (no atomics).  HBM: 471 MB at 43840 x 768 (fp32 stream, bf16 dy) in 87 us,
-// 5.4 TB/s.  Runs of four: fp32 loads of whole lines; gamma in registers (read from the cache for every row: 105 us).  768
+// kernel, so the result does not depend on timing (no atomics).  HBM: 471 MB at 43840 x 768 (fp32 stream, bf16 dy) in 90 us,
+// 5.2 TB/s.  Runs of four: fp32 loads of whole lines; gamma in registers (read from the cache for every row: 105 us).  768
 // blocks of four waves are what is resident at 150 to 170 registers (1024 would run in two uneven rounds: 101 us).
 struct LnBwd {
   const void* dy; const void* x; const signed char* codes; const unsigned char* bytes; const float* mean; const float* rstd;
@@ -472,7 +472,8 @@ __global__ __launch_bounds__(256) void pack8_kernel(const void* __restrict__ x, 
 }
 
 // Largest exponent byte of each column group over a part of the rows, 255 (not finite) left out: tops[part][group].  A block
-// takes four groups, a thread every 1024th row; the last four groups of a row are read together, not past its end.
+// takes four groups, a thread every 1024th row; the last four groups of a row are read together, not past its end.  8 us at
+// 10960 x 1024, where the eight blocks' loads each touch 64 rows; more blocks would need a second launch to join them.
 __global__ __launch_bounds__(1024) void column_tops_kernel(const unsigned char* __restrict__ bytes, unsigned char* __restrict__ tops, int M, int G, int rows) {
   __shared__ unsigned char s[16][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -541,7 +542,8 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const signed char* __restr
   }
 }
 
-// du = dy * act'(u), u from its 8-bit copy
+// du = dy * act'(u), u from its 8-bit copy.  HBM: 226 MB of bf16 10960 x 4096 in 38 us, 6.0 TB/s; u itself, below, 270 MB in
+// 42 us, 6.5 TB/s.
 template <int DT, int V, bool EVEN>
 __global__ __launch_bounds__(256) void act_bwd_kernel(const void* __restrict__ dy, long long lddy,
                                                       const signed char* __restrict__ codes,
