@@ -472,15 +472,14 @@ __global__ __launch_bounds__(256) void pack8_kernel(const void* __restrict__ x, 
 }
 
 // Largest exponent byte of each column group over a part of the rows, 255 (not finite) left out: tops[part][group].  A block
-// takes four groups, a thread every 1024th row; the last four groups of a row are read together, not past its end.  8 us at
-// 10960 x 1024, where the eight blocks' loads each touch 64 rows; more blocks would need a second launch to join them.
+// takes four groups, a thread every 1024th row of its part; the last four groups of a row are read together, not past its end.
 __global__ __launch_bounds__(1024) void column_tops_kernel(const unsigned char* __restrict__ bytes, unsigned char* __restrict__ tops, int M, int G, int rows) {
   __shared__ unsigned char s[16][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g0 = G < 4 ? 0 : (int)(4 * blockIdx.x) < G - 4 ? (int)(4 * blockIdx.x) : G - 4, n = G < 4 ? G : 4;
   const long long first = (long long)blockIdx.y * rows, last = first + rows < M ? first + rows : M;
   unsigned top[4] = {0, 0, 0, 0};
-#pragma unroll 8
+#pragma unroll 4
   for (long long r = first + threadIdx.x; r < last; r += 1024) {
     const unsigned char* p = bytes + r * G + g0;
     unsigned w = 0;
@@ -510,16 +509,48 @@ __global__ __launch_bounds__(1024) void column_tops_kernel(const unsigned char* 
     tops[(size_t)blockIdx.y * G + g0 + threadIdx.x] = (unsigned char)t;
   }
 }
-// rows of a part, at most 1024 parts (more than one: a second launch over the parts)
-int tops_rows(int M) { return M <= 16384 * 1024 ? 16384 : (int)((M + 1023LL) / 1024); }
-int tops_parts(int M) { return (int)((M + tops_rows(M) - 1LL) / tops_rows(M)); }
+// The unpacking kernel joins the parts itself, and its first block leaves the result in memory for the sums: with few rows a
+// block joins the exponents of all of them in LDS and there is no other launch, with more a thread joins the eight parts
+// of its run's group.  (One part of 16384 rows: 10960 x 1024 x 1024 55 us, 7 x 768 x 768 14.5.)
+constexpr int UNITS_G = 2048, UNITS_BYTES = 4096, UNITS_PARTS = 8;       // groups and exponents that a block joins; parts
+struct Units { const unsigned char* part; int parts; bool rows; unsigned char* tops; };      // rows: the parts are the rows' exponents
+__device__ __forceinline__ unsigned joined_top(const Units& u, int G, int g) {
+  unsigned t = 0;
+#pragma unroll
+  for (int p = 0; p < UNITS_PARTS; ++p) t = umax(t, u.part[(size_t)(p < u.parts ? p : u.parts - 1) * G + g]);
+  return t;
+}
 
-// codes [M, D] -> out [M, width >= D] (columns past D are written as zero); tops, or null: in units (fp16)
-template <int DT, int V, bool EVEN>
+// codes [M, D] -> out [M, width >= D] (columns past D are written as zero); UNITS: in units (fp16)
+template <int DT, int V, bool EVEN, bool UNITS = false>
 __global__ __launch_bounds__(256) void unpack8_kernel(const signed char* __restrict__ codes,
                                                       const unsigned char* __restrict__ bytes, void* __restrict__ out,
-                                                      long long ldo, int M, int D, int width, const unsigned char* __restrict__ tops) {
+                                                      long long ldo, int M, int D, int width, Units units) {
   const long long groups = groups_of(D);
+  __shared__ unsigned top[UNITS ? UNITS_G : 1];
+  if constexpr (UNITS) {
+    const int G = (int)groups;
+    if (units.rows) {
+      int wide = 1;                                             // lanes across the groups, a power of two
+      while (wide < G && wide < 256) wide *= 2;
+      for (int g = threadIdx.x; g < G; g += 256) top[g] = 0;
+      __syncthreads();
+      for (int g = threadIdx.x & (wide - 1); g < G; g += wide) {
+        unsigned t = 0;
+#pragma unroll 8
+        for (int p = threadIdx.x / wide; p < units.parts; p += 256 / wide) {
+          const unsigned b = units.part[(size_t)p * G + g];
+          t = umax(t, b == 255u ? 0u : b);
+        }
+        atomicMax(&top[g], t);                                  // in LDS; a maximum has no order
+      }
+      __syncthreads();
+      if (blockIdx.x == 0)
+        for (int g = threadIdx.x; g < G; g += 256) units.tops[g] = (unsigned char)top[g];
+    } else if (blockIdx.x == 0) {
+      for (int g = threadIdx.x; g < G; g += 256) units.tops[g] = (unsigned char)joined_top(units, G, g);
+    }
+  }
   for (Walk w((unsigned)(width + V - 1) / V); w.row < (unsigned long long)M; w.step()) {
     const long long row = (long long)w.row;
     const int c = (int)w.run * V;
@@ -530,7 +561,7 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const signed char* __restr
       const Codes<V> q = EVEN || row + V <= M ? load_codes<V, true>(codes + row * D, c, D) : load_codes<V, false>(codes + row * D, c, D);
       float u[V];
       unsigned byte = bytes[row * groups + c / GROUP];
-      if (DT == DT_FP16 && tops) byte = unit_byte(byte, tops[c / GROUP]);
+      if constexpr (UNITS) byte = unit_byte(byte, units.rows ? top[c / GROUP] : joined_top(units, (int)groups, c / GROUP));
       decode_run<V>(q, group_step(byte), u);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -688,15 +719,19 @@ template <int DYT> void run_ln_bwd_from(const LnBwd& a, int x_dt, int blocks, hi
   } while (0)
 
 namespace train {
-long long tops_bytes(int M, int D) { return ((tops_parts(M) > 1 ? tops_parts(M) : 0) + 1LL) * groups_of(D); }
+long long tops_bytes(int, int D) { return (UNITS_PARTS + 1LL) * groups_of(D); }
 
 int unpack8_units(const void* codes, const void* exponents, unsigned char* tops, void* out, int M, int D, int width, hipStream_t st) {
-  const int G = (int)groups_of(D), parts = tops_parts(M);
-  unsigned char* const first = parts > 1 ? tops + G : tops;
-  hipLaunchKernelGGL(column_tops_kernel, dim3((G + 3) / 4, parts), dim3(1024), 0, st, (const unsigned char*)exponents, first, M, G, tops_rows(M));
-  if (parts > 1) hipLaunchKernelGGL(column_tops_kernel, dim3((G + 3) / 4), dim3(1024), 0, st, (const unsigned char*)first, tops, parts, G, parts);
-  BY_EVEN(DT_FP16, 8, (D | width), unpack8_kernel, dim3(blocks_for((unsigned long long)M * (width / 8LL + 1))), dim3(256), 0, st, (const signed char*)codes,
-          (const unsigned char*)exponents, out, (long long)width, M, D, width, (const unsigned char*)tops);
+  const int G = (int)groups_of(D);
+  Units u{(const unsigned char*)exponents, M, true, tops};
+  if (G > UNITS_G || (long long)M * G > UNITS_BYTES) {
+    const int rows = (int)((M + UNITS_PARTS - 1LL) / UNITS_PARTS);
+    u = Units{tops + G, (int)((M + rows - 1LL) / rows), false, tops};
+    hipLaunchKernelGGL(column_tops_kernel, dim3((G + 3) / 4, u.parts), dim3(1024), 0, st, (const unsigned char*)exponents, tops + G, M, G, rows);
+  }
+  const dim3 grid(blocks_for((unsigned long long)M * (width / 8LL + 1)));
+  if ((D | width) % 8 == 0) hipLaunchKernelGGL((unpack8_kernel<DT_FP16, 8, true, true>), grid, dim3(256), 0, st, (const signed char*)codes, (const unsigned char*)exponents, out, (long long)width, M, D, width, u);
+  else hipLaunchKernelGGL((unpack8_kernel<DT_FP16, 8, false, true>), grid, dim3(256), 0, st, (const signed char*)codes, (const unsigned char*)exponents, out, (long long)width, M, D, width, u);
   return COGAIM_LAUNCH_CHECK();
 }
 }  // namespace train
@@ -766,7 +801,7 @@ int cogaim_unpack8(const void* codes, const void* exponents, void* out, int out_
       !aligned(out, dt_size(out_dtype)))
     return COGAIM_EINVAL;
   BY_TYPE(out_dtype, (D | width), unpack8_kernel, dim3(blocks_for((unsigned long long)M * (width / (out_dtype == DT_FP32 ? 4LL : 8LL) + 1))), dim3(256), 0, (hipStream_t)stream,
-          (const signed char*)codes, (const unsigned char*)exponents, out, ldo, M, D, width, (const unsigned char*)nullptr);
+          (const signed char*)codes, (const unsigned char*)exponents, out, ldo, M, D, width, Units{});
   return COGAIM_LAUNCH_CHECK();
 }
 

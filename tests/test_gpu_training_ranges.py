@@ -349,3 +349,17 @@ def test_gelu_gradient_does_not_depend_on_the_rows_around(M, N, K):
     two = T.linear_backward_input(dy, w, "gelu", T.pack8(mixed), out_dtype=torch.float32, want_activation=True)
     for a, b in zip(one, two):
         assert torch.equal(a[rest], b[rest]) and not torch.equal(a, b)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 8, 70016), (3, 5, 65700), (9, 16, 66000), (300, 8, 4129)])
+def test_linear_backward_weight_fp16_wide(M, N, K):
+    """More column groups than a block joins in LDS, and rows whose parts are not all there."""
+    t = torch.float16
+    size = torch.exp2(torch.randint(-60, 60, (1, -(-K // 32)), device="cuda").float()).repeat_interleave(32, 1)[:, :K]
+    saved = T.pack8(rnd(M, K) * size)
+    v, dy = decode(saved.codes, saved.exponents), rnd(M, N, dtype=t)
+    dW, db, _ = T.linear_backward_weight(dy, saved)
+    d = dy.double()
+    bound = (M + 8) * 2 * U32 * (d.abs().t() @ v.abs()) + d.abs().sum(0)[:, None] * steps(saved.exponents, K).amax(0) * 2.0 ** -34
+    within(dW, d.t() @ v, bound + least(torch.float32), "dW")
+    within(db, d.sum(0), (M + 8) * 2 * U32 * d.abs().sum(0), "db")
