@@ -607,7 +607,8 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const void* __restrict__ d
   }
 }
 
-// the same with u itself, of a type known at run time
+// the same with u itself, of a type known at run time; an infinite one (a pre-activation past fp16's range) has the slope's
+// limit, 1 or 0
 template <int DT, int V, bool EVEN>
 __global__ __launch_bounds__(256) void act_bwd_from_kernel(const void* __restrict__ dy, long long lddy, const void* __restrict__ u, int u_dt, long long ldu,
                                                            void* __restrict__ du, int du_dt, long long lddu, int act, int M, int D) {
@@ -629,7 +630,7 @@ __global__ __launch_bounds__(256) void act_bwd_from_kernel(const void* __restric
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float value, slope;
-      if (act == ACT_GELU) gelu_both(v[j], value, slope);
+      if (act == ACT_GELU) gelu_both(fabsf(v[j]) == __builtin_inff() ? __builtin_copysignf(100.f, v[j]) : v[j], value, slope);
       else slope = relu_slope(v[j]);
       g[j] *= slope;
     }

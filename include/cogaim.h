@@ -353,7 +353,7 @@ int cogaim_unpack8(const void* codes, const void* exponents, void* out, int out_
 int cogaim_activation_bwd(const void* dy, int dy_dtype, long long lddy, const void* codes, const void* exponents, void* du,
                           int du_dtype, long long lddu, int activation, int M, int D, void* stream);
 
-/* The same with u [M, D] itself, of its own type. */
+/* The same with u [M, D] itself, of its own type (an infinite u has the slope's limit). */
 int cogaim_activation_bwd_from(const void* dy, int dy_dtype, long long lddy, const void* u, int u_dtype, long long ldu, void* du,
                                int du_dtype, long long lddu, int activation, int M, int D, void* stream);
 

@@ -363,3 +363,23 @@ def test_linear_backward_weight_fp16_wide(M, N, K):
     bound = (M + 8) * 2 * U32 * (d.abs().t() @ v.abs()) + d.abs().sum(0)[:, None] * steps(saved.exponents, K).amax(0) * 2.0 ** -34
     within(dW, d.t() @ v, bound + least(torch.float32), "dW")
     within(db, d.sum(0), (M + 8) * 2 * U32 * d.abs().sum(0), "db")
+
+
+@pytest.mark.parametrize("M", [3, 80])
+@pytest.mark.parametrize("name", ["relu", "gelu"])
+def test_linear_pre_activation_past_fp16(M, name):
+    """A pre-activation that fp16 cannot hold, kept as an infinity, has the gradient of the finite fp32 result: all or none."""
+    x = torch.full((M, 8), 300.0, device="cuda", dtype=torch.float16)
+    x[1] = -300.0
+    x.requires_grad_()
+    w = torch.full((16, 8), 250.0, device="cuda", dtype=torch.float16).requires_grad_()
+    y = T.linear(x, w, None, name, out_dtype=torch.float32)
+    want = torch.full((M, 16), 600000.0, device="cuda")
+    want[1] = 0
+    assert float((y.detach() - want).abs().max()) <= 2e-28          # what is left of GELU below -10
+    dx, dw = torch.autograd.grad(y, (x, w), torch.full_like(y, 0.125))
+    ok = torch.full((M, 8), 500.0, device="cuda", dtype=torch.float16)
+    ok[1] = 0
+    assert torch.equal(dx, ok) and torch.equal(dw, torch.full_like(w, 37.5 * (M - 1)))
+    u = torch.tensor([[float("inf"), -float("inf"), float("nan")]], device="cuda")
+    assert T.activation_backward(torch.full((1, 3), 2.0, device="cuda"), u, name).nan_to_num(7.0).tolist() == [[2.0, 0.0, 7.0]]
